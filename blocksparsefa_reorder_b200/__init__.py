@@ -29,8 +29,13 @@ The CUDA kernels live in ``_lib/libbsattn_b200.so`` (built by
 from ._lib import BsaError
 from .api import (BlockSparsePlan, block_sparse_attention, block_sparse_attention_autograd,
                   block_sparse_attention_backward, infer_block, inverse_permutation, permute_rows, transposed_plan)
+from .dense import (cross_attention, cross_attention_autograd, cross_attention_backward,
+                    shared_prefix_attention)
+from .rope import qk_norm_rope, qk_norm_rope_autograd, qk_norm_rope_backward, rope_table
 
 __all__ = ["BsaError", "BlockSparsePlan", "block_sparse_attention", "block_sparse_attention_autograd",
-           "block_sparse_attention_backward", "infer_block", "inverse_permutation", "permute_rows",
+           "block_sparse_attention_backward", "cross_attention", "cross_attention_autograd",
+           "cross_attention_backward", "infer_block", "inverse_permutation", "permute_rows",
+           "qk_norm_rope", "qk_norm_rope_autograd", "qk_norm_rope_backward", "rope_table", "shared_prefix_attention",
            "transposed_plan"]
 __version__ = "0.1.0"

@@ -262,3 +262,64 @@ extern "C" int bsa_fwd_reordered(const bsa_fwd_args* a, const void* q_perm, cons
   }
   return BSA_OK;
 }
+
+extern "C" int bsa_qk_norm_rope(const bsa_rope_args* a, void* stream) {
+  int rc = rope_validate(a, false);
+  if (rc) return rc;
+  if ((rc = check_device())) return rc;
+  return launch_rope_fwd(a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int bsa_qk_norm_rope_bwd_workspace_bytes(const bsa_rope_args* a, size_t* bytes) {
+  if (!bytes) return BSA_ERR_INVALID_ARG;
+  const int rc = rope_validate(a, true);
+  if (rc) return rc;
+  *bytes = a->dq_weight || a->dk_weight ? rope_bwd_workspace(a) : 0;
+  return BSA_OK;
+}
+
+extern "C" int bsa_qk_norm_rope_bwd(const bsa_rope_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = rope_validate(a, true);
+  if (rc) return rc;
+  if ((a->dq_weight || a->dk_weight) && (!workspace || workspace_bytes < rope_bwd_workspace(a)))
+    return BSA_ERR_WORKSPACE;
+  if ((rc = check_device())) return rc;
+  return launch_rope_bwd(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int bsa_cross_fwd_workspace_bytes(const bsa_cross_args* a, size_t* bytes) {
+  if (!bytes) return BSA_ERR_INVALID_ARG;
+  const int rc = cross_validate(a);
+  if (rc) return rc;
+  *bytes = cross_workspace(a);
+  return BSA_OK;
+}
+
+extern "C" int bsa_cross_fwd(const bsa_cross_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = cross_validate(a);
+  if (rc) return rc;
+  if ((rc = check_device())) return rc;
+  return launch_cross(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int bsa_cross_bwd(const bsa_cross_bwd_args* a, void* stream) {
+  int rc = cross_bwd_validate(a);
+  if (rc) return rc;
+  if ((rc = check_device())) return rc;
+  return launch_cross_bwd(a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int bsa_prefix_fwd_workspace_bytes(const bsa_prefix_args* a, size_t* bytes) {
+  if (!bytes) return BSA_ERR_INVALID_ARG;
+  const int rc = prefix_validate(a);
+  if (rc) return rc;
+  *bytes = prefix_workspace(a);
+  return BSA_OK;
+}
+
+extern "C" int bsa_prefix_fwd(const bsa_prefix_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = prefix_validate(a);
+  if (rc) return rc;
+  if ((rc = check_device())) return rc;
+  return launch_prefix(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}

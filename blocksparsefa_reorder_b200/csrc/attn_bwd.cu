@@ -71,15 +71,6 @@ struct BwdCfg {
   static constexpr int BAR_BYTES = 256;
 };
 
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-
 __device__ __forceinline__ void ew_bar_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // The 128x(D) accumulator in TMEM columns [col, col + D) of this thread's
@@ -575,6 +566,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
 }
 
+}  // namespace
+
+int launch_bwd_delta(const bsa_tensor4d& o, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
+                     bool bf16, cudaStream_t st) {
+  const int64_t rows = static_cast<int64_t>(B) * H * N;
+  const int64_t rows_per_block = 8 * (32 / (D / 8));
+  const unsigned grid = static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block);
+#define BSA_DELTA_CASE(BF_, D_)                                                                                     \
+  if (bf16 == BF_ && D == D_)                                                                                      \
+    bwd_delta_kernel<BF_, D_><<<grid, 256, 0, st>>>(                                                               \
+        static_cast<const uint8_t*>(o.data), o.stride_b, o.stride_h, o.stride_n,                                   \
+        static_cast<const uint8_t*>(dout.data), dout.stride_b, dout.stride_h, dout.stride_n, delta, B, H, N);
+  BSA_DELTA_CASE(true, 128)
+  BSA_DELTA_CASE(false, 128)
+  BSA_DELTA_CASE(true, 64)
+  BSA_DELTA_CASE(false, 64)
+#undef BSA_DELTA_CASE
+  BSA_CUDA_CHECK(cudaGetLastError());
+  return BSA_OK;
+}
+
+namespace {
+
 template <int D, int BN, bool BF16>
 int launch_bwd_t(const bsa_bwd_args* a, cudaStream_t st) {
   using C = BwdCfg<D, BN>;
@@ -604,13 +618,7 @@ int launch_bwd_t(const bsa_bwd_args* a, cudaStream_t st) {
   if ((r = make_tensor_map_4d(&mv_s, a->v, a->B, a->H, a->N, D, BF16, BN))) return r;
   if ((r = make_tensor_map_4d(&mdo_s, a->dout, a->B, a->H, a->N, D, BF16, BN))) return r;
 
-  const int64_t rows = static_cast<int64_t>(a->B) * a->H * a->N;
-  const int64_t rows_per_block = 8 * (32 / (D / 8));
-  bwd_delta_kernel<BF16, D><<<static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block), 256, 0, st>>>(
-      static_cast<const uint8_t*>(a->o.data), a->o.stride_b, a->o.stride_h, a->o.stride_n,
-      static_cast<const uint8_t*>(a->dout.data), a->dout.stride_b, a->dout.stride_h, a->dout.stride_n, a->delta,
-      a->B, a->H, a->N);
-  BSA_CUDA_CHECK(cudaGetLastError());
+  if ((r = launch_bwd_delta(a->o, a->dout, a->delta, a->B, a->H, a->N, D, BF16, st))) return r;
 
   BwdParams p{};
   p.H = a->H;

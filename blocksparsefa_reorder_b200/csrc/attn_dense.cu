@@ -1,0 +1,1065 @@
+// Attention over contiguous key ranges for sm_100a: cross attention (queries
+// of one length, keys of another, padded per sequence, key / value heads
+// shared by groups of query heads) and attention of a batch behind a shared
+// prefix.  bf16 / fp16, head dim 64 or 128.
+//
+//   o = sum_j p_j v_j / l,  p_j = 2^(s_j scale - m),  l = sum_j p_j,
+//   lse = m + log2 l,       s_j = q . k_j for the keys j the row may see
+//
+// A unit is one key / value head of one sequence, with the rows of every query
+// head that shares it; in the shared prefix one unit holds the rows of all
+// sequences, so that its keys are read once for the whole batch.  An item is
+// one row tile of a unit times one range of key tiles (128 keys each); items
+// are dealt to the persistent CTAs round robin.  Where few items would leave
+// SMs idle the host splits the keys, and partial results (normalised o in fp32
+// and its lse) are joined by attn_join_kernel:
+//   m = max_i lse_i,  w_i = 2^(lse_i - m),  o = sum w_i o_i / sum w_i.
+//
+// A CTA runs two streams, each with its own softmax warpgroup, S and O
+// columns in tensor memory:
+//  * rows above 128: stream s takes rows 128 s .. 128 s + 127 of a 256-row
+//    tile, and both read each K / V tile once from shared memory;
+//  * at most 128 rows: both streams hold the same rows, stream s takes the key
+//    tiles of parity s, and the epilogue joins the two.
+// While one stream's softmax runs, the tensor cores work for the other.
+// Per stream: S_i = Q K_i^T into TMEM, softmax (one row a thread) writes P_i as
+// 16-bit pairs over S_i, then O += P_i V_i, then S_i+1; so S_i+1 seen complete
+// means PV_i complete, and the softmax may rescale O and hand back the stages
+// of V_i and K_i+1 without any further commit.
+// Roles: warp 0 TMA producer; warp 1 issues tcgen05.mma; warps 2-3 gather
+// query rows of several heads (or sequences) into one tile where a head has
+// fewer than 128; warpgroups 1, 2 softmax of streams 0, 1; warpgroup 3 epilogue.
+//
+// Bound: 4 rows keys D flops against the tensor rate and, row by row, the 16
+// exponentials a clock of an SM (as many cycles as the products at D = 128);
+// with few rows the bytes of K and V.
+//
+// Keys behind a sequence's length take no part: their scores are replaced, and
+// their V rows are zeroed in shared memory (0 x NaN would reach O).
+// Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and all roles drain.
+#include <cudaTypedefs.h>
+
+#include <atomic>
+
+#include "common.cuh"
+#include "internal.h"
+#include "softmax.cuh"
+
+namespace bsa {
+
+namespace {
+
+constexpr int kThreadsD = 512;
+constexpr int kSmemLimitD = 232448;
+// setmaxnreg split: issue / two softmax / epilogue warpgroups, of a launch with 128 a thread
+constexpr int kRegsLaunchD = 128;
+constexpr int kRegsIssueD = 64;
+constexpr int kRegsSoftmaxD = 176;
+constexpr int kRegsEpilogueD = 96;
+constexpr int kRegsSplitD = kRegsIssueD + 2 * kRegsSoftmaxD + kRegsEpilogueD;
+static_assert(128 * kRegsSplitD <= kThreadsD * kRegsLaunchD, "register split");
+
+// One source of keys.  Row r of a unit is query (sequence, head, token):
+// with `seqs` sequences in a unit, r = (seq * G + g) * M + m.
+struct DensePart {
+  int units;       // seqs == 1: B * Hk, else Hk
+  int seqs;        // sequences whose rows one unit holds
+  int rows;        // seqs * G * M
+  int tiles;       // row tiles of a unit
+  int splits;      // key ranges
+  int chunk;       // key tiles of a range
+  int keys;        // keys the tensors hold
+  int items;       // units * tiles * splits
+  int shared_kv;   // the unit's K / V do not depend on the sequence
+  int kb_mul;      // 0: K / V batch stride 0 (one copy for the batch)
+  int vb_mul;
+  int causal;      // query m of M sees keys below len - (M - 1 - m)
+  const void* lens;  // [B] valid keys, or null (all)
+  float* part_o;   // partial results, or null: this part is the whole result
+  float* part_lse;
+};
+
+struct DenseParams {
+  DensePart part[2];
+  int nparts;
+  int B, H, Hk, G, M;
+  int lens_i64;
+  int packed;      // query rows gathered by warps 2-3 (fewer than 128 queries a head)
+  int dual;        // bit i: part i runs both streams over the same rows
+  const uint8_t* q;
+  int64_t qs_b, qs_h, qs_n;
+  uint8_t* o;
+  int64_t os_b, os_h, os_n;
+  float* lse;
+  float scale_log2;
+  int32_t* err;
+  uint64_t wait_ns;
+};
+
+template <int D>
+struct DenseCfg {
+  static constexpr int NCHUNK = D / 64;
+  static constexpr int CHUNK = 128 * 128;   // 64 columns of 128 rows, 128-byte swizzle
+  static constexpr int TILE = 128 * D * 2;
+  static constexpr int SLOTS = D == 128 ? 5 : 12;
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int STATS = 2 * 2 * 128 * 4;  // [stream][m, l][row]
+  static constexpr int SMEM = (2 + SLOTS) * TILE + BAR_BYTES + STATS;
+  static constexpr int O_COL = 256;  // S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [256+D, 256+2D)
+  static_assert(SMEM <= kSmemLimitD, "shared memory budget");
+  static_assert((2 * SLOTS + 18) * 8 + 8 <= BAR_BYTES, "barriers");
+};
+
+// One item as every role derives it from its number.
+struct Item {
+  int part, unit, tile, split;
+  int nk;       // key tiles to do
+  int k0;       // first key
+  int len;      // valid keys of the unit (all its sequences alike, but for causal rows)
+  int rows;     // rows of the tile: 1 .. 256 (dual: 1 .. 128)
+  int b, hk;    // K / V coordinates (b: of the only sequence)
+  int row0;     // packed: first row of the unit in the tile
+  int qb, qh, m0;  // not packed: the tile's query sequence, head and first token
+  bool dual;
+};
+
+__device__ __forceinline__ int clamp_len(const DenseParams& p, const DensePart& pt, int b) {
+  if (!pt.lens) return pt.keys;
+  const int64_t l = p.lens_i64 ? __ldg(static_cast<const int64_t*>(pt.lens) + b)
+                               : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(pt.lens) + b));
+  if (l < 0 || l > pt.keys) set_err(p.err, BSA_DEVERR_COORD);
+  return static_cast<int>(l < 0 ? 0 : l > pt.keys ? pt.keys : l);
+}
+
+__device__ __forceinline__ void get_item(const DenseParams& p, int w, Item& it) {
+  it.part = w >= p.part[0].items ? 1 : 0;
+  const DensePart& pt = p.part[it.part];
+  w -= it.part ? p.part[0].items : 0;
+  const int per_unit = pt.tiles * pt.splits;
+  it.unit = w / per_unit;
+  w -= it.unit * per_unit;
+  it.split = w / pt.tiles;  // neighbouring CTAs: the same keys, so K / V come from L2
+  it.tile = w - it.split * pt.tiles;
+  it.dual = (p.dual >> it.part) & 1;
+  if (pt.shared_kv) {
+    it.b = 0;
+    it.hk = it.unit;
+    it.len = pt.keys;
+  } else {
+    it.b = it.unit / p.Hk;
+    it.hk = it.unit - it.b * p.Hk;
+    it.len = clamp_len(p, pt, it.b);
+  }
+  it.k0 = it.split * pt.chunk * 128;
+  const int left = it.len - it.k0;
+  it.nk = left <= 0 ? 0 : min(pt.chunk, (left + 127) / 128);
+  const int per = it.dual ? 128 : 256;
+  if (p.packed) {
+    it.row0 = it.tile * per;
+    it.rows = min(per, pt.rows - it.row0);
+    it.qb = it.qh = it.m0 = 0;
+  } else {
+    const int mt = (p.M + per - 1) / per;
+    const int hh = it.tile / mt;  // seq * G + g
+    it.m0 = (it.tile - hh * mt) * per;
+    it.rows = min(per, p.M - it.m0);
+    const int sq = hh / p.G;
+    it.qb = pt.shared_kv ? sq : it.b;
+    it.qh = it.hk * p.G + (hh - sq * p.G);
+    it.row0 = hh * p.M + it.m0;
+  }
+}
+
+// (sequence, head, token) of row `r` of the unit.
+__device__ __forceinline__ void row_of(const DenseParams& p, const Item& it, int r, int& b, int& h, int& m) {
+  const int sg = r / p.M;
+  m = r - sg * p.M;
+  const int sq = sg / p.G;
+  h = it.hk * p.G + (sg - sq * p.G);
+  b = p.part[it.part].shared_kv ? sq : it.b;
+}
+
+// Stage positions of K_t and V_t in the item's sequence of 2 nk loads (the
+// order in which the MMA warp needs them).
+__device__ __forceinline__ int k_at(const Item& it, int t) { return it.dual ? (t ? 2 * t - 1 : 0) : 2 * t; }
+__device__ __forceinline__ int v_at(const Item& it, int t) {
+  return it.dual ? min(2 * t + 2, 2 * it.nk - 1) : 2 * t + 1;
+}
+// steps of stream s, and the key tile of its i-th step
+__device__ __forceinline__ int steps_of(const Item& it, int s) {
+  return it.dual ? (it.nk - s + 1) / 2 : (it.rows > 128 * s ? it.nk : 0);
+}
+__device__ __forceinline__ int tile_of(const Item& it, int s, int i) { return it.dual ? 2 * i + s : i; }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// The values loaded by tcgen05.ld may be used from here on: they pass through
+// the wait, so that no use of them can move ahead of it.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreadsD, 1)
+    attn_dense_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK0,
+                      const __grid_constant__ CUtensorMap tmV0, const __grid_constant__ CUtensorMap tmK1,
+                      const __grid_constant__ CUtensorMap tmV1, const __grid_constant__ DenseParams p) {
+  using C = DenseCfg<D>;
+  constexpr int SL = C::SLOTS;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) set_err(p.err, BSA_DEVERR_ALIGN);
+    return;
+  }
+  uint8_t* sQ = smem;                // [2][TILE]
+  uint8_t* sKV = sQ + 2 * C::TILE;   // [SLOTS][TILE]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SL * C::TILE);
+  float* stats = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + C::BAR_BYTES);
+  uint64_t* full = bars;                  // [SLOTS] tile landed
+  uint64_t* empty = full + SL;            // [SLOTS] its last reader completed
+  uint64_t* q_full = empty + SL;
+  uint64_t* q_empty = q_full + 1;         // the item's last S completed
+  uint64_t* s_full = q_empty + 1;         // [2] by stream
+  uint64_t* p_ready = s_full + 2;         // [2] 4 softmax warps wrote P
+  uint64_t* o_final = p_ready + 2;        // [2] the item's last PV completed
+  uint64_t* o_empty = o_final + 2;        // [2] 4 epilogue warps read O
+  uint64_t* stats_ready = o_empty + 2;    // [2] 4 softmax warps wrote (m, l)
+  uint64_t* stats_empty = stats_ready + 2;  // [2] 4 epilogue warps read them
+  uint64_t* drain = stats_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SL; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_full, p.packed ? 2 : 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 4);
+      mbar_init(&o_final[i], 1);
+      mbar_init(&o_empty[i], 4);
+      mbar_init(&stats_ready[i], 4);
+      mbar_init(&stats_empty[i], 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // set-up above touched this CTA's shared and tensor memory alone
+  grid_dependency_wait();
+
+  const int total = p.part[0].items + (p.nparts > 1 ? p.part[1].items : 0);
+  auto wait = [&](uint64_t* bar, int n) { return mbar_wait(bar, n & 1, abort_flag, p.err, p.wait_ns); };
+  auto wait_all = [&](uint64_t* bar, int n) { return __all_sync(0xffffffffu, wait(bar, n)) != 0; };
+
+  if (warp < 4) {
+    regs_dec<kRegsIssueD>();
+    if (warp == 0 && lane == 0) {
+      // ------------------------------------------------------------ producer
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK0);
+      tma_prefetch_desc(&tmV0);
+      int c = 0;      // loads so far
+      int nq = 0;     // non-empty items so far
+      bool ok = true;
+      for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+        Item it;
+        get_item(p, w, it);
+        if (it.nk == 0) continue;
+        const DensePart& pt = p.part[it.part];
+        const CUtensorMap* mk = it.part ? &tmK1 : &tmK0;
+        const CUtensorMap* mv = it.part ? &tmV1 : &tmV0;
+        auto load = [&](bool is_v, int t) {
+          const int st = c % SL;
+          if (c >= SL && !wait(&empty[st], c / SL - 1)) return false;
+          mbar_arrive_expect_tx(&full[st], C::TILE);
+          const int cb = it.b * (is_v ? pt.vb_mul : pt.kb_mul);
+          for (int ch = 0; ch < C::NCHUNK; ++ch)
+            tma_load_4d(sKV + st * C::TILE + ch * C::CHUNK, is_v ? mv : mk, &full[st], ch * 64, it.k0 + t * 128, it.hk,
+                        cb);
+          ++c;
+          return true;
+        };
+        if (!(ok = load(false, 0))) break;
+        if (it.dual && it.nk > 1 && !(ok = load(false, 1))) break;
+        if (!p.packed) {
+          if (nq > 0 && !(ok = wait(q_empty, nq - 1))) break;
+          const int nsub = it.rows > 128 ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, nsub * C::TILE);
+          for (int s = 0; s < nsub; ++s)
+            for (int ch = 0; ch < C::NCHUNK; ++ch)
+              tma_load_4d(sQ + s * C::TILE + ch * C::CHUNK, &tmQ, q_full, ch * 64, it.m0 + s * 128, it.qh, it.qb);
+        }
+        ++nq;
+        const int ahead = it.dual ? 2 : 1;
+        for (int t = 0; ok && t < it.nk; ++t) {
+          ok = load(true, t);
+          if (ok && t + ahead < it.nk) ok = load(false, t + ahead);
+        }
+      }
+      // the next kernel of the stream may set itself up
+      allow_dependents();
+      // every load issued lands before the CTA exits
+      for (int i = c > SL ? c - SL : 0; i < c; ++i) mbar_wait(&full[i % SL], (i / SL) & 1, nullptr, nullptr, p.wait_ns);
+      if (!p.packed && nq > 0) mbar_wait(q_full, (nq - 1) & 1, nullptr, nullptr, p.wait_ns);
+    } else if (warp == 1) {
+      // ------------------------------------------------- MMA issue (whole warp, lane 0 issues)
+      constexpr uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128, false, false);
+      constexpr uint32_t idesc_pv = make_idesc_f16(BF16, 128, D, false, true);
+      const uint32_t q_addr = smem_u32(sQ);
+      const uint32_t kv_addr = smem_u32(sKV);
+      int c0 = 0;           // loads of earlier items
+      int nq = 0;           // non-empty items so far
+      int np[2] = {0, 0};   // P tiles consumed, by stream
+      int no[2] = {0, 0};   // items whose O this stream wrote
+      bool ok = true;
+      for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+        Item it;
+        get_item(p, w, it);
+        if (it.nk == 0) continue;
+        const int n0 = steps_of(it, 0), n1 = steps_of(it, 1);
+        const int last_s = it.dual ? (it.nk - 1) & 1 : (n1 ? 1 : 0);  // stream of the item's last S and PV
+        auto issue_s = [&](int s, int i) {
+          const int at = c0 + k_at(it, tile_of(it, s, i)), st = at % SL;
+          if (!(ok = wait_all(&full[st], at / SL))) return;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t qa = q_addr + (it.dual ? 0 : s * C::TILE);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * C::CHUNK + (kk & 3) * 32;
+              tc_mma_ss(tmem + s * 128, make_sw128_desc(qa + off, 16, 1024),
+                        make_sw128_desc(kv_addr + st * C::TILE + off, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(&s_full[s]);
+            if (s == last_s && i == (s ? n1 : n0) - 1) tc_commit(q_empty);
+          }
+          __syncwarp();
+        };
+        auto issue_pv = [&](int s, int i) {
+          const int t = tile_of(it, s, i);
+          const int at = c0 + v_at(it, t), st = at % SL;
+          if (i == 0 && no[s] > 0 && !(ok = wait_all(&o_empty[s], no[s] - 1))) return;
+          if (!(ok = wait_all(&full[st], at / SL))) return;
+          const int tail = it.len - (it.k0 + t * 128);  // valid keys of this tile
+          if (tail < 128 && (it.dual || s == 0)) {
+            // V rows of keys past the length: zero (a row is 128 bytes of each chunk, whatever its swizzle)
+            uint8_t* vt = sKV + st * C::TILE;
+            for (int x = tail * 8 + lane; x < 128 * 8; x += 32) {
+#pragma unroll
+              for (int ch = 0; ch < C::NCHUNK; ++ch)
+                *reinterpret_cast<uint4*>(vt + ch * C::CHUNK + x * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (!(ok = wait_all(&p_ready[s], np[s]))) return;
+          ++np[s];
+          tc_fence_after();
+          const bool last = i == (s ? n1 : n0) - 1;
+          if (lane == 0) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              tc_mma_ts(tmem + C::O_COL + s * D, tmem + s * 128 + kk * 8,
+                        make_sw128_desc(kv_addr + st * C::TILE + kk * 16 * 128, C::CHUNK, 1024), idesc_pv,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+            if (last) {
+              tc_commit(&o_final[s]);
+              // no later S of this stream tells the softmax that V is free
+              if (it.dual || s == last_s) tc_commit(&empty[st]);
+            }
+          }
+          __syncwarp();
+          if (last) ++no[s];
+        };
+        if (!(ok = wait_all(q_full, nq))) break;
+        ++nq;
+        issue_s(0, 0);
+        if (ok && n1 > 0) issue_s(1, 0);
+        for (int i = 0; ok && i < n0; ++i) {
+          issue_pv(0, i);
+          if (ok && i + 1 < n0) issue_s(0, i + 1);
+          if (ok && i < n1) issue_pv(1, i);
+          if (ok && i + 1 < n1) issue_s(1, i + 1);
+        }
+        c0 += 2 * it.nk;
+      }
+      if (lane == 0) {
+        tc_commit(drain);
+        mbar_wait(drain, 0, nullptr, nullptr, p.wait_ns);
+      }
+      __syncwarp();
+    } else if (warp >= 2 && p.packed) {
+      // ------------------------------------------------------ query rows of several heads
+      int nq = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; w < total; w += gridDim.x) {
+        Item it;
+        get_item(p, w, it);
+        if (it.nk == 0) continue;
+        if (nq > 0) ok = ok && wait_all(q_empty, nq - 1);
+        ++nq;
+        if (!ok) continue;
+        // one 16-byte piece a lane: the D / 8 pieces of a row by neighbouring lanes
+        constexpr int PIECES = D / 8;
+        for (int x = (warp - 2) * 32 + lane; x < it.rows * PIECES; x += 64) {
+          const int r = x / PIECES, g = x - r * PIECES;
+          int b, h, m;
+          row_of(p, it, it.row0 + r, b, h, m);
+          const uint8_t* src = p.q + 2 * (b * p.qs_b + h * p.qs_h + m * p.qs_n + g * 8);
+          const int rr = r & 127;
+          cp_async16(smem_u32(sQ + (r >> 7) * C::TILE + (g >> 3) * C::CHUNK + rr * 128 + (((g & 7) ^ (rr & 7)) * 16)),
+                     src, 16);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+    }
+  } else if (warp < 12) {
+    regs_inc<kRegsSoftmaxD>();
+    // ---------------------------------------------------------------- softmax
+    const int s = (warp - 4) >> 2;  // stream
+    const int q4 = warp & 3;        // TMEM lane quarter
+    const int row = q4 * 32 + lane;
+    const uint32_t s_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + s * 128;
+    const uint32_t o_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + C::O_COL + s * D;
+    int c0 = 0;   // loads of earlier items
+    int ns = 0;   // S tiles of this stream so far
+    int ni = 0;   // items of this stream so far
+    bool ok = true;
+    for (int w = blockIdx.x; w < total; w += gridDim.x) {
+      Item it;
+      get_item(p, w, it);
+      if (it.nk == 0) continue;
+      const int n = steps_of(it, s);
+      if (n == 0) {
+        c0 += 2 * it.nk;
+        continue;
+      }
+      const bool releases = it.dual || it.rows <= 128 || s == 1;  // last reader of the shared tiles
+      const int r = it.dual ? row : s * 128 + row;
+      // a warp without rows only keeps the barriers going
+      const bool any_rows = (it.dual ? 0 : s * 128) + q4 * 32 < it.rows;
+      int limit = r < it.rows ? it.len : 0;  // keys this row sees
+      if (p.part[it.part].causal && r < it.rows) {
+        const int m = (it.row0 + r) % p.M;
+        limit = max(0, it.len - (p.M - 1 - m));
+      }
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int i = 0; i < n; ++i, ++ns) {
+        if (!(ok = ok && wait_all(&s_full[s], ns))) continue;
+        tc_fence_after();
+        const int t = tile_of(it, s, i);
+        if (q4 == 0 && lane == 0 && releases) {
+          // S_i complete, and with it the PV of the step before
+          mbar_arrive(&empty[(c0 + k_at(it, t)) % SL]);
+          if (i > 0) mbar_arrive(&empty[(c0 + v_at(it, tile_of(it, s, i - 1))) % SL]);
+        }
+        if (any_rows) {
+          const int valid = limit - (it.k0 + t * 128);  // keys of this tile the row sees
+          const bool mask = __any_sync(0xffffffffu, valid < 128);
+          auto load = [&](int ch, uint32_t (&v)[32]) {
+            tmem_ld32(s_base + ch * 32, v);
+            tmem_wait_ld32(v);
+            if (mask) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (ch * 32 + k >= valid) v[k] = __float_as_uint(-INFINITY);
+            }
+          };
+          auto tile_max = [&]() {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+              uint32_t v[32];
+              load(ch, v);
+              mx = fmaxf(mx, row_max<32>(v));
+            }
+            return mx * p.scale_log2;
+          };
+          uint32_t pr[64];
+          auto exps = [&]() {
+            // a row that has seen nothing yet keeps m = -inf: its exponentials are 2^(-inf - 0) = 0
+            const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+            float sum = 0.f;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+              uint32_t v[32], pp[16];
+              load(ch, v);
+              sum += exp_block<32, BF16>(v, pp, p.scale_log2, neg_m);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) pr[ch * 16 + k] = pp[k];
+            }
+            return sum;
+          };
+          // the reference point is the max of the row's first seen tile, and
+          // moves only when a tile's sum passes the slack (softmax.cuh)
+          if (__any_sync(0xffffffffu, m_run == -INFINITY && valid > 0)) {
+            const float mx = tile_max();
+            if (m_run == -INFINITY) m_run = mx;
+          }
+          float ls = exps();
+          if (__any_sync(0xffffffffu, !(ls <= ref_slack<BF16>()))) {
+            const float m_new = fmaxf(m_run, tile_max());
+            const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m_run - m_new);
+            l_run *= alpha;
+            m_run = m_new;
+            ls = exps();
+            if (i > 0) {
+#pragma unroll
+              for (int ch = 0; ch < D / 32; ++ch) {
+                uint32_t v[32];
+                tmem_ld32(o_base + ch * 32, v);
+                tmem_wait_ld32(v);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+                tmem_st32(o_base + ch * 32, v);
+              }
+            }
+          }
+          l_run += ls;
+          tmem_st32(s_base, pr);
+          tmem_st32(s_base + 32, pr + 32);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[s]);
+      }
+      if (ni > 0) ok = ok && wait_all(&stats_empty[s], ni - 1);
+      ++ni;
+      stats[s * 256 + row] = m_run;
+      stats[s * 256 + 128 + row] = l_run;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&stats_ready[s]);
+      c0 += 2 * it.nk;
+    }
+  } else {
+    regs_dec<kRegsEpilogueD>();
+    // --------------------------------------------------------------- epilogue
+    const int q4 = warp & 3;
+    const int row = q4 * 32 + lane;
+    const uint32_t o_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + C::O_COL;
+    int ni[2] = {0, 0};
+    bool ok = true;
+    for (int w = blockIdx.x; w < total; w += gridDim.x) {
+      Item it;
+      get_item(p, w, it);
+      const DensePart& pt = p.part[it.part];
+      const int nst = it.nk == 0 ? 0 : (steps_of(it, 1) > 0 ? 2 : 1);  // streams with an O
+      const int passes = it.dual || it.rows <= 128 ? 1 : 2;
+      for (int ps = 0; ps < passes; ++ps) {
+        // streams whose O make up this pass's rows: [first, last)
+        const int first = it.dual ? 0 : ps, last = it.nk == 0 ? first : (it.dual ? nst : ps + 1);
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int s = first; s < last; ++s) {
+          ok = ok && wait_all(&stats_ready[s], ni[s]);
+          if (ok) {
+            m[s - first] = stats[s * 256 + row];
+            l[s - first] = stats[s * 256 + 128 + row];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&stats_empty[s]);
+          ok = ok && wait_all(&o_final[s], ni[s]);
+          ++ni[s];
+        }
+        if (ok) tc_fence_after();
+        const int r = ps * 128 + row;
+        const bool store = ok && r < it.rows;
+        // weights of the streams' sums: 2^(m_s - max) / l, 0 for a stream without any key
+        const float mx = fmaxf(l[0] > 0.f ? m[0] : -INFINITY, l[1] > 0.f ? m[1] : -INFINITY);
+        float f0 = l[0] > 0.f ? ex2_approx(m[0] - mx) : 0.f;
+        float f1 = l[1] > 0.f ? ex2_approx(m[1] - mx) : 0.f;
+        const float lt = f0 * l[0] + f1 * l[1];
+        // (a sum that is NaN stays NaN: l > 0 is false only for 0 and NaN)
+        const bool nan = isnan(l[0]) || isnan(l[1]);
+        const float inv = nan ? NAN : (lt > 0.f ? 1.f / lt : 0.f);
+        f0 *= inv;
+        f1 *= inv;
+        const float lse = nan ? NAN : (lt > 0.f ? mx + log2f(lt) : -INFINITY);
+        int b = 0, h = 0, mm = 0;
+        row_of(p, it, it.row0 + (store ? r : 0), b, h, mm);
+        uint8_t* orow = p.o + 2 * (b * p.os_b + h * p.os_h + mm * p.os_n);
+        const int64_t slot = (static_cast<int64_t>(it.unit) * pt.rows + it.row0 + r) * pt.splits + it.split;
+        float* prow = pt.part_o ? pt.part_o + slot * D : nullptr;
+        if (it.nk > 0) {
+#pragma unroll
+          for (int ch = 0; ch < D / 32; ++ch) {
+            uint32_t v[32];
+            tmem_ld32(o_base + first * D + ch * 32, v);
+            tmem_wait_ld32(v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float x = __uint_as_float(v[k]);
+              v[k] = __float_as_uint(l[0] > 0.f || nan ? x * f0 : 0.f);
+            }
+            if (last - first == 2) {
+              uint32_t u[32];
+              tmem_ld32(o_base + D + ch * 32, u);
+              tmem_wait_ld32(u);
+              if (l[1] > 0.f) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  v[k] = __float_as_uint(fmaf(__uint_as_float(u[k]), f1, __uint_as_float(v[k])));
+              }
+            }
+            if (ch == D / 32 - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0)
+                for (int s = first; s < last; ++s) mbar_arrive(&o_empty[s]);
+            }
+            if (store) {
+              if (prow) {
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+                  reinterpret_cast<uint4*>(prow)[ch * 8 + g] =
+                      make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+              } else {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  uint4 x;
+                  x.x = pack2<BF16>(__uint_as_float(v[8 * g + 0]), __uint_as_float(v[8 * g + 1]));
+                  x.y = pack2<BF16>(__uint_as_float(v[8 * g + 2]), __uint_as_float(v[8 * g + 3]));
+                  x.z = pack2<BF16>(__uint_as_float(v[8 * g + 4]), __uint_as_float(v[8 * g + 5]));
+                  x.w = pack2<BF16>(__uint_as_float(v[8 * g + 6]), __uint_as_float(v[8 * g + 7]));
+                  reinterpret_cast<uint4*>(orow)[ch * 4 + g] = x;
+                }
+              }
+            }
+          }
+        } else if (store && !prow) {
+          // no key at all: o = 0 (a partial result is only its lse)
+#pragma unroll
+          for (int g = 0; g < D / 8; ++g) reinterpret_cast<uint4*>(orow)[g] = make_uint4(0, 0, 0, 0);
+        }
+        if (store) {
+          if (prow)
+            pt.part_lse[slot] = lse;
+          else if (p.lse)
+            p.lse[(static_cast<int64_t>(b) * p.H + h) * p.M + mm] = lse;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the partial results of an output row: one warp a row, D / 32 columns a
+// lane.  A partial result whose lse is -inf saw no key and its o is not read.
+// ---------------------------------------------------------------------------
+struct JoinSrc {
+  const float* o;
+  const float* lse;
+  int splits, rows, shared_kv;
+};
+struct JoinParams {
+  JoinSrc src[2];
+  int nsrc;
+  int B, H, Hk, G, M;
+  uint8_t* o;
+  int64_t os_b, os_h, os_n;
+  float* lse;
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attn_join_kernel(const JoinParams p) {
+  constexpr int V = D / 32;
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= static_cast<int64_t>(p.B) * p.H * p.M) return;
+  const int m = static_cast<int>(row % p.M);
+  const int64_t bh = row / p.M;
+  const int h = static_cast<int>(bh % p.H), b = static_cast<int>(bh / p.H);
+  const int hk = h / p.G, g = h - hk * p.G;
+  // the running max and sums over both sources
+  float mx = -INFINITY, sum = 0.f, acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const JoinSrc sr = p.src[s];
+    if (s >= p.nsrc) break;
+    const int64_t r = sr.shared_kv ? static_cast<int64_t>(hk) * sr.rows + (static_cast<int64_t>(b) * p.G + g) * p.M + m
+                                   : (static_cast<int64_t>(b) * p.Hk + hk) * sr.rows + g * p.M + m;
+    const float* ls = sr.lse + r * sr.splits;
+    const float* os = sr.o + r * sr.splits * D + lane * V;
+    for (int c = 0; c < sr.splits; c += 32) {
+      const int n = min(32, sr.splits - c);
+      const float mine = lane < n ? ls[c + lane] : -INFINITY;
+      float t = mine;
+      bool nan = isnan(mine);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
+      if (__any_sync(0xffffffffu, nan)) t = NAN;
+      if (t == -INFINITY) continue;
+      const float m_new = isnan(t) ? t : fmaxf(mx, t);
+      const float alpha = mx == -INFINITY ? 0.f : ex2_approx(mx - m_new);
+      mx = m_new;
+      sum *= alpha;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] *= alpha;
+      const float wt = mine == -INFINITY ? 0.f : ex2_approx(mine - mx);
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, wt, k);
+        if (wk == 0.f) continue;
+        sum += wk;
+        const float* src = os + static_cast<int64_t>(c + k) * D;
+        float x[V];
+        if constexpr (V == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(src);
+          x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+        } else {
+          const float2 f = *reinterpret_cast<const float2*>(src);
+          x[0] = f.x, x[1] = f.y;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(wk, x[i], acc[i]);
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint8_t* dst = p.o + 2 * (b * p.os_b + h * p.os_h + m * p.os_n + lane * V);
+  if constexpr (V == 4)
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
+  if (lane == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : mx + log2f(sum);
+}
+
+// ---------------------------------------------------------------------------
+// Host: splitting, workspace, launch.
+// ---------------------------------------------------------------------------
+constexpr int kSMs = 148;
+constexpr int kMaxSplits = 128;
+// An item's fixed cost in key tiles (query load, first scores, epilogue), and
+// what a second launch that joins costs, as measured (see the split rule).
+constexpr int kItemCost = 3;
+constexpr int kJoinCost = 3;
+
+size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct Shape {
+  int units, rows, tiles, keys;
+  bool dual;
+};
+
+// One source of keys for `seqs` sequences a unit.
+Shape shape_of(int B, int H, int Hk, int M, int keys, bool shared_kv) {
+  Shape s;
+  const int G = H / Hk, seqs = shared_kv ? B : 1;
+  s.units = shared_kv ? Hk : B * Hk;
+  s.rows = seqs * G * M;
+  const bool packed = M < 128;
+  const int64_t one = packed ? s.rows : M;  // rows that can share a tile
+  s.dual = one <= 128;
+  const int per = s.dual ? 128 : 256;
+  s.tiles = static_cast<int>(packed ? (one + per - 1) / per : static_cast<int64_t>(seqs) * G * ((M + per - 1) / per));
+  s.keys = keys;
+  return s;
+}
+
+// Key tiles of a range, the same for all sources: the smallest of
+//   ceil(cost of all items / SMs) (every SM busy) or the longest item,
+// over all range lengths, with the join's cost once anything is split.
+int choose_chunk(const Shape* s, int n) {
+  int longest = 1;
+  for (int i = 0; i < n; ++i) longest = longest > (s[i].keys + 127) / 128 ? longest : (s[i].keys + 127) / 128;
+  int best = longest;
+  double best_cost = 1e30;
+  for (int c = longest; c >= 1; --c) {
+    double items = 0, work = 0;
+    int most = 0;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int nk = (s[i].keys + 127) / 128;
+      const int splits = nk ? (nk + c - 1) / c : 1;
+      if (splits > kMaxSplits) ok = false;
+      const double per = static_cast<double>(s[i].units) * s[i].tiles;
+      // (a dual item does two key tiles at a time)
+      const double t = (s[i].dual ? (nk + 1) / 2 : nk) + static_cast<double>(splits) * kItemCost;
+      items += per * splits;
+      work += per * t;
+      const int one = (s[i].dual ? (c + 1) / 2 : c) + kItemCost;
+      if (nk && one > most) most = one;
+    }
+    if (!ok) break;
+    if (items > 2.0e9) break;
+    const double waves = static_cast<double>(static_cast<int64_t>((items + kSMs - 1) / kSMs));
+    double cost = work / kSMs;
+    // the last wave: whole items on part of the SMs
+    if (waves * most < 3.0 * cost && waves * most > cost) cost = waves * most;
+    if (cost < most) cost = most;
+    if (n > 1 || c < longest) cost += kJoinCost;
+    if (cost < best_cost * 0.999) best_cost = cost, best = c;
+  }
+  return best;
+}
+
+struct DenseCall {
+  int B, H, Hk, M, D, dtype;
+  bsa_tensor4d q, o;
+  int n;                      // sources
+  bsa_tensor4d k[2], v[2];
+  int keys[2];
+  bool shared_kv[2], causal[2];
+  const void* lens[2];
+  int lens_dtype;
+  float sm_scale;
+  float* lse;
+  int32_t* err;
+};
+
+// Layout of the workspace: per split source its partial o, then its lse.
+struct DensePlan {
+  Shape s[2];
+  int chunk, splits[2];
+  bool join;
+  size_t o_off[2], lse_off[2], total;
+};
+
+DensePlan plan_of(const DenseCall& c) {
+  DensePlan pl{};
+  for (int i = 0; i < c.n; ++i) pl.s[i] = shape_of(c.B, c.H, c.Hk, c.M, c.keys[i], c.shared_kv[i]);
+  pl.chunk = choose_chunk(pl.s, c.n);
+  for (int i = 0; i < c.n; ++i) {
+    const int nk = (c.keys[i] + 127) / 128;
+    pl.splits[i] = nk ? (nk + pl.chunk - 1) / pl.chunk : 1;
+  }
+  pl.join = c.n > 1 || pl.splits[0] > 1;
+  size_t off = 0;
+  for (int i = 0; pl.join && i < c.n; ++i) {
+    const size_t rows = static_cast<size_t>(pl.s[i].units) * pl.s[i].rows * pl.splits[i];
+    pl.o_off[i] = off;
+    off += round256(rows * c.D * sizeof(float));
+    pl.lse_off[i] = off;
+    off += round256(rows * sizeof(float));
+  }
+  pl.total = off;
+  return pl;
+}
+
+// A tensor map's batch dimension of 1 where the batch shares one copy.
+int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul) {
+  const bool one = B == 1 || t.stride_b == 0;
+  *mul = one ? 0 : 1;
+  // a dimension of length 1 has no stride of its own
+  if (one) t.stride_b = 8;
+  if (H == 1) t.stride_h = 8;
+  if (N == 1) t.stride_n = 8;
+  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, 128);
+}
+
+template <int D, bool BF16>
+int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_t st) {
+  using C = DenseCfg<D>;
+  auto kern = attn_dense_kernel<D, BF16>;
+  int dev = 0;
+  BSA_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return BSA_ERR_DEVICE;
+  static std::atomic<bool> ready[64] = {};
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    cudaFuncAttributes fa;
+    BSA_CUDA_CHECK(cudaFuncGetAttributes(&fa, kern));
+    // with fewer registers at launch the split's increases would never be granted
+    if (fa.numRegs * kThreadsD < 128 * kRegsSplitD) return BSA_ERR_UNSUPPORTED;
+    BSA_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  DenseParams p{};
+  CUtensorMap mq, mk[2], mv[2];
+  int r, unused;
+  const bool packed = c.M < 128;
+  // (gathered query rows need no map; the kernel then never reads it)
+  bsa_tensor4d q = c.q;
+  if (packed)
+    mq = CUtensorMap{};
+  else if ((r = map_of(&mq, q, c.B, c.H, c.M, D, BF16, &unused)))
+    return r;
+  p.nparts = c.n;
+  for (int i = 0; i < c.n; ++i) {
+    DensePart& pt = p.part[i];
+    const Shape& s = pl.s[i];
+    pt.units = s.units;
+    pt.seqs = c.shared_kv[i] ? c.B : 1;
+    pt.rows = s.rows;
+    pt.tiles = s.tiles;
+    pt.splits = pl.splits[i];
+    pt.chunk = pl.chunk;
+    pt.keys = c.keys[i];
+    pt.items = s.units * s.tiles * pl.splits[i];
+    pt.shared_kv = c.shared_kv[i];
+    pt.causal = c.causal[i];
+    pt.lens = c.lens[i];
+    if (pl.join) {
+      pt.part_o = reinterpret_cast<float*>(ws + pl.o_off[i]);
+      pt.part_lse = reinterpret_cast<float*>(ws + pl.lse_off[i]);
+    }
+    p.dual |= s.dual ? 1 << i : 0;
+    if (c.keys[i]) {
+      const int kb = c.shared_kv[i] ? 1 : c.B;
+      if ((r = map_of(&mk[i], c.k[i], kb, c.Hk, c.keys[i], D, BF16, &pt.kb_mul))) return r;
+      if ((r = map_of(&mv[i], c.v[i], kb, c.Hk, c.keys[i], D, BF16, &pt.vb_mul))) return r;
+    } else {
+      mk[i] = mv[i] = CUtensorMap{};  // no key tile is ever loaded
+    }
+  }
+  if (c.n == 1) mk[1] = mk[0], mv[1] = mv[0];
+  p.B = c.B, p.H = c.H, p.Hk = c.Hk, p.G = c.H / c.Hk, p.M = c.M;
+  p.lens_i64 = c.lens_dtype == BSA_INDEX_I64;
+  p.packed = packed;
+  p.q = static_cast<const uint8_t*>(c.q.data);
+  p.qs_b = c.q.stride_b, p.qs_h = c.q.stride_h, p.qs_n = c.q.stride_n;
+  p.o = static_cast<uint8_t*>(c.o.data);
+  p.os_b = c.o.stride_b, p.os_h = c.o.stride_h, p.os_n = c.o.stride_n;
+  p.lse = c.lse;
+  p.scale_log2 = c.sm_scale * 1.4426950408889634f;
+  p.err = c.err;
+  p.wait_ns = kWaitNs;
+  const int total = p.part[0].items + (c.n > 1 ? p.part[1].items : 0);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(total < kSMs ? total : kSMs);
+  cfg.blockDim = dim3(kThreadsD);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq, mk[0], mv[0], mk[1], mv[1], p));
+  if (!pl.join) return BSA_OK;
+  JoinParams j{};
+  j.nsrc = c.n;
+  for (int i = 0; i < c.n; ++i) {
+    j.src[i].o = p.part[i].part_o;
+    j.src[i].lse = p.part[i].part_lse;
+    j.src[i].splits = p.part[i].splits;
+    j.src[i].rows = p.part[i].rows;
+    j.src[i].shared_kv = p.part[i].shared_kv;
+  }
+  j.B = c.B, j.H = c.H, j.Hk = c.Hk, j.G = p.G, j.M = c.M;
+  j.o = p.o, j.os_b = p.os_b, j.os_h = p.os_h, j.os_n = p.os_n;
+  j.lse = c.lse;
+  const int64_t rows = static_cast<int64_t>(c.B) * c.H * c.M;
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16>, j));
+  return BSA_OK;
+}
+
+bool aligned(const bsa_tensor4d& t, int B, int H, int N) {
+  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && (B == 1 || t.stride_b * 2 % 16 == 0) &&
+         (H == 1 || t.stride_h * 2 % 16 == 0) && (N == 1 || t.stride_n * 2 % 16 == 0);
+}
+
+// Checks common to both operators; the sources' keys may be zero.
+int validate(const DenseCall& c) {
+  if (c.B <= 0 || c.H <= 0 || c.Hk <= 0 || c.M <= 0 || c.D <= 0) return BSA_ERR_INVALID_ARG;
+  if (c.dtype != BSA_DTYPE_F16 && c.dtype != BSA_DTYPE_BF16) return BSA_ERR_DTYPE;
+  if (c.H % c.Hk) return BSA_ERR_SHAPE;
+  if (c.D != 64 && c.D != 128) return BSA_ERR_UNSUPPORTED;
+  if (!(c.sm_scale > 0.f) || !(c.sm_scale < INFINITY)) return BSA_ERR_UNSUPPORTED;
+  if (!c.q.data || !c.o.data) return BSA_ERR_INVALID_ARG;
+  // row and item numbers are 32-bit
+  if (static_cast<int64_t>(c.B) * c.H * c.M > INT32_MAX / 2) return BSA_ERR_UNSUPPORTED;
+  if (!aligned(c.q, c.B, c.H, c.M) || !aligned(c.o, c.B, c.H, c.M)) return BSA_ERR_ALIGNMENT;
+  for (int i = 0; i < c.n; ++i) {
+    if (c.keys[i] < 0) return BSA_ERR_INVALID_ARG;
+    if (c.keys[i] > INT32_MAX - 65536) return BSA_ERR_UNSUPPORTED;
+    if (!c.keys[i]) continue;
+    if (!c.k[i].data || !c.v[i].data) return BSA_ERR_INVALID_ARG;
+    const int kb = c.shared_kv[i] ? 1 : c.B;
+    const bsa_tensor4d* ts[] = {&c.k[i], &c.v[i]};
+    for (const bsa_tensor4d* t : ts) {
+      if (t->stride_b < 0 || t->stride_h < 0 || t->stride_n < 0) return BSA_ERR_INVALID_ARG;
+      if (!aligned(*t, kb, c.Hk, c.keys[i])) return BSA_ERR_ALIGNMENT;
+    }
+    if (c.lens[i] && c.lens_dtype != BSA_INDEX_I32 && c.lens_dtype != BSA_INDEX_I64) return BSA_ERR_DTYPE;
+  }
+  return BSA_OK;
+}
+
+DenseCall call_of(const bsa_cross_args* a) {
+  DenseCall c{};
+  c.B = a->B, c.H = a->H, c.Hk = a->Hk, c.M = a->M, c.D = a->D, c.dtype = a->dtype;
+  c.q = a->q, c.o = a->o;
+  c.n = 1;
+  c.k[0] = a->k, c.v[0] = a->v, c.keys[0] = a->N;
+  c.lens[0] = a->k_lens, c.lens_dtype = a->lens_dtype;
+  c.sm_scale = a->sm_scale, c.lse = a->lse, c.err = a->err_flag;
+  return c;
+}
+
+DenseCall call_of(const bsa_prefix_args* a) {
+  DenseCall c{};
+  c.B = a->B, c.H = a->H, c.Hk = a->Hk, c.M = a->T, c.D = a->D, c.dtype = a->dtype;
+  c.q = a->q, c.o = a->o;
+  c.n = 2;
+  c.k[0] = a->k_prefix, c.v[0] = a->v_prefix, c.keys[0] = a->P, c.shared_kv[0] = true;
+  c.k[1] = a->k, c.v[1] = a->v, c.keys[1] = a->C, c.lens[1] = a->lens, c.causal[1] = a->T > 1;
+  c.lens_dtype = a->lens_dtype;
+  c.sm_scale = a->sm_scale, c.lse = a->lse, c.err = a->err_flag;
+  return c;
+}
+
+int run(const DenseCall& c, void* ws, size_t bytes, cudaStream_t st) {
+  const DensePlan pl = plan_of(c);
+  if (pl.total && (!ws || bytes < pl.total)) return BSA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return BSA_ERR_ALIGNMENT;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  const bool bf = c.dtype == BSA_DTYPE_BF16;
+  if (c.D == 128) return bf ? launch_dense<128, true>(c, pl, w, st) : launch_dense<128, false>(c, pl, w, st);
+  return bf ? launch_dense<64, true>(c, pl, w, st) : launch_dense<64, false>(c, pl, w, st);
+}
+
+}  // namespace
+
+int cross_validate(const bsa_cross_args* a) { return a ? validate(call_of(a)) : BSA_ERR_INVALID_ARG; }
+size_t cross_workspace(const bsa_cross_args* a) { return plan_of(call_of(a)).total; }
+int launch_cross(const bsa_cross_args* a, void* ws, size_t bytes, cudaStream_t st) {
+  return run(call_of(a), ws, bytes, st);
+}
+int prefix_validate(const bsa_prefix_args* a) { return a ? validate(call_of(a)) : BSA_ERR_INVALID_ARG; }
+size_t prefix_workspace(const bsa_prefix_args* a) { return plan_of(call_of(a)).total; }
+int launch_prefix(const bsa_prefix_args* a, void* ws, size_t bytes, cudaStream_t st) {
+  return run(call_of(a), ws, bytes, st);
+}
+
+}  // namespace bsa

@@ -1,0 +1,689 @@
+// Gradient of cross attention (attn_dense.cu) for sm_100a: bf16 / fp16, head
+// dim 64 or 128, key / value heads shared by groups of query heads, padded keys.
+//
+//   P = 2^(s scale_log2 - lse),  dP = dO V^T,  dS = P o (dP - Delta)
+//   dQ = sm_scale dS K,  dK = sm_scale sum_g dS^T Q,  dV = sum_g P^T dO
+// with Delta = rowsum(dO o O) and the sums over the query heads g of a key /
+// value head.  No atomics: every gradient row is written by one CTA.
+//
+// Bound by the tensor cores: dQ needs three products of a 128 x 128 tile (S,
+// dP, dS K), dK / dV four.  Both kernels keep them fed by the order in which
+// the MMA warp issues:
+//  * dQ: S two tiles ahead in two buffers; once dS_j is written, dP_j+1, then
+//    dQ += dS_j K_j, then S_j+2.  The exponentials of tile j+1 run under dP_j+1;
+//  * dK / dV: P_i^T ready -> dV += P_i^T dO_i, S_i+1^T (over P_i); dS_i^T ready
+//    -> dK += dS_i^T Q_i, dP_i+1^T (over dS_i).  The exponentials of step i+1
+//    run under the last two.
+// Roles of a CTA: warp 0 TMA producer, warp 1 MMA issue, warpgroups 1 and 2
+// elementwise: a row is shared by two threads, one of each warpgroup, with 64
+// of the tile's 128 columns, so that each 16-bit result lies over columns its
+// own thread has read (columns 0-31 and 64-95 of the score buffer).
+// Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and all roles drain.
+#include <cudaTypedefs.h>
+
+#include <atomic>
+
+#include "common.cuh"
+#include "internal.h"
+#include "softmax.cuh"
+
+namespace bsa {
+
+namespace {
+
+constexpr int kThreadsB = 384;
+
+struct DBwdParams {
+  int B, H, Hk, G, M, N;
+  int q_tiles, k_tiles;
+  int qb_mul, kb_mul, vb_mul, db_mul;  // 0: the tensor's batch stride is 0
+  const void* lens;
+  int lens_i64;
+  float scale_log2, sm_scale;
+  const float* lse;    // [B, H, M]
+  const float* delta;  // [B, H, M]
+  uint8_t *dq, *dk, *dv;
+  int64_t dq_b, dq_h, dq_n, dk_b, dk_h, dk_n, dv_b, dv_h, dv_n;
+  int32_t* err;
+  uint64_t wait_ns;
+};
+
+template <int D>
+struct DBwdCfg {
+  static constexpr int NCHUNK = D / 64;
+  static constexpr int CHUNK = 128 * 128;
+  static constexpr int TILE = 128 * D * 2;
+  static constexpr int STAGES = D == 128 ? 2 : 4;  // of the two streamed tensors
+  static constexpr int BAR_BYTES = 256;
+  static constexpr int STATS = 2 * 2 * 128 * 4;
+  static constexpr int SMEM = (2 + 2 * STAGES) * TILE + BAR_BYTES + STATS;
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+__device__ __forceinline__ int bwd_len(const DBwdParams& p, int b) {
+  if (!p.lens) return p.N;
+  const int64_t l = p.lens_i64 ? __ldg(static_cast<const int64_t*>(p.lens) + b)
+                               : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.lens) + b));
+  if (l < 0 || l > p.N) set_err(p.err, BSA_DEVERR_COORD);
+  return static_cast<int>(l < 0 ? 0 : l > p.N ? p.N : l);
+}
+
+// -lse as the exponent's offset; a row without any weight (lse -inf) and a row
+// past the end get P = 0.
+__device__ __forceinline__ float neg_lse_of(const DBwdParams& p, bool in, int64_t i) {
+  const float l = in ? __ldg(&p.lse[i]) : -INFINITY;
+  return l == -INFINITY ? -INFINITY : -l;
+}
+
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// A 128 x 64-column part of an accumulator row (this thread's 32 columns at a
+// time) times `scale`, as 16-bit values; zeros where `zero`.
+template <int D, bool BF16>
+__device__ __forceinline__ void store_half_row(uint32_t base, int half, float scale, uint8_t* row, bool store, bool zero) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    const int col = half * (D / 2) + c * 32;
+    uint32_t a[32];
+    tmem_ld32(base + col, a);
+    tmem_wait32(a);
+    if (store) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint4 v;
+        v.x = pack2<BF16>(__uint_as_float(a[8 * g + 0]) * scale, __uint_as_float(a[8 * g + 1]) * scale);
+        v.y = pack2<BF16>(__uint_as_float(a[8 * g + 2]) * scale, __uint_as_float(a[8 * g + 3]) * scale);
+        v.z = pack2<BF16>(__uint_as_float(a[8 * g + 4]) * scale, __uint_as_float(a[8 * g + 5]) * scale);
+        v.w = pack2<BF16>(__uint_as_float(a[8 * g + 6]) * scale, __uint_as_float(a[8 * g + 7]) * scale);
+        if (zero) v = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(row)[col / 8 + g] = v;
+      }
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void zero_half_row(int half, uint8_t* row) {
+#pragma unroll
+  for (int g = 0; g < D / 16; ++g) reinterpret_cast<uint4*>(row)[half * (D / 16) + g] = make_uint4(0, 0, 0, 0);
+}
+
+// C (+)= A B^T of two 128 x D shared-memory tiles (both K-major)
+template <int D>
+__device__ __forceinline__ void mma_abt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    const uint32_t off = (kk >> 2) * DBwdCfg<D>::CHUNK + (kk & 3) * 32;
+    tc_mma_ss(d, make_sw128_desc(a + off, 16, 1024), make_sw128_desc(b + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+  }
+}
+// C (+)= A B of a 128 x 128 16-bit A in tensor memory (columns 0-31 and
+// 64-95) and a 128 x D shared-memory tile (MN-major)
+template <int D>
+__device__ __forceinline__ void mma_ab(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    tc_mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, make_sw128_desc(b + kk * 16 * 128, DBwdCfg<D>::CHUNK, 1024), idesc,
+              (first && kk == 0) ? 0u : 1u);
+}
+
+// ---------------------------------------------------------------------------
+// dQ: one CTA per 128 query rows of one head, over the key tiles.
+// TMEM: S_j / dS_j [128 (j & 1), +128), dP [256, 384), dQ [384, 384 + D).
+// ---------------------------------------------------------------------------
+template <int D, bool BF16>
+__device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmDO,
+                        const DBwdParams& p, uint8_t* smem, int item) {
+  using C = DBwdCfg<D>;
+  constexpr int ST = C::STAGES;
+  uint8_t* sQ = smem;
+  uint8_t* sDO = sQ + C::TILE;
+  uint8_t* sK = sDO + C::TILE;      // [ST]
+  uint8_t* sV = sK + ST * C::TILE;  // [ST]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * C::TILE);
+  uint64_t* q_full = bars;
+  uint64_t* kv_full = bars + 1;            // [ST]
+  uint64_t* kv_empty = kv_full + ST;       // [ST] dQ_j (the last reader) completed
+  uint64_t* s_full = kv_empty + ST;        // [2]
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_ready = dp_full + 1;        // 8 elementwise warps
+  uint64_t* done = ds_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bh = item / p.q_tiles, t = item - bh * p.q_tiles;
+  const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 8);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+  constexpr uint32_t kDP = 256, kDQ = 384;
+  const int len = bwd_len(p, b);
+  const int n = (len + 127) / 128;
+  auto wait = [&](uint64_t* bar, int k) { return mbar_wait(bar, k & 1, abort_flag, p.err, p.wait_ns); };
+  auto wait_all = [&](uint64_t* bar, int k) { return __all_sync(0xffffffffu, wait(bar, k)) != 0; };
+
+  if (warp == 0 && lane == 0 && n > 0) {
+    // ------------------------------------------------------------- producer
+    mbar_arrive_expect_tx(q_full, 2 * C::TILE);
+    for (int c = 0; c < C::NCHUNK; ++c) {
+      tma_load_4d(sQ + c * C::CHUNK, &tmQ, q_full, c * 64, t * 128, h, b * p.qb_mul);
+      tma_load_4d(sDO + c * C::CHUNK, &tmDO, q_full, c * 64, t * 128, h, b * p.db_mul);
+    }
+    int j = 0;
+    for (; j < n; ++j) {
+      const int st = j % ST;
+      if (j >= ST && !wait(&kv_empty[st], j / ST - 1)) break;
+      mbar_arrive_expect_tx(&kv_full[st], 2 * C::TILE);
+      for (int c = 0; c < C::NCHUNK; ++c) {
+        tma_load_4d(sK + st * C::TILE + c * C::CHUNK, &tmK, &kv_full[st], c * 64, j * 128, hk, b * p.kb_mul);
+        tma_load_4d(sV + st * C::TILE + c * C::CHUNK, &tmV, &kv_full[st], c * 64, j * 128, hk, b * p.vb_mul);
+      }
+    }
+    mbar_wait(q_full, 0, nullptr, nullptr, p.wait_ns);
+    for (int i = j > ST ? j - ST : 0; i < j; ++i) mbar_wait(&kv_full[i % ST], (i / ST) & 1, nullptr, nullptr, p.wait_ns);
+  } else if (warp == 1 && n > 0) {
+    // ------------------------------------------------------------ MMA issue
+    constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
+    constexpr uint32_t idesc_dq = make_idesc_f16(BF16, 128, D, false, true);
+    const uint32_t q_addr = smem_u32(sQ), do_addr = smem_u32(sDO), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+    bool ok = wait_all(q_full, 0);
+    auto issue_s = [&](int j) {
+      const int st = j % ST;
+      if (!(ok = ok && wait_all(&kv_full[st], j / ST))) return;
+      const int tail = len - j * 128;
+      if (tail < 128) {
+        // K rows past the length: zero, for dS = 0 times what lies there
+        uint8_t* kt = sK + st * C::TILE;
+        for (int x = tail * 8 + lane; x < 128 * 8; x += 32) {
+#pragma unroll
+          for (int c = 0; c < C::NCHUNK; ++c)
+            *reinterpret_cast<uint4*>(kt + c * C::CHUNK + x * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        mma_abt<D>(tmem + (j & 1) * 128, q_addr, k_addr + st * C::TILE, idesc_s);
+        tc_commit(&s_full[j & 1]);
+      }
+      __syncwarp();
+    };
+    auto issue_dp = [&](int j) {
+      if (lane == 0) {
+        mma_abt<D>(tmem + kDP, do_addr, v_addr + (j % ST) * C::TILE, idesc_s);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
+    };
+    if (ok) issue_s(0);
+    if (ok) issue_dp(0);
+    if (ok && n > 1) issue_s(1);
+    for (int j = 0; ok && j < n; ++j) {
+      if (!(ok = wait_all(ds_ready, j))) break;
+      tc_fence_after();
+      // dP's buffer is free (dS_j is written): step j+1 can go on
+      if (j + 1 < n) issue_dp(j + 1);
+      if (lane == 0) {
+        mma_ab<D>(tmem + kDQ, tmem + (j & 1) * 128, k_addr + (j % ST) * C::TILE, idesc_dq, j == 0);
+        tc_commit(&kv_empty[j % ST]);
+      }
+      __syncwarp();
+      // over dS_j, which dQ_j (issued before) has read
+      if (j + 2 < n) issue_s(j + 2);
+    }
+    if (lane == 0) {
+      tc_commit(done);
+      mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------- elementwise, epilogue
+    const int q4 = warp & 3, half = (warp - 4) >> 2;
+    const int row = q4 * 32 + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+    const int grow = t * 128 + row;
+    const bool live = grow < p.M;
+    uint8_t* orow = p.dq + 2 * (b * p.dq_b + h * p.dq_h + static_cast<int64_t>(grow) * p.dq_n);
+    if (n == 0) {
+      if (live) zero_half_row<D>(half, orow);
+    } else {
+      const int64_t ri = (static_cast<int64_t>(b) * p.H + h) * p.M + grow;
+      const float neg_lse = neg_lse_of(p, live, ri);
+      const float dlt = live ? __ldg(&p.delta[ri]) : 0.f;
+      const uint64_t sc2 = f32x2_pack(p.scale_log2, p.scale_log2), nl2 = f32x2_pack(neg_lse, neg_lse);
+      const uint64_t nd2 = f32x2_pack(-dlt, -dlt);
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t s_col = (j & 1) * 128 + half * 64;
+        const int valid = len - j * 128 - half * 64;  // keys of this thread's columns
+        if (!(ok = ok && wait_all(&s_full[j & 1], j >> 1))) break;
+        tc_fence_after();
+        float pv[64];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sv[32];
+          tmem_ld32(lane_base + s_col + c * 32, sv);
+          tmem_wait32(sv);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const uint64_t x = f32x2_fma(f32x2_pack(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc2, nl2);
+            float x0, x1;
+            f32x2_unpack(x, x0, x1);
+            pv[c * 32 + k] = ex2_approx(x0);
+            pv[c * 32 + k + 1] = ex2_approx(x1);
+          }
+        }
+        if (!(ok = wait_all(dp_full, j))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t dp[32], ds[16];
+          tmem_ld32(lane_base + kDP + half * 64 + c * 32, dp);
+          tmem_wait32(dp);
+          if (valid < 64) {
+            // keys past the length: dS = 0, whatever their scores and values are
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c * 32 + k >= valid) pv[c * 32 + k] = 0.f, dp[k] = 0u;
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const uint64_t g = f32x2_add(f32x2_pack(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), nd2);
+            float g0, g1;
+            f32x2_unpack(g, g0, g1);
+            ds[k / 2] = pack2<BF16>(pv[c * 32 + k] * g0, pv[c * 32 + k + 1] * g1);
+          }
+          tmem_st16(lane_base + s_col + c * 16, ds);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      ok = ok && wait_all(done, 0);
+      if (ok) {
+        tc_fence_after();
+        store_half_row<D, BF16>(lane_base + kDQ, half, p.sm_scale, orow, live, false);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dK, dV: one CTA per 128 keys of one key / value head, over the query tiles of
+// every query head that shares it.
+// TMEM: S^T / P^T [0, 128), dP^T / dS^T [128, 256), dV [256, 256 + D), dK
+// [256 + D, 256 + 2D).
+// ---------------------------------------------------------------------------
+template <int D, bool BF16>
+__device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmDO,
+                          const DBwdParams& p, uint8_t* smem, int item) {
+  using C = DBwdCfg<D>;
+  constexpr int ST = C::STAGES;
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + C::TILE;
+  uint8_t* sQ = sV + C::TILE;        // [ST]
+  uint8_t* sDO = sQ + ST * C::TILE;  // [ST]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sDO + ST * C::TILE);
+  float* col_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + C::BAR_BYTES);  // [2][128]
+  float* col_dlt = col_lse + 256;                                                                 // [2][128]
+  uint64_t* kv_full = bars;
+  uint64_t* qd_full = bars + 1;         // [ST]
+  uint64_t* qd_empty = qd_full + ST;    // [ST] dK_i (the last reader) completed
+  uint64_t* s_full = qd_empty + ST;
+  uint64_t* dp_full = s_full + 1;
+  uint64_t* p_ready = dp_full + 1;      // 8 elementwise warps wrote P^T
+  uint64_t* ds_ready = p_ready + 1;     // 8 elementwise warps wrote dS^T
+  uint64_t* done = ds_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bh = item / p.k_tiles, t = item - bh * p.k_tiles;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&qd_full[i], 1);
+      mbar_init(&qd_empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(ds_ready, 8);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+  const int len = bwd_len(p, b);
+  const int n = t * 128 < len ? p.G * p.q_tiles : 0;  // steps: query tiles of all heads of the group
+  auto wait = [&](uint64_t* bar, int k) { return mbar_wait(bar, k & 1, abort_flag, p.err, p.wait_ns); };
+  auto wait_all = [&](uint64_t* bar, int k) { return __all_sync(0xffffffffu, wait(bar, k)) != 0; };
+
+  if (warp == 0 && lane == 0 && n > 0) {
+    // ------------------------------------------------------------- producer
+    mbar_arrive_expect_tx(kv_full, 2 * C::TILE);
+    for (int c = 0; c < C::NCHUNK; ++c) {
+      tma_load_4d(sK + c * C::CHUNK, &tmK, kv_full, c * 64, t * 128, hk, b * p.kb_mul);
+      tma_load_4d(sV + c * C::CHUNK, &tmV, kv_full, c * 64, t * 128, hk, b * p.vb_mul);
+    }
+    int i = 0;
+    for (; i < n; ++i) {
+      const int st = i % ST, g = i / p.q_tiles, qt = i - g * p.q_tiles;
+      if (i >= ST && !wait(&qd_empty[st], i / ST - 1)) break;
+      mbar_arrive_expect_tx(&qd_full[st], 2 * C::TILE);
+      for (int c = 0; c < C::NCHUNK; ++c) {
+        tma_load_4d(sQ + st * C::TILE + c * C::CHUNK, &tmQ, &qd_full[st], c * 64, qt * 128, hk * p.G + g, b * p.qb_mul);
+        tma_load_4d(sDO + st * C::TILE + c * C::CHUNK, &tmDO, &qd_full[st], c * 64, qt * 128, hk * p.G + g, b * p.db_mul);
+      }
+    }
+    mbar_wait(kv_full, 0, nullptr, nullptr, p.wait_ns);
+    for (int k = i > ST ? i - ST : 0; k < i; ++k) mbar_wait(&qd_full[k % ST], (k / ST) & 1, nullptr, nullptr, p.wait_ns);
+  } else if (warp == 1 && n > 0) {
+    // ------------------------------------------------------------ MMA issue
+    constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
+    constexpr uint32_t idesc_acc = make_idesc_f16(BF16, 128, D, false, true);
+    const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV), q_addr = smem_u32(sQ), do_addr = smem_u32(sDO);
+    bool ok = wait_all(kv_full, 0);
+    auto issue_s = [&](int i) {
+      if (!(ok = ok && wait_all(&qd_full[i % ST], i / ST))) return;
+      tc_fence_after();
+      if (lane == 0) {
+        mma_abt<D>(tmem, k_addr, q_addr + (i % ST) * C::TILE, idesc_s);
+        tc_commit(s_full);
+      }
+      __syncwarp();
+    };
+    auto issue_dp = [&](int i) {
+      if (lane == 0) {
+        mma_abt<D>(tmem + 128, v_addr, do_addr + (i % ST) * C::TILE, idesc_s);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
+    };
+    if (ok) issue_s(0);
+    if (ok) issue_dp(0);
+    for (int i = 0; ok && i < n; ++i) {
+      if (!(ok = wait_all(p_ready, i))) break;
+      tc_fence_after();
+      if (lane == 0) mma_ab<D>(tmem + 256, tmem, do_addr + (i % ST) * C::TILE, idesc_acc, i == 0);
+      __syncwarp();
+      if (i + 1 < n) issue_s(i + 1);  // over P_i^T, which dV_i has read
+      if (!(ok = ok && wait_all(ds_ready, i))) break;
+      tc_fence_after();
+      if (lane == 0) {
+        mma_ab<D>(tmem + 256 + D, tmem + 128, q_addr + (i % ST) * C::TILE, idesc_acc, i == 0);
+        tc_commit(&qd_empty[i % ST]);
+      }
+      __syncwarp();
+      if (i + 1 < n) issue_dp(i + 1);  // over dS_i^T
+    }
+    if (lane == 0) {
+      tc_commit(done);
+      mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------- elementwise, epilogue
+    const int q4 = warp & 3, half = (warp - 4) >> 2;
+    const int row = q4 * 32 + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+    const int krow = t * 128 + row;
+    const bool live = krow < p.N;
+    uint8_t* krow_out = p.dk + 2 * (b * p.dk_b + hk * p.dk_h + static_cast<int64_t>(krow) * p.dk_n);
+    uint8_t* vrow_out = p.dv + 2 * (b * p.dv_b + hk * p.dv_h + static_cast<int64_t>(krow) * p.dv_n);
+    if (n == 0) {
+      if (live) {
+        zero_half_row<D>(half, krow_out);
+        zero_half_row<D>(half, vrow_out);
+      }
+    } else {
+      const uint64_t sc2 = f32x2_pack(p.scale_log2, p.scale_log2);
+      // the first warpgroup stages -lse, the second -Delta, of the step's 128
+      // query rows; the value of the next step is fetched a step ahead
+      auto fetch = [&](int i) -> float {
+        const int g = i / p.q_tiles, qrow = (i - g * p.q_tiles) * 128 + row;
+        const int64_t at = (static_cast<int64_t>(b) * p.H + hk * p.G + g) * p.M + qrow;
+        const bool in = i < n && qrow < p.M;
+        return half == 0 ? neg_lse_of(p, in, at) : (in ? -__ldg(&p.delta[at]) : 0.f);
+      };
+      float next = fetch(0);
+      bool ok = true;
+      for (int i = 0; i < n; ++i) {
+        const float* lb = col_lse + (i & 1) * 128 + half * 64;
+        const float* db = col_dlt + (i & 1) * 128 + half * 64;
+        (half == 0 ? col_lse : col_dlt)[(i & 1) * 128 + row] = next;
+        if (i + 1 < n) next = fetch(i + 1);
+        // (a warp whose wait failed keeps taking part in this barrier, which
+        // has no time limit, and skips the rest of each step)
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (!(ok = ok && wait_all(s_full, i))) continue;
+        tc_fence_after();
+        float pv[64];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sv[32], pt[16];
+          tmem_ld32(lane_base + half * 64 + c * 32, sv);
+          tmem_wait32(sv);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float2 nl = *reinterpret_cast<const float2*>(lb + c * 32 + k);
+            const uint64_t x =
+                f32x2_fma(f32x2_pack(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc2, f32x2_pack(nl.x, nl.y));
+            float x0, x1;
+            f32x2_unpack(x, x0, x1);
+            pv[c * 32 + k] = ex2_approx(x0);
+            pv[c * 32 + k + 1] = ex2_approx(x1);
+            pt[k / 2] = pack2<BF16>(pv[c * 32 + k], pv[c * 32 + k + 1]);
+          }
+          tmem_st16(lane_base + half * 64 + c * 16, pt);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        if (!(ok = wait_all(dp_full, i))) continue;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t dp[32], ds[16];
+          tmem_ld32(lane_base + 128 + half * 64 + c * 32, dp);
+          tmem_wait32(dp);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float2 nd = *reinterpret_cast<const float2*>(db + c * 32 + k);
+            const uint64_t g =
+                f32x2_add(f32x2_pack(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), f32x2_pack(nd.x, nd.y));
+            float g0, g1;
+            f32x2_unpack(g, g0, g1);
+            ds[k / 2] = pack2<BF16>(pv[c * 32 + k] * g0, pv[c * 32 + k + 1] * g1);
+          }
+          tmem_st16(lane_base + 128 + half * 64 + c * 16, ds);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      ok = ok && wait_all(done, 0);
+      if (ok) {
+        tc_fence_after();
+        // keys past the length have no gradient
+        const bool zero = krow >= len;
+        store_half_row<D, BF16>(lane_base + 256, half, 1.f, vrow_out, live, zero);
+        store_half_row<D, BF16>(lane_base + 256 + D, half, p.sm_scale, krow_out, live, zero);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// One launch for both: the dK / dV tiles first (the longer ones), then dQ.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreadsB, 1)
+    dense_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
+                     const __grid_constant__ DBwdParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) set_err(p.err, BSA_DEVERR_ALIGN);
+    return;
+  }
+  const int kv_items = p.B * p.Hk * p.k_tiles;
+  const int item = static_cast<int>(blockIdx.x);
+  if (item < kv_items)
+    dkdv_tile<D, BF16>(tmQ, tmK, tmV, tmDO, p, smem, item);
+  else
+    dq_tile<D, BF16>(tmQ, tmK, tmV, tmDO, p, smem, item - kv_items);
+}
+
+int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul) {
+  const bool one = B == 1 || t.stride_b == 0;
+  *mul = one ? 0 : 1;
+  if (one) t.stride_b = 8;
+  if (H == 1) t.stride_h = 8;
+  if (N == 1) t.stride_n = 8;
+  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, 128);
+}
+
+template <int D, bool BF16>
+int launch_t(const bsa_cross_bwd_args* a, cudaStream_t st) {
+  using C = DBwdCfg<D>;
+  auto kern = dense_bwd_kernel<D, BF16>;
+  static std::atomic<bool> ready[64] = {};
+  int dev = 0;
+  BSA_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return BSA_ERR_DEVICE;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    BSA_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  DBwdParams p{};
+  CUtensorMap mq, mk{}, mv{}, mdo;
+  int r;
+  if ((r = map_of(&mq, a->q, a->B, a->H, a->M, D, BF16, &p.qb_mul))) return r;
+  if ((r = map_of(&mdo, a->dout, a->B, a->H, a->M, D, BF16, &p.db_mul))) return r;
+  if (a->N > 0) {
+    if ((r = map_of(&mk, a->k, a->B, a->Hk, a->N, D, BF16, &p.kb_mul))) return r;
+    if ((r = map_of(&mv, a->v, a->B, a->Hk, a->N, D, BF16, &p.vb_mul))) return r;
+  }
+  if ((r = launch_bwd_delta(a->o, a->dout, a->delta, a->B, a->H, a->M, D, BF16, st))) return r;
+  p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.G = a->H / a->Hk, p.M = a->M, p.N = a->N;
+  p.q_tiles = (a->M + 127) / 128;
+  p.k_tiles = (a->N + 127) / 128;
+  p.lens = a->k_lens;
+  p.lens_i64 = a->lens_dtype == BSA_INDEX_I64;
+  p.scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p.sm_scale = a->sm_scale;
+  p.lse = a->lse;
+  p.delta = a->delta;
+  p.dq = static_cast<uint8_t*>(a->dq.data), p.dq_b = a->dq.stride_b, p.dq_h = a->dq.stride_h, p.dq_n = a->dq.stride_n;
+  p.dk = static_cast<uint8_t*>(a->dk.data), p.dk_b = a->dk.stride_b, p.dk_h = a->dk.stride_h, p.dk_n = a->dk.stride_n;
+  p.dv = static_cast<uint8_t*>(a->dv.data), p.dv_b = a->dv.stride_b, p.dv_h = a->dv.stride_h, p.dv_n = a->dv.stride_n;
+  p.err = a->err_flag;
+  p.wait_ns = kWaitNs;
+  const int64_t items =
+      static_cast<int64_t>(p.B) * p.Hk * p.k_tiles + static_cast<int64_t>(p.B) * p.H * p.q_tiles;
+  if (items > INT32_MAX) return BSA_ERR_UNSUPPORTED;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items));
+  cfg.blockDim = dim3(kThreadsB);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, mdo, p));
+  return BSA_OK;
+}
+
+bool aligned(const bsa_tensor4d& t, int B, int H, int N) {
+  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && (B == 1 || t.stride_b * 2 % 16 == 0) &&
+         (H == 1 || t.stride_h * 2 % 16 == 0) && (N == 1 || t.stride_n * 2 % 16 == 0);
+}
+
+}  // namespace
+
+int cross_bwd_validate(const bsa_cross_bwd_args* a) {
+  if (!a) return BSA_ERR_INVALID_ARG;
+  if (a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->M <= 0 || a->N < 0 || a->D <= 0) return BSA_ERR_INVALID_ARG;
+  if (a->dtype != BSA_DTYPE_F16 && a->dtype != BSA_DTYPE_BF16) return BSA_ERR_DTYPE;
+  if (a->H % a->Hk) return BSA_ERR_SHAPE;
+  if (a->D != 64 && a->D != 128) return BSA_ERR_UNSUPPORTED;
+  if (!(a->sm_scale > 0.f) || !(a->sm_scale < INFINITY)) return BSA_ERR_UNSUPPORTED;
+  if (!a->lse || !a->delta) return BSA_ERR_INVALID_ARG;
+  if (static_cast<int64_t>(a->B) * a->H * a->M > INT32_MAX / 2 || a->N > INT32_MAX - 65536) return BSA_ERR_UNSUPPORTED;
+  const bsa_tensor4d* qs[] = {&a->q, &a->o, &a->dout, &a->dq};
+  const bsa_tensor4d* ks[] = {&a->k, &a->v, &a->dk, &a->dv};
+  for (int i = 0; i < 4; ++i) {
+    if (!qs[i]->data) return BSA_ERR_INVALID_ARG;
+    if (!aligned(*qs[i], a->B, a->H, a->M)) return BSA_ERR_ALIGNMENT;
+    if (a->N == 0) continue;
+    if (!ks[i]->data || ks[i]->stride_b < 0) return BSA_ERR_INVALID_ARG;
+    if (!aligned(*ks[i], a->B, a->Hk, a->N)) return BSA_ERR_ALIGNMENT;
+  }
+  if (a->k_lens && a->lens_dtype != BSA_INDEX_I32 && a->lens_dtype != BSA_INDEX_I64) return BSA_ERR_DTYPE;
+  return BSA_OK;
+}
+
+int launch_cross_bwd(const bsa_cross_bwd_args* a, cudaStream_t st) {
+  const bool bf = a->dtype == BSA_DTYPE_BF16;
+  if (a->D == 128) return bf ? launch_t<128, true>(a, st) : launch_t<128, false>(a, st);
+  return bf ? launch_t<64, true>(a, st) : launch_t<64, false>(a, st);
+}
+
+}  // namespace bsa

@@ -34,6 +34,9 @@ int launch_permute_rows(bsa_tensor4d dst, bsa_tensor4d src, int B, int H, int N,
 int launch_attn_simt(const bsa_fwd_args* a, cudaStream_t st);
 // The backward kernels (attn_bwd.cu): Delta, dQ, dK / dV; arguments validated.
 int launch_attn_bwd(const bsa_bwd_args* a, cudaStream_t st);
+// Delta = rowsum(dout o o) per query row, contiguous fp32 [B, H, N] (D 64 / 128).
+int launch_bwd_delta(const bsa_tensor4d& o, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
+                     bool bf16, cudaStream_t st);
 
 // tma_maps.cu: whether the tcgen05 path takes these arguments (bf16 / fp16,
 // D 64 or 128, BLOCK 64 or 128, 16-byte-aligned rows), and the 4-D TMA map
@@ -50,6 +53,24 @@ int launch_attn_tcp(const bsa_fwd_args* a, cudaStream_t st, const void* q_perm =
 // bsa_test_arm_wait_timeout).
 int arm_test_wait_timeout(uint32_t wait_us);
 
+// qk_norm_rope.cu: norm and rotation of query / key heads, and its gradient
+// (each launcher validates its arguments).
+int rope_validate(const bsa_rope_args* a, bool bwd);
+int launch_rope_fwd(const bsa_rope_args* a, cudaStream_t st);
+size_t rope_bwd_workspace(const bsa_rope_args* a);
+int launch_rope_bwd(const bsa_rope_args* a, void* workspace, size_t bytes, cudaStream_t st);
+
+// attn_dense.cu: attention over contiguous key ranges (arguments validated
+// by the caller with the *_validate functions).
+int cross_validate(const bsa_cross_args* a);
+size_t cross_workspace(const bsa_cross_args* a);
+int launch_cross(const bsa_cross_args* a, void* workspace, size_t bytes, cudaStream_t st);
+int prefix_validate(const bsa_prefix_args* a);
+size_t prefix_workspace(const bsa_prefix_args* a);
+int launch_prefix(const bsa_prefix_args* a, void* workspace, size_t bytes, cudaStream_t st);
+// attn_dense_bwd.cu: gradient of cross attention
+int cross_bwd_validate(const bsa_cross_bwd_args* a);
+int launch_cross_bwd(const bsa_cross_bwd_args* a, cudaStream_t st);
 
 }  // namespace bsa
 

@@ -240,6 +240,109 @@ typedef struct bsa_bwd_args {
 } bsa_bwd_args;
 BSA_API int bsa_bwd(const bsa_bwd_args* args, void* stream);
 
+/* Norm of every query and key head and the rotation of its token's position,
+ * in one pass over q [B, H, N, D] and k [B, Hk, N, D] (either head count may
+ * be 0: that side is absent):
+ *   y = R(pos) (x / sqrt(mean(x^2) + eps) * w)
+ * No counterpart in the reference, whose inputs are q and k as attention takes
+ * them.  D a multiple of 8 up to 256, R (rotated leading dimensions) a
+ * multiple of 16 up to D, 0 = norm only.  The rotation turns the pairs
+ * (i, i + R/2), or neighbours (2i, 2i + 1) with `interleaved`, by the angles
+ * whose cosines and sines row `pos` of the tables holds.  Positions outside
+ * [0, table_len) set BSA_DEVERR_COORD and give NaN rows.  Outputs may be the
+ * inputs themselves (same strides); they may not overlap them otherwise. */
+typedef struct bsa_rope_args {
+  int32_t B, H, Hk, N, D, R;
+  int32_t dtype;                 /* bsa_dtype of q, k and the outputs               */
+  int32_t weight_dtype;          /* of the weights: dtype or BSA_DTYPE_F32          */
+  bsa_tensor4d q, k;             /* inputs                                          */
+  bsa_tensor4d q_out, k_out;     /* forward: outputs; backward: dq, dk              */
+  bsa_tensor4d dq_out, dk_out;   /* backward only: gradients of the outputs         */
+  const void* q_weight;          /* [D]; NULL = ones                                */
+  const void* k_weight;
+  const float* cos;              /* [table_len, R/2], rows table_stride apart       */
+  const float* sin;
+  int64_t table_stride;
+  int32_t table_len;
+  int32_t pos_dtype;             /* bsa_index_dtype of positions                    */
+  const void* positions;         /* [N] (pos_stride_b 0) or [B, N]; NULL = 0 .. N-1 */
+  int64_t pos_stride_b;
+  float eps;
+  int32_t interleaved;
+  void* dq_weight;               /* backward: [D] of weight_dtype; NULL = not wanted */
+  void* dk_weight;
+  int32_t* err_flag;             /* optional device int32 for BSA_DEVERR_* bits     */
+} bsa_rope_args;
+BSA_API int bsa_qk_norm_rope(const bsa_rope_args* args, void* stream);
+/* Its gradient: q_out, k_out receive dq, dk for the gradients dq_out, dk_out;
+ * the weights' gradients are sums in a fixed order (no atomics), held in the
+ * workspace per block first (needed when either is wanted). */
+BSA_API int bsa_qk_norm_rope_bwd_workspace_bytes(const bsa_rope_args* args, size_t* bytes);
+BSA_API int bsa_qk_norm_rope_bwd(const bsa_rope_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Cross attention: q, o [B, H, M, D] over k, v [B, Hk, N, D] of another
+ * length, H a multiple of Hk (head h reads key / value head h / (H / Hk)):
+ *   o = softmax over keys j < k_lens[b] of (q k^T * sm_scale) v
+ * bf16 / fp16, D 64 or 128, tcgen05.  No counterpart in the reference, whose
+ * queries and keys share one length.  k_lens NULL = all N keys; a length of 0
+ * (or N = 0) gives o = 0 and lse = -inf; lengths outside [0, N] set
+ * BSA_DEVERR_COORD and are clamped.  Keys behind a length are not read into
+ * the result, whatever they hold.  k and v with stride_b 0 are one copy for
+ * the batch.  Few rows split the keys over the SMs; the partial results live
+ * in the workspace and a second kernel joins them. */
+typedef struct bsa_cross_args {
+  int32_t B, H, Hk, M, N, D;
+  int32_t dtype;            /* bsa_dtype: f16 or bf16                              */
+  int32_t lens_dtype;       /* bsa_index_dtype of k_lens                           */
+  bsa_tensor4d q, o, k, v;
+  const void* k_lens;       /* optional [B]                                        */
+  float* lse;               /* optional contiguous [B, H, M], log2 units           */
+  int32_t* err_flag;
+  float sm_scale;
+} bsa_cross_args;
+BSA_API int bsa_cross_fwd_workspace_bytes(const bsa_cross_args* args, size_t* bytes);
+BSA_API int bsa_cross_fwd(const bsa_cross_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradient, from the forward's o and lse: dq [B, H, M, D]; dk, dv
+ * [B, Hk, N, D], summed over the query heads of a key / value head in a fixed
+ * order, zero for keys behind k_lens[b].  delta: workspace, contiguous
+ * [B, H, M] fp32.  Enqueues two kernels on `stream`; no atomics. */
+typedef struct bsa_cross_bwd_args {
+  int32_t B, H, Hk, M, N, D;
+  int32_t dtype;
+  int32_t lens_dtype;
+  bsa_tensor4d q, k, v, o, dout;
+  bsa_tensor4d dq, dk, dv;  /* outputs                                             */
+  const void* k_lens;       /* the forward's                                       */
+  const float* lse;         /* the forward's contiguous [B, H, M]                  */
+  float* delta;
+  int32_t* err_flag;
+  float sm_scale;
+} bsa_cross_bwd_args;
+BSA_API int bsa_cross_bwd(const bsa_cross_bwd_args* args, void* stream);
+
+/* Attention of a batch behind a shared prefix: T new tokens of each of B
+ * sequences, q, o [B, H, T, D], over k_prefix, v_prefix [Hk, P, D] (stride_b
+ * unused), which all of them see whole and which are read once for the batch,
+ * and over each sequence's own keys k, v [B, Hk, C, D], of which lens[b]
+ * (NULL = C) are valid and the last T belong to the new tokens: token t sees
+ * own keys j < lens[b] - (T - 1 - t).  P or C may be 0.  Lengths outside
+ * [0, C] set BSA_DEVERR_COORD and are clamped.  A value row that some tokens
+ * of a sequence see and others do not must be finite for the latter's sake
+ * (0 x V).  No counterpart in the reference. */
+typedef struct bsa_prefix_args {
+  int32_t B, H, Hk, T, P, C, D;
+  int32_t dtype;            /* bsa_dtype: f16 or bf16                              */
+  int32_t lens_dtype;
+  bsa_tensor4d q, o, k_prefix, v_prefix, k, v;
+  const void* lens;         /* optional [B]                                        */
+  float* lse;               /* optional contiguous [B, H, T], log2 units           */
+  int32_t* err_flag;
+  float sm_scale;
+} bsa_prefix_args;
+BSA_API int bsa_prefix_fwd_workspace_bytes(const bsa_prefix_args* args, size_t* bytes);
+BSA_API int bsa_prefix_fwd(const bsa_prefix_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Test hook for the bounded device waits, not for production use.  Arms the
  * NEXT tcgen05 forward (bsa_fwd / bsa_fwd_reordered) of the process: every
  * mbarrier wait of its launch gives up after `wait_us` microseconds (100 ..
