@@ -26,9 +26,9 @@
 // 16-bit pairs over S_i, then O += P_i V_i, then S_i+1; so S_i+1 seen complete
 // means PV_i complete, and the softmax may rescale O and hand back the stages
 // of V_i and K_i+1 without any further commit.
-// Roles: warp 0 TMA producer; warp 1 issues tcgen05.mma; warps 2-3 gather
-// query rows of several heads (or sequences) into one tile where a head has
-// fewer than 128; warpgroups 1, 2 softmax of streams 0, 1; warpgroup 3 epilogue.
+// Roles: warp 0 TMA producer; warp 1 one thread issues tcgen05.mma; warps
+// 2-3 gather query rows of several heads (or sequences) into one tile where a
+// head has fewer than 128; warpgroups 1, 2 softmax of streams 0, 1; warpgroup 3 epilogue.
 //
 // Bound: 4 rows keys D flops against the tensor rate and, row by row, the 16
 // exponentials a clock of an SM (as many cycles as the products at D = 128);
@@ -191,6 +191,16 @@ __device__ __forceinline__ int steps_of(const Item& it, int s) {
 }
 __device__ __forceinline__ int tile_of(const Item& it, int s, int i) { return it.dual ? 2 * i + s : i; }
 
+// A stage of the K / V ring and its phase.
+template <int SL>
+struct Ring {
+  int st = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++st == SL) st = 0, ph ^= 1;
+  }
+};
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -325,93 +335,105 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       // every load issued lands before the CTA exits
       for (int i = c > SL ? c - SL : 0; i < c; ++i) mbar_wait(&full[i % SL], (i / SL) & 1, nullptr, nullptr, p.wait_ns);
       if (!p.packed && nq > 0) mbar_wait(q_full, (nq - 1) & 1, nullptr, nullptr, p.wait_ns);
-    } else if (warp == 1) {
-      // ------------------------------------------------- MMA issue (whole warp, lane 0 issues)
+    } else if (warp == 1 && lane == 0) {
+      // ------------------------------------------------------------ MMA issue
+      // One thread, with nothing between the MMAs but adding to descriptors:
+      // a group of 8 occupies the tensor cores for 512 cycles, and they queue
+      // about half of one, so an issuer slower than that leaves them idle.
       constexpr uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128, false, false);
       constexpr uint32_t idesc_pv = make_idesc_f16(BF16, 128, D, false, true);
-      const uint32_t q_addr = smem_u32(sQ);
-      const uint32_t kv_addr = smem_u32(sKV);
-      int c0 = 0;           // loads of earlier items
+      const uint64_t qd = make_sw128_desc(smem_u32(sQ), 16, 1024);
+      const uint64_t kd = make_sw128_desc(smem_u32(sKV), 16, 1024);
+      const uint64_t vd = make_sw128_desc(smem_u32(sKV), C::CHUNK, 1024);
+      Ring<SL> ring;
       int nq = 0;           // non-empty items so far
       int np[2] = {0, 0};   // P tiles consumed, by stream
       int no[2] = {0, 0};   // items whose O this stream wrote
       bool ok = true;
+      auto landed = [&](const Ring<SL>& r) {
+        return ok = ok && mbar_wait(&full[r.st], r.ph, abort_flag, p.err, p.wait_ns);
+      };
       for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
         Item it;
         get_item(p, w, it);
         if (it.nk == 0) continue;
         const int n0 = steps_of(it, 0), n1 = steps_of(it, 1);
-        const int last_s = it.dual ? (it.nk - 1) & 1 : (n1 ? 1 : 0);  // stream of the item's last S and PV
-        auto issue_s = [&](int s, int i) {
-          const int at = c0 + k_at(it, tile_of(it, s, i)), st = at % SL;
-          if (!(ok = wait_all(&full[st], at / SL))) return;
+        const bool dual = it.dual;
+        const int last_s = dual ? (it.nk - 1) & 1 : (n1 ? 1 : 0);  // stream of the item's last S and PV
+        auto issue_s = [&](int s, const Ring<SL>& k, bool last) {
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t qa = q_addr + (it.dual ? 0 : s * C::TILE);
+          const uint64_t a = qd + (dual ? 0 : s * (C::TILE >> 4)), b = kd + k.st * (C::TILE >> 4);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * C::CHUNK + (kk & 3) * 32;
-              tc_mma_ss(tmem + s * 128, make_sw128_desc(qa + off, 16, 1024),
-                        make_sw128_desc(kv_addr + st * C::TILE + off, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
-            }
-            tc_commit(&s_full[s]);
-            if (s == last_s && i == (s ? n1 : n0) - 1) tc_commit(q_empty);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            constexpr int step = 2;  // 32 bytes
+            const int off = (kk >> 2) * (C::CHUNK >> 4) + (kk & 3) * step;
+            tc_mma_ss(tmem + s * 128, a + off, b + off, idesc_qk, kk > 0 ? 1u : 0u);
           }
-          __syncwarp();
+          tc_commit(&s_full[s]);
+          if (last && s == last_s) tc_commit(q_empty);
         };
-        auto issue_pv = [&](int s, int i) {
-          const int t = tile_of(it, s, i);
-          const int at = c0 + v_at(it, t), st = at % SL;
-          if (i == 0 && no[s] > 0 && !(ok = wait_all(&o_empty[s], no[s] - 1))) return;
-          if (!(ok = wait_all(&full[st], at / SL))) return;
-          const int tail = it.len - (it.k0 + t * 128);  // valid keys of this tile
-          if (tail < 128 && (it.dual || s == 0)) {
-            // V rows of keys past the length: zero (a row is 128 bytes of each chunk, whatever its swizzle)
-            uint8_t* vt = sKV + st * C::TILE;
-            for (int x = tail * 8 + lane; x < 128 * 8; x += 32) {
-#pragma unroll
-              for (int ch = 0; ch < C::NCHUNK; ++ch)
-                *reinterpret_cast<uint4*>(vt + ch * C::CHUNK + x * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-          if (!(ok = wait_all(&p_ready[s], np[s]))) return;
+        auto issue_pv = [&](int s, const Ring<SL>& v, bool first, bool last) {
+          if (first && no[s] > 0 && !(ok = ok && wait(&o_empty[s], no[s] - 1))) return;
+          if (!(ok = ok && wait(&p_ready[s], np[s]))) return;
           ++np[s];
           tc_fence_after();
-          const bool last = i == (s ? n1 : n0) - 1;
-          if (lane == 0) {
+          const uint64_t b = vd + v.st * (C::TILE >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              tc_mma_ts(tmem + C::O_COL + s * D, tmem + s * 128 + kk * 8,
-                        make_sw128_desc(kv_addr + st * C::TILE + kk * 16 * 128, C::CHUNK, 1024), idesc_pv,
-                        (i > 0 || kk > 0) ? 1u : 0u);
-            if (last) {
-              tc_commit(&o_final[s]);
-              // no later S of this stream tells the softmax that V is free
-              if (it.dual || s == last_s) tc_commit(&empty[st]);
+          for (int kk = 0; kk < 8; ++kk)
+            tc_mma_ts(tmem + C::O_COL + s * D, tmem + s * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_pv,
+                      (!first || kk > 0) ? 1u : 0u);
+          if (last) {
+            tc_commit(&o_final[s]);
+            // no later S of this stream tells the softmax that V is free
+            if (dual || s == last_s) tc_commit(&empty[v.st]);
+            ++no[s];
+          }
+        };
+        if (!(ok = wait(q_full, nq))) break;
+        ++nq;
+        Ring<SL> k = ring, v;
+        ring.next();
+        if (!landed(k)) break;
+        issue_s(0, k, n0 == 1);
+        if (n1 > 0) {
+          if (dual) {
+            k = ring;
+            ring.next();
+            if (!landed(k)) break;
+          }
+          issue_s(1, k, n1 == 1);
+        }
+        auto take_v = [&]() {
+          v = ring;
+          ring.next();
+          return landed(v);
+        };
+        auto take_k = [&]() {
+          k = ring;
+          ring.next();
+          return landed(k);
+        };
+        for (int i = 0; ok && i < n0; ++i) {
+          if (!take_v()) break;
+          issue_pv(0, v, i == 0, i == n0 - 1);
+          if (!ok) break;
+          if (i + 1 < n0) {
+            if (!take_k()) break;
+            issue_s(0, k, i + 2 == n0);
+          }
+          if (i < n1) {
+            if (dual && !take_v()) break;
+            issue_pv(1, v, i == 0, i == n1 - 1);
+            if (!ok) break;
+            if (i + 1 < n1) {
+              if (dual && !take_k()) break;
+              issue_s(1, k, i + 2 == n1);
             }
           }
-          __syncwarp();
-          if (last) ++no[s];
-        };
-        if (!(ok = wait_all(q_full, nq))) break;
-        ++nq;
-        issue_s(0, 0);
-        if (ok && n1 > 0) issue_s(1, 0);
-        for (int i = 0; ok && i < n0; ++i) {
-          issue_pv(0, i);
-          if (ok && i + 1 < n0) issue_s(0, i + 1);
-          if (ok && i < n1) issue_pv(1, i);
-          if (ok && i + 1 < n1) issue_s(1, i + 1);
         }
-        c0 += 2 * it.nk;
       }
-      if (lane == 0) {
-        tc_commit(drain);
-        mbar_wait(drain, 0, nullptr, nullptr, p.wait_ns);
-      }
-      __syncwarp();
+      tc_commit(drain);
+      mbar_wait(drain, 0, nullptr, nullptr, p.wait_ns);
     } else if (warp >= 2 && p.packed) {
       // ------------------------------------------------------ query rows of several heads
       int nq = 0;
@@ -546,6 +568,21 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           tmem_st32(s_base, pr);
           tmem_st32(s_base + 32, pr + 32);
           tmem_wait_st();
+        }
+        const int tail = it.len - (it.k0 + t * 128);
+        if (tail < 128 && (it.dual || s == 0)) {
+          // V rows past the length: zero before P V may start (a row is 128
+          // bytes of each chunk, whatever its swizzle).  This stage's earlier
+          // use was over before S_i, so the phase waited for is this load's.
+          const int at = c0 + v_at(it, t);
+          if (!(ok = wait_all(&full[at % SL], at / SL))) continue;
+          uint8_t* vt = sKV + (at % SL) * C::TILE;
+          for (int x = tail * 8 + row; x < 128 * 8; x += 128) {
+#pragma unroll
+            for (int ch = 0; ch < C::NCHUNK; ++ch)
+              *reinterpret_cast<uint4*>(vt + ch * C::CHUNK + x * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
         }
         tc_fence_before();
         __syncwarp();

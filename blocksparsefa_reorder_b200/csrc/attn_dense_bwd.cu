@@ -14,8 +14,8 @@
 //  * dK / dV: P_i^T ready -> dV += P_i^T dO_i, S_i+1^T (over P_i); dS_i^T ready
 //    -> dK += dS_i^T Q_i, dP_i+1^T (over dS_i).  The exponentials of step i+1
 //    run under the last two.
-// Roles of a CTA: warp 0 TMA producer, warp 1 MMA issue, warpgroups 1 and 2
-// elementwise: a row is shared by two threads, one of each warpgroup, with 64
+// Roles of a CTA: warp 0 TMA producer, warp 1 MMA issue (one thread each),
+// warpgroups 1 and 2 elementwise: a row is shared by two threads, one of each warpgroup, with 64
 // of the tile's 128 columns, so that each 16-bit result lies over columns its
 // own thread has read (columns 0-31 and 64-95 of the score buffer).
 // Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and all roles drain.
@@ -117,24 +117,25 @@ __device__ __forceinline__ void zero_half_row(int half, uint8_t* row) {
   for (int g = 0; g < D / 16; ++g) reinterpret_cast<uint4*>(row)[half * (D / 16) + g] = make_uint4(0, 0, 0, 0);
 }
 
-// C (+)= A B^T of two 128 x D shared-memory tiles (both K-major)
+// C (+)= A B^T of two 128 x D shared-memory tiles (K-major descriptors)
 template <int D>
-__device__ __forceinline__ void mma_abt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_abt(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
-    const uint32_t off = (kk >> 2) * DBwdCfg<D>::CHUNK + (kk & 3) * 32;
-    tc_mma_ss(d, make_sw128_desc(a + off, 16, 1024), make_sw128_desc(b + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+    const int off = (kk >> 2) * (DBwdCfg<D>::CHUNK >> 4) + (kk & 3) * 2;
+    tc_mma_ss(d, a + off, b + off, idesc, kk > 0 ? 1u : 0u);
   }
 }
 // C (+)= A B of a 128 x 128 16-bit A in tensor memory (columns 0-31 and
-// 64-95) and a 128 x D shared-memory tile (MN-major)
+// 64-95) and a 128 x D shared-memory tile (MN-major descriptor)
 template <int D>
-__device__ __forceinline__ void mma_ab(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+__device__ __forceinline__ void mma_ab(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool first) {
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    tc_mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, make_sw128_desc(b + kk * 16 * 128, DBwdCfg<D>::CHUNK, 1024), idesc,
-              (first && kk == 0) ? 0u : 1u);
+    tc_mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + kk * (16 * 128 >> 4), idesc, (first && kk == 0) ? 0u : 1u);
 }
+__device__ __forceinline__ uint64_t k_major(const void* t) { return make_sw128_desc(smem_u32(t), 16, 1024); }
+__device__ __forceinline__ uint64_t mn_major(const void* t) { return make_sw128_desc(smem_u32(t), 128 * 128, 1024); }
 
 // ---------------------------------------------------------------------------
 // dQ: one CTA per 128 query rows of one head, over the key tiles.
@@ -211,62 +212,39 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
     }
     mbar_wait(q_full, 0, nullptr, nullptr, p.wait_ns);
     for (int i = j > ST ? j - ST : 0; i < j; ++i) mbar_wait(&kv_full[i % ST], (i / ST) & 1, nullptr, nullptr, p.wait_ns);
-  } else if (warp == 1 && n > 0) {
+  } else if (warp == 1 && lane == 0 && n > 0) {
     // ------------------------------------------------------------ MMA issue
     constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
     constexpr uint32_t idesc_dq = make_idesc_f16(BF16, 128, D, false, true);
-    const uint32_t q_addr = smem_u32(sQ), do_addr = smem_u32(sDO), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
-    bool ok = wait_all(q_full, 0);
+    constexpr int TS = C::TILE >> 4;
+    const uint64_t qd = k_major(sQ), dod = k_major(sDO), kd = k_major(sK), vd = k_major(sV), kmn = mn_major(sK);
+    bool ok = wait(q_full, 0);
     auto issue_s = [&](int j) {
       const int st = j % ST;
-      if (!(ok = ok && wait_all(&kv_full[st], j / ST))) return;
-      const int tail = len - j * 128;
-      if (tail < 128) {
-        // K rows past the length: zero, for dS = 0 times what lies there
-        uint8_t* kt = sK + st * C::TILE;
-        for (int x = tail * 8 + lane; x < 128 * 8; x += 32) {
-#pragma unroll
-          for (int c = 0; c < C::NCHUNK; ++c)
-            *reinterpret_cast<uint4*>(kt + c * C::CHUNK + x * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
+      if (!(ok = ok && wait(&kv_full[st], j / ST))) return;
       tc_fence_after();
-      if (lane == 0) {
-        mma_abt<D>(tmem + (j & 1) * 128, q_addr, k_addr + st * C::TILE, idesc_s);
-        tc_commit(&s_full[j & 1]);
-      }
-      __syncwarp();
+      mma_abt<D>(tmem + (j & 1) * 128, qd, kd + st * TS, idesc_s);
+      tc_commit(&s_full[j & 1]);
     };
     auto issue_dp = [&](int j) {
-      if (lane == 0) {
-        mma_abt<D>(tmem + kDP, do_addr, v_addr + (j % ST) * C::TILE, idesc_s);
-        tc_commit(dp_full);
-      }
-      __syncwarp();
+      mma_abt<D>(tmem + kDP, dod, vd + (j % ST) * TS, idesc_s);
+      tc_commit(dp_full);
     };
     if (ok) issue_s(0);
     if (ok) issue_dp(0);
     if (ok && n > 1) issue_s(1);
     for (int j = 0; ok && j < n; ++j) {
-      if (!(ok = wait_all(ds_ready, j))) break;
+      if (!(ok = wait(ds_ready, j))) break;
       tc_fence_after();
       // dP's buffer is free (dS_j is written): step j+1 can go on
       if (j + 1 < n) issue_dp(j + 1);
-      if (lane == 0) {
-        mma_ab<D>(tmem + kDQ, tmem + (j & 1) * 128, k_addr + (j % ST) * C::TILE, idesc_dq, j == 0);
-        tc_commit(&kv_empty[j % ST]);
-      }
-      __syncwarp();
+      mma_ab<D>(tmem + kDQ, tmem + (j & 1) * 128, kmn + (j % ST) * TS, idesc_dq, j == 0);
+      tc_commit(&kv_empty[j % ST]);
       // over dS_j, which dQ_j (issued before) has read
       if (j + 2 < n) issue_s(j + 2);
     }
-    if (lane == 0) {
-      tc_commit(done);
-      mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
-    }
-    __syncwarp();
+    tc_commit(done);
+    mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
   } else if (warp >= 4) {
     // ------------------------------------------------- elementwise, epilogue
     const int q4 = warp & 3, half = (warp - 4) >> 2;
@@ -327,6 +305,17 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
           tmem_st16(lane_base + s_col + c * 16, ds);
         }
         tmem_wait_st();
+        if (j == n - 1 && (len & 127)) {
+          // K rows past the length: zero before dS K may start, for dS = 0 times
+          // what lies there (S_j, the tile's other reader, is complete)
+          uint8_t* kt = sK + (j % ST) * C::TILE;
+          for (int x = (len & 127) * 8 + (threadIdx.x - 128); x < 128 * 8; x += 256) {
+#pragma unroll
+            for (int c = 0; c < C::NCHUNK; ++c)
+              *reinterpret_cast<uint4*>(kt + c * C::CHUNK + x * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_ready);
@@ -426,50 +415,39 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     }
     mbar_wait(kv_full, 0, nullptr, nullptr, p.wait_ns);
     for (int k = i > ST ? i - ST : 0; k < i; ++k) mbar_wait(&qd_full[k % ST], (k / ST) & 1, nullptr, nullptr, p.wait_ns);
-  } else if (warp == 1 && n > 0) {
+  } else if (warp == 1 && lane == 0 && n > 0) {
     // ------------------------------------------------------------ MMA issue
     constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
     constexpr uint32_t idesc_acc = make_idesc_f16(BF16, 128, D, false, true);
-    const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV), q_addr = smem_u32(sQ), do_addr = smem_u32(sDO);
-    bool ok = wait_all(kv_full, 0);
+    constexpr int TS = C::TILE >> 4;
+    const uint64_t kd = k_major(sK), vd = k_major(sV), qd = k_major(sQ), dod = k_major(sDO);
+    const uint64_t qmn = mn_major(sQ), domn = mn_major(sDO);
+    bool ok = wait(kv_full, 0);
     auto issue_s = [&](int i) {
-      if (!(ok = ok && wait_all(&qd_full[i % ST], i / ST))) return;
+      if (!(ok = ok && wait(&qd_full[i % ST], i / ST))) return;
       tc_fence_after();
-      if (lane == 0) {
-        mma_abt<D>(tmem, k_addr, q_addr + (i % ST) * C::TILE, idesc_s);
-        tc_commit(s_full);
-      }
-      __syncwarp();
+      mma_abt<D>(tmem, kd, qd + (i % ST) * TS, idesc_s);
+      tc_commit(s_full);
     };
     auto issue_dp = [&](int i) {
-      if (lane == 0) {
-        mma_abt<D>(tmem + 128, v_addr, do_addr + (i % ST) * C::TILE, idesc_s);
-        tc_commit(dp_full);
-      }
-      __syncwarp();
+      mma_abt<D>(tmem + 128, vd, dod + (i % ST) * TS, idesc_s);
+      tc_commit(dp_full);
     };
     if (ok) issue_s(0);
     if (ok) issue_dp(0);
     for (int i = 0; ok && i < n; ++i) {
-      if (!(ok = wait_all(p_ready, i))) break;
+      if (!(ok = wait(p_ready, i))) break;
       tc_fence_after();
-      if (lane == 0) mma_ab<D>(tmem + 256, tmem, do_addr + (i % ST) * C::TILE, idesc_acc, i == 0);
-      __syncwarp();
+      mma_ab<D>(tmem + 256, tmem, domn + (i % ST) * TS, idesc_acc, i == 0);
       if (i + 1 < n) issue_s(i + 1);  // over P_i^T, which dV_i has read
-      if (!(ok = ok && wait_all(ds_ready, i))) break;
+      if (!(ok = ok && wait(ds_ready, i))) break;
       tc_fence_after();
-      if (lane == 0) {
-        mma_ab<D>(tmem + 256 + D, tmem + 128, q_addr + (i % ST) * C::TILE, idesc_acc, i == 0);
-        tc_commit(&qd_empty[i % ST]);
-      }
-      __syncwarp();
+      mma_ab<D>(tmem + 256 + D, tmem + 128, qmn + (i % ST) * TS, idesc_acc, i == 0);
+      tc_commit(&qd_empty[i % ST]);
       if (i + 1 < n) issue_dp(i + 1);  // over dS_i^T
     }
-    if (lane == 0) {
-      tc_commit(done);
-      mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
-    }
-    __syncwarp();
+    tc_commit(done);
+    mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
   } else if (warp >= 4) {
     // ------------------------------------------------- elementwise, epilogue
     const int q4 = warp & 3, half = (warp - 4) >> 2;

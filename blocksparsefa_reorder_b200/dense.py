@@ -23,27 +23,28 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .api import _DTYPES, _check_err, _require_cuda, _stream
+from .api import _DTYPES, _check_err, _require_cuda, on_device, raw_stream
 
 _INDEX = {torch.int32: _lib.INDEX_I32, torch.int64: _lib.INDEX_I64}
 _HALF = (torch.float16, torch.bfloat16)
 
 
-def _t4(t: torch.Tensor, name: str) -> _lib.Tensor4d:
-    if t.stride(-1) != 1:
+def _t4(t: torch.Tensor, name: str):
+    """Address and batch, head and token strides; heads or tokens expanded from
+    one are spread out before (:func:`_spread`)."""
+    s = t.stride()
+    if s[-1] != 1:
         raise ValueError(f"the last (head) dimension of {name} must be contiguous")
-    if t.dim() == 3:
-        return _lib.Tensor4d(t.data_ptr(), 0, t.stride(0), t.stride(1))
-    return _lib.Tensor4d(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), 0, s[0], s[1])
 
 
 def _spread(t: torch.Tensor) -> torch.Tensor:
     """Heads or tokens expanded from one (stride 0) get memory of their own: the
     TMA descriptors need real strides there.  An expanded batch is kept."""
-    d = t.dim()
-    if (t.stride(d - 3) == 0 and t.shape[d - 3] > 1) or (t.stride(d - 2) == 0 and t.shape[d - 2] > 1):
-        return t.contiguous()
-    return t
+    s = t.stride()
+    if s[-3] and s[-2]:
+        return t
+    return t.contiguous() if (not s[-3] and t.shape[-3] > 1) or (not s[-2] and t.shape[-2] > 1) else t
 
 
 def _check_tensors(q, others) -> None:
@@ -76,29 +77,37 @@ def _scale(sm_scale, D: int) -> float:
 
 
 def _outputs(q, out, return_lse: bool, lse_out):
-    o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if o.shape != q.shape or o.dtype != q.dtype or o.device != q.device:
-        raise ValueError("out has the wrong shape, dtype or device")
+    if out is None:
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        o = out
+        if o.shape != q.shape or o.dtype != q.dtype or o.device != q.device:
+            raise ValueError("out has the wrong shape, dtype or device")
     lse = None
     if return_lse or lse_out is not None:
         lse = lse_out if lse_out is not None else torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
+        if lse_out is not None and (lse.shape != q.shape[:3] or lse.dtype != torch.float32 or
+                                    not lse.is_contiguous() or lse.device != q.device):
             raise ValueError("lse_out must be a contiguous float32 [B, H, tokens] tensor on q's device")
     return o, lse
 
 
-def _launch(name: str, a, q, check_errors: bool) -> None:
+def _flag(check_errors: bool, device):
+    """(error word or None, its address)"""
+    if not check_errors:
+        return None, 0
+    err = torch.zeros(1, dtype=torch.int32, device=device)
+    return err, err.data_ptr()
+
+
+def _launch(name: str, query, call, a: bytes, device, err) -> None:
     """Workspace query, workspace, launch, optional device check."""
-    err = torch.zeros(1, dtype=torch.int32, device=q.device) if check_errors else None
-    a.err_flag = err.data_ptr() if err is not None else None
-    L = _lib.lib()
-    with torch.cuda.device(q.device):
+    with on_device(device):
         nbytes = ctypes.c_size_t()
-        ref = ctypes.byref(a)
-        _lib.check(getattr(L, f"bsa_{name}_workspace_bytes")(ref, ctypes.byref(nbytes)), f"bsa_{name}_workspace_bytes")
+        _lib.check(query(a, ctypes.byref(nbytes)), name)
         n = nbytes.value
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _lib.check(getattr(L, f"bsa_{name}")(ref, ws.data_ptr() if n else None, n, _stream(q.device)), f"bsa_{name}")
+        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        _lib.check(call(a, ws.data_ptr() if n else None, n, raw_stream(device)), name)
     _check_err(err, name)
 
 
@@ -141,15 +150,13 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, k_lens
     if B == 0 or M == 0 or H == 0:
         return (o, lse) if return_lse else o
     q, k, v = _spread(q), _spread(k), _spread(v)
-    a = _lib.CrossArgs()
-    a.B, a.H, a.Hk, a.M, a.N, a.D = B, H, Hk, M, N, D
-    a.dtype = _DTYPES[q.dtype]
-    a.q, a.o, a.k, a.v = _t4(q, "q"), _t4(o, "out"), _t4(k, "k"), _t4(v, "v")
-    if k_lens is not None:
-        a.k_lens, a.lens_dtype = k_lens.data_ptr(), _INDEX[k_lens.dtype]
-    a.lse = lse.data_ptr() if lse is not None else None
-    a.sm_scale = scale
-    _launch("cross_fwd", a, q, check_errors)
+    err, flag = _flag(check_errors, q.device)
+    a = _lib.CROSS_ARGS.pack(B, H, Hk, M, N, D, _DTYPES[q.dtype], _INDEX[k_lens.dtype] if k_lens is not None else 0,
+                             *_t4(q, "q"), *_t4(o, "out"), *_t4(k, "k"), *_t4(v, "v"),
+                             k_lens.data_ptr() if k_lens is not None else 0, lse.data_ptr() if lse is not None else 0,
+                             flag, scale)
+    L = _lib.lib()
+    _launch("bsa_cross_fwd", L.bsa_cross_fwd_workspace_bytes, L.bsa_cross_fwd, a, q.device, err)
     return (o, lse) if return_lse else o
 
 
@@ -171,26 +178,19 @@ def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse must be the forward's contiguous float32 [B, H, M] LSE")
     scale = _scale(sm_scale, D)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     if B == 0 or M == 0 or H == 0:
         return dq, dk.zero_(), dv.zero_()
-    q, k, v, dout = _spread(q), _spread(k), _spread(v), _spread(dout)
-    delta = torch.empty((B, H, M), dtype=torch.float32, device=q.device)
-    a = _lib.CrossBwdArgs()
-    a.B, a.H, a.Hk, a.M, a.N, a.D = B, H, Hk, M, N, D
-    a.dtype = _DTYPES[q.dtype]
-    a.q, a.k, a.v, a.o, a.dout = _t4(q, "q"), _t4(k, "k"), _t4(v, "v"), _t4(o, "o"), _t4(dout, "dout")
-    a.dq, a.dk, a.dv = _t4(dq, "dq"), _t4(dk, "dk"), _t4(dv, "dv")
-    if k_lens is not None:
-        a.k_lens, a.lens_dtype = k_lens.data_ptr(), _INDEX[k_lens.dtype]
-    a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
-    a.sm_scale = scale
-    err = torch.zeros(1, dtype=torch.int32, device=q.device) if check_errors else None
-    a.err_flag = err.data_ptr() if err is not None else None
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().bsa_cross_bwd(ctypes.byref(a), _stream(q.device)), "bsa_cross_bwd")
+    q, k, v, o, dout = _spread(q), _spread(k), _spread(v), _spread(o), _spread(dout)
+    delta = torch.empty_like(lse)
+    err, flag = _flag(check_errors, q.device)
+    a = _lib.CROSS_BWD_ARGS.pack(B, H, Hk, M, N, D, _DTYPES[q.dtype],
+                                 _INDEX[k_lens.dtype] if k_lens is not None else 0, *_t4(q, "q"), *_t4(k, "k"),
+                                 *_t4(v, "v"), *_t4(o, "o"), *_t4(dout, "dout"), *_t4(dq, "dq"), *_t4(dk, "dk"),
+                                 *_t4(dv, "dv"), k_lens.data_ptr() if k_lens is not None else 0, lse.data_ptr(),
+                                 delta.data_ptr(), flag, scale)
+    with on_device(q.device):
+        _lib.check(_lib.lib().bsa_cross_bwd(a, raw_stream(q.device)), "bsa_cross_bwd")
     _check_err(err, "cross_attention_backward")
     return dq, dk, dv
 
@@ -263,15 +263,12 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     if B == 0 or T == 0 or H == 0:
         return (o, lse) if return_lse else o
     q, k_prefix, v_prefix, k, v = (_spread(t) for t in (q, k_prefix, v_prefix, k, v))
-    a = _lib.PrefixArgs()
-    a.B, a.H, a.Hk, a.T, a.P, a.C, a.D = B, H, Hk, T, P, k.shape[2], D
-    a.dtype = _DTYPES[q.dtype]
-    a.q, a.o = _t4(q, "q"), _t4(o, "out")
-    a.k_prefix, a.v_prefix = _t4(k_prefix, "k_prefix"), _t4(v_prefix, "v_prefix")
-    a.k, a.v = _t4(k, "k"), _t4(v, "v")
-    if lens is not None:
-        a.lens, a.lens_dtype = lens.data_ptr(), _INDEX[lens.dtype]
-    a.lse = lse.data_ptr() if lse is not None else None
-    a.sm_scale = scale
-    _launch("prefix_fwd", a, q, check_errors)
+    err, flag = _flag(check_errors, q.device)
+    a = _lib.PREFIX_ARGS.pack(B, H, Hk, T, P, k.shape[2], D, _DTYPES[q.dtype],
+                              _INDEX[lens.dtype] if lens is not None else 0, *_t4(q, "q"), *_t4(o, "out"),
+                              *_t4(k_prefix, "k_prefix"), *_t4(v_prefix, "v_prefix"), *_t4(k, "k"), *_t4(v, "v"),
+                              lens.data_ptr() if lens is not None else 0, lse.data_ptr() if lse is not None else 0,
+                              flag, scale)
+    L = _lib.lib()
+    _launch("bsa_prefix_fwd", L.bsa_prefix_fwd_workspace_bytes, L.bsa_prefix_fwd, a, q.device, err)
     return (o, lse) if return_lse else o

@@ -14,12 +14,13 @@ them.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .api import _DTYPES, _check_err, _require_cuda, _stream
+from .api import _DTYPES, _check_err, _require_cuda, on_device, raw_stream
 
 _INDEX = {torch.int32: _lib.INDEX_I32, torch.int64: _lib.INDEX_I64}
 
@@ -37,100 +38,124 @@ def rope_table(length: int, dim: int, base: float = 10000.0, device="cuda"):
     return ang.cos().float(), ang.sin().float()
 
 
-def _check_side(x, w, name: str, like=None):
-    _require_cuda(x, name)
-    if x.dim() != 4:
-        raise ValueError(f"{name} must be [B, H, N, D], got {tuple(x.shape)}")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
-    if like is not None:
-        if (x.shape[0], x.shape[2], x.shape[3]) != (like.shape[0], like.shape[2], like.shape[3]):
-            raise ValueError(f"q and k must share B, N and D, got {tuple(like.shape)} and {tuple(x.shape)}")
-        if x.dtype != like.dtype:
-            raise TypeError(f"q and k must share a dtype, got {like.dtype} and {x.dtype}")
-        if x.device != like.device:
-            raise ValueError("q and k must be on one device")
-    if w is not None:
-        _require_cuda(w, f"{name}_weight")
-        if tuple(w.shape) != (x.shape[3],) or not w.is_contiguous():
-            raise ValueError(f"{name}_weight must be a contiguous [{x.shape[3]}] tensor, got {tuple(w.shape)}")
-        if w.dtype not in (torch.float32, x.dtype):
-            raise TypeError(f"{name}_weight must be float32 or {x.dtype}, got {w.dtype}")
-        if w.device != x.device:
-            raise ValueError(f"{name}_weight is on another device")
-
-
-def _t4(t: torch.Tensor, name: str) -> _lib.Tensor4d:
-    if t.stride(3) != 1 and t.shape[3] > 1:
+def _t4(t: torch.Tensor, name: str):
+    s = t.stride()
+    if s[3] != 1 and t.shape[3] > 1:
         raise ValueError(f"the last (head) dimension of {name} must be contiguous")
-    return _lib.Tensor4d(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    return t.data_ptr(), s[0], s[1], s[2]
 
 
-def _out(out, x, name: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise ValueError(f"{name} has the wrong shape, dtype or device")
-    return out
+def _check_weight(w, x, name: str) -> int:
+    _require_cuda(w, name)
+    if w.dim() != 1 or w.shape[0] != x.shape[3] or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{x.shape[3]}] tensor, got {tuple(w.shape)}")
+    if w.dtype != torch.float32 and w.dtype != x.dtype:
+        raise TypeError(f"{name} must be float32 or {x.dtype}, got {w.dtype}")
+    if w.device != x.device:
+        raise ValueError(f"{name} is on another device")
+    return w.data_ptr()
 
 
-def _args(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved):
-    """Checks, and the C arguments but for the outputs."""
-    if q is None and k is None:
-        raise ValueError("pass q or k")
-    if q is not None:
-        _check_side(q, q_weight, "q")
-    if k is not None:
-        _check_side(k, k_weight, "k", q)
-    x = q if q is not None else k
-    a = _lib.RopeArgs()
-    a.B, a.N, a.D = x.shape[0], x.shape[2], x.shape[3]
-    a.H = q.shape[1] if q is not None else 0
-    a.Hk = k.shape[1] if k is not None else 0
-    a.dtype = _DTYPES[x.dtype]
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise TypeError("q_weight and k_weight must share a dtype")
-    w = q_weight if q_weight is not None else k_weight
-    a.weight_dtype = _DTYPES[w.dtype] if w is not None else a.dtype
-    if q is not None:
-        a.q = _t4(q, "q")
-        a.q_weight = q_weight.data_ptr() if q_weight is not None else None
-    if k is not None:
-        a.k = _t4(k, "k")
-        a.k_weight = k_weight.data_ptr() if k_weight is not None else None
-    if not eps >= 0:
-        raise ValueError("eps must not be negative")
-    a.eps = eps
-    a.interleaved = 1 if interleaved else 0
-    if (cos is None) != (sin is None):
-        raise ValueError("pass both cos and sin, or neither (norm only)")
-    if cos is None:
-        if positions is not None:
-            raise ValueError("positions need the cos and sin tables")
-        return a, x
+def _check_tables(x, N: int, B: int, positions, cos, sin):
+    """(cos, sin, table_stride, table_len, R, positions, pos_dtype, pos_stride_b)"""
     for name, t in (("cos", cos), ("sin", sin)):
         _require_cuda(t, name)
         if t.dtype != torch.float32 or t.dim() != 2:
             raise TypeError(f"{name} must be a float32 [length, R / 2] table")
         if t.device != x.device:
             raise ValueError(f"{name} is on another device")
-    if cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1:
+    length, half = cos.shape
+    stride = cos.stride()
+    if sin.shape != cos.shape or sin.stride() != stride or (stride[1] != 1 and half > 1):
         raise ValueError("cos and sin must share their shape and strides, with contiguous rows")
-    a.R = 2 * cos.shape[1]
-    a.cos, a.sin, a.table_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    a.table_stride = max(cos.stride(0), cos.shape[1])
+    if half == 0 or length == 0:
+        raise ValueError("cos and sin must not be empty (pass None for the norm alone)")
+    pos, pos_dtype, pos_stride = 0, _lib.INDEX_I32, 0
     if positions is not None:
         _require_cuda(positions, "positions")
         if positions.dtype not in _INDEX:
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
         if positions.device != x.device:
             raise ValueError("positions are on another device")
-        if tuple(positions.shape) not in ((a.N,), (a.B, a.N)) or (positions.stride(-1) != 1 and a.N > 1):
-            raise ValueError(f"positions must be [{a.N}] or [{a.B}, {a.N}] with contiguous rows, "
-                             f"got {tuple(positions.shape)}")
-        a.positions, a.pos_dtype = positions.data_ptr(), _INDEX[positions.dtype]
-        a.pos_stride_b = positions.stride(0) if positions.dim() == 2 else 0
-    return a, x
+        shape = tuple(positions.shape)
+        if (shape != (N,) and shape != (B, N)) or (positions.stride(-1) != 1 and N > 1):
+            raise ValueError(f"positions must be [{N}] or [{B}, {N}] with contiguous rows, got {shape}")
+        pos, pos_dtype = positions.data_ptr(), _INDEX[positions.dtype]
+        pos_stride = positions.stride(0) if len(shape) == 2 else 0
+    return cos.data_ptr(), sin.data_ptr(), max(stride[0], half), length, 2 * half, pos, pos_dtype, pos_stride
+
+
+class _Call:
+    """The checked arguments of a forward or backward call."""
+
+    __slots__ = ("x", "B", "N", "D", "H", "Hk", "head", "q", "k", "weights", "table", "tail")
+
+    def __init__(self, q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved):
+        x = q if q is not None else k
+        if x is None:
+            raise ValueError("pass q or k")
+        for name, t in (("q", q), ("k", k)):
+            if t is None:
+                continue
+            _require_cuda(t, name)
+            if t.dim() != 4:
+                raise ValueError(f"{name} must be [B, H, N, D], got {tuple(t.shape)}")
+            if t.dtype not in _DTYPES:
+                raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+        B, _, N, D = x.shape
+        if q is not None and k is not None:
+            if k.shape[0] != B or k.shape[2] != N or k.shape[3] != D:
+                raise ValueError(f"q and k must share B, N and D, got {tuple(q.shape)} and {tuple(k.shape)}")
+            if k.dtype != q.dtype:
+                raise TypeError(f"q and k must share a dtype, got {q.dtype} and {k.dtype}")
+            if k.device != q.device:
+                raise ValueError("q and k must be on one device")
+        dtype = wdtype = _DTYPES[x.dtype]
+        wq = _check_weight(q_weight, q, "q_weight") if q is not None and q_weight is not None else 0
+        wk = _check_weight(k_weight, k, "k_weight") if k is not None and k_weight is not None else 0
+        if wq or wk:
+            if wq and wk and q_weight.dtype != k_weight.dtype:
+                raise TypeError("q_weight and k_weight must share a dtype")
+            wdtype = _DTYPES[(q_weight if wq else k_weight).dtype]
+        if not 0 <= eps < math.inf:
+            raise ValueError("eps must be finite and not negative")
+        if (cos is None) != (sin is None):
+            raise ValueError("pass both cos and sin, or neither (norm only)")
+        if cos is not None:
+            c, s, stride, length, R, pos, pos_dtype, pos_stride = _check_tables(x, N, B, positions, cos, sin)
+        elif positions is not None:
+            raise ValueError("positions need the cos and sin tables")
+        else:
+            c, s, stride, length, R, pos, pos_dtype, pos_stride = 0, 0, 0, 0, 0, 0, _lib.INDEX_I32, 0
+        self.x, self.B, self.N, self.D = x, B, N, D
+        self.H = q.shape[1] if q is not None else 0
+        self.Hk = k.shape[1] if k is not None else 0
+        self.head = (B, self.H, self.Hk, N, D, R, dtype, wdtype)
+        self.q = _t4(q, "q") if q is not None else _lib.NO_TENSOR
+        self.k = _t4(k, "k") if k is not None else _lib.NO_TENSOR
+        self.weights = (wq, wk)
+        self.table = (c, s, stride, length, pos_dtype, pos, pos_stride)
+        self.tail = (eps, 1 if interleaved else 0)
+
+    @property
+    def empty(self) -> bool:
+        return self.B == 0 or self.N == 0 or self.H + self.Hk == 0
+
+    def pack(self, q_out, k_out, dq_out, dk_out, dqw, dkw, err) -> bytes:
+        return _lib.ROPE_ARGS.pack(*self.head, *self.q, *self.k, *q_out, *k_out, *dq_out, *dk_out, *self.weights,
+                                   *self.table, *self.tail, dqw, dkw, err.data_ptr() if err is not None else 0)
+
+
+def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _out(out, x, name: str) -> torch.Tensor:
+    if out is None:
+        return _contiguous_like(x)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{name} has the wrong shape, dtype or device")
+    return out
 
 
 def qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor] = None,
@@ -153,20 +178,19 @@ def qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], q_weight:
     themselves.  Returns ``(q_out, k_out)``; sums, norm and rotation are fp32,
     rounded once.
     """
-    a, x = _args(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
+    c = _Call(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
     oq, ok = out if out is not None else (None, None)
     oq = _out(oq, q, "q_out") if q is not None else None
     ok = _out(ok, k, "k_out") if k is not None else None
-    if x.shape[0] == 0 or x.shape[2] == 0 or a.H + a.Hk == 0:
+    if c.empty:
         return oq, ok
-    if oq is not None:
-        a.q_out = _t4(oq, "q_out")
-    if ok is not None:
-        a.k_out = _t4(ok, "k_out")
-    err = torch.zeros(1, dtype=torch.int32, device=x.device) if check_errors else None
-    a.err_flag = err.data_ptr() if err is not None else None
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().bsa_qk_norm_rope(ctypes.byref(a), _stream(x.device)), "bsa_qk_norm_rope")
+    device = c.x.device
+    err = torch.zeros(1, dtype=torch.int32, device=device) if check_errors else None
+    none = _lib.NO_TENSOR
+    a = c.pack(_t4(oq, "q_out") if oq is not None else none, _t4(ok, "k_out") if ok is not None else none, none, none,
+               0, 0, err)
+    with on_device(device):
+        _lib.check(_lib.lib().bsa_qk_norm_rope(a, raw_stream(device)), "bsa_qk_norm_rope")
     _check_err(err, "qk_norm_rope")
     return oq, ok
 
@@ -180,39 +204,37 @@ def qk_norm_rope_backward(dq_out: Optional[torch.Tensor], dk_out: Optional[torch
     ``dk_out`` (the forward's inputs again, same keywords): returns
     ``dq, dk, dq_weight, dk_weight`` (None for what is absent).  The weights'
     gradients are summed over batch, heads and tokens in fp32 in a fixed order."""
-    a, x = _args(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
-    outs = []
-    for name, t, g, w in (("q", q, dq_out, q_weight), ("k", k, dk_out, k_weight)):
+    c = _Call(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
+    dx, dw, outs, grads = [None, None], [None, None], [_lib.NO_TENSOR] * 2, [_lib.NO_TENSOR] * 2
+    for i, (name, t, g, w) in enumerate((("q", q, dq_out, q_weight), ("k", k, dk_out, k_weight))):
         if t is None:
-            outs += [None, None]
             continue
         _require_cuda(g, f"d{name}_out")
         if g.shape != t.shape or g.dtype != t.dtype or g.device != t.device:
             raise ValueError(f"d{name}_out must have {name}'s shape, dtype and device")
-        dx = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        dw = torch.empty_like(w) if w is not None else None
-        outs += [dx, dw]
-        setattr(a, f"{name}_out", _t4(dx, f"d{name}"))
-        setattr(a, f"d{name}_out", _t4(g, f"d{name}_out"))
-        setattr(a, f"d{name}_weight", dw.data_ptr() if dw is not None else None)
-    dq, dqw, dk, dkw = outs
-    if x.shape[0] == 0 or x.shape[2] == 0 or a.H + a.Hk == 0:
-        for dw in (dqw, dkw):
-            if dw is not None:
-                dw.zero_()
-        return dq, dk, dqw, dkw
-    err = torch.zeros(1, dtype=torch.int32, device=x.device) if check_errors else None
-    a.err_flag = err.data_ptr() if err is not None else None
+        dx[i] = _contiguous_like(t)
+        outs[i], grads[i] = _t4(dx[i], f"d{name}"), _t4(g, f"d{name}_out")
+        if w is not None:
+            dw[i] = torch.empty_like(w)
+    if c.empty:
+        for t in dw:
+            if t is not None:
+                t.zero_()
+        return (*dx, *dw)
+    device = c.x.device
+    err = torch.zeros(1, dtype=torch.int32, device=device) if check_errors else None
+    a = c.pack(*outs, *grads, *(t.data_ptr() if t is not None else 0 for t in dw), err)
     L = _lib.lib()
-    with torch.cuda.device(x.device):
+    with on_device(device):
         nbytes = ctypes.c_size_t()
-        _lib.check(L.bsa_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(nbytes)),
+        _lib.check(L.bsa_qk_norm_rope_bwd_workspace_bytes(a, ctypes.byref(nbytes)),
                    "bsa_qk_norm_rope_bwd_workspace_bytes")
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device) if nbytes.value else None
-        _lib.check(L.bsa_qk_norm_rope_bwd(ctypes.byref(a), ws.data_ptr() if ws is not None else None, nbytes.value,
-                                          _stream(x.device)), "bsa_qk_norm_rope_bwd")
+        n = nbytes.value
+        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        _lib.check(L.bsa_qk_norm_rope_bwd(a, ws.data_ptr() if n else None, n, raw_stream(device)),
+                   "bsa_qk_norm_rope_bwd")
     _check_err(err, "qk_norm_rope_backward")
-    return dq, dk, dqw, dkw
+    return (*dx, *dw)
 
 
 def _rows(g: torch.Tensor) -> torch.Tensor:
