@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // warp-uniform for the compiler too
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       // every load issued lands before the CTA exits
       for (int i = c > SL ? c - SL : 0; i < c; ++i) mbar_wait(&full[i % SL], (i / SL) & 1, nullptr, nullptr, p.wait_ns);
       if (!p.packed && nq > 0) mbar_wait(q_full, (nq - 1) & 1, nullptr, nullptr, p.wait_ns);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issue
       // One thread, with nothing between the MMAs but adding to descriptors:
       // a group of 8 occupies the tensor cores for 512 cycles, and they queue
@@ -347,11 +347,11 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       const uint64_t vd = make_sw128_desc(smem_u32(sKV), C::CHUNK, 1024);
       Ring<SL> ring;
       int nq = 0;           // non-empty items so far
-      int np[2] = {0, 0};   // P tiles consumed, by stream
-      int no[2] = {0, 0};   // items whose O this stream wrote
+      // by stream: P tiles consumed, items whose O it wrote
+      int np0 = 0, np1 = 0, no0 = 0, no1 = 0;
       bool ok = true;
       auto landed = [&](const Ring<SL>& r) {
-        return ok = ok && mbar_wait(&full[r.st], r.ph, abort_flag, p.err, p.wait_ns);
+        return ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[r.st], r.ph, abort_flag, p.err, p.wait_ns));
       };
       for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
         Item it;
@@ -363,33 +363,38 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         auto issue_s = [&](int s, const Ring<SL>& k, bool last) {
           tc_fence_after();
           const uint64_t a = qd + (dual ? 0 : s * (C::TILE >> 4)), b = kd + k.st * (C::TILE >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            constexpr int step = 2;  // 32 bytes
-            const int off = (kk >> 2) * (C::CHUNK >> 4) + (kk & 3) * step;
-            tc_mma_ss(tmem + s * 128, a + off, b + off, idesc_qk, kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const int off = (kk >> 2) * (C::CHUNK >> 4) + (kk & 3) * 2;  // 32 bytes inside a chunk's rows
+              tc_mma_ss(tmem + s * 128, a + off, b + off, idesc_qk, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(&s_full[s]);
+            if (last && s == last_s) tc_commit(q_empty);
           }
-          tc_commit(&s_full[s]);
-          if (last && s == last_s) tc_commit(q_empty);
+          __syncwarp();
         };
-        auto issue_pv = [&](int s, const Ring<SL>& v, bool first, bool last) {
-          if (first && no[s] > 0 && !(ok = ok && wait(&o_empty[s], no[s] - 1))) return;
-          if (!(ok = ok && wait(&p_ready[s], np[s]))) return;
-          ++np[s];
+        auto issue_pv = [&](int s, int& np, int& no, const Ring<SL>& v, bool first, bool last) {
+          if (first && no > 0 && !(ok = ok && wait_all(&o_empty[s], no - 1))) return;
+          if (!(ok = ok && wait_all(&p_ready[s], np))) return;
+          ++np;
           tc_fence_after();
           const uint64_t b = vd + v.st * (C::TILE >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            tc_mma_ts(tmem + C::O_COL + s * D, tmem + s * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_pv,
-                      (!first || kk > 0) ? 1u : 0u);
-          if (last) {
-            tc_commit(&o_final[s]);
-            // no later S of this stream tells the softmax that V is free
-            if (dual || s == last_s) tc_commit(&empty[v.st]);
-            ++no[s];
+            for (int kk = 0; kk < 8; ++kk)
+              tc_mma_ts(tmem + C::O_COL + s * D, tmem + s * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_pv,
+                        (!first || kk > 0) ? 1u : 0u);
+            if (last) {
+              tc_commit(&o_final[s]);
+              // no later S of this stream tells the softmax that V is free
+              if (dual || s == last_s) tc_commit(&empty[v.st]);
+            }
           }
+          __syncwarp();
+          if (last) ++no;
         };
-        if (!(ok = wait(q_full, nq))) break;
+        if (!(ok = wait_all(q_full, nq))) break;
         ++nq;
         Ring<SL> k = ring, v;
         ring.next();
@@ -415,7 +420,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         };
         for (int i = 0; ok && i < n0; ++i) {
           if (!take_v()) break;
-          issue_pv(0, v, i == 0, i == n0 - 1);
+          issue_pv(0, np0, no0, v, i == 0, i == n0 - 1);
           if (!ok) break;
           if (i + 1 < n0) {
             if (!take_k()) break;
@@ -423,7 +428,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           }
           if (i < n1) {
             if (dual && !take_v()) break;
-            issue_pv(1, v, i == 0, i == n1 - 1);
+            issue_pv(1, np1, no1, v, i == 0, i == n1 - 1);
             if (!ok) break;
             if (i + 1 < n1) {
               if (dual && !take_k()) break;
@@ -432,8 +437,11 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           }
         }
       }
-      tc_commit(drain);
-      mbar_wait(drain, 0, nullptr, nullptr, p.wait_ns);
+      if (elect_one()) {
+        tc_commit(drain);
+        mbar_wait(drain, 0, nullptr, nullptr, p.wait_ns);
+      }
+      __syncwarp();
     } else if (warp >= 2 && p.packed) {
       // ------------------------------------------------------ query rows of several heads
       int nq = 0;
@@ -484,6 +492,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         continue;
       }
       const bool releases = it.dual || it.rows <= 128 || s == 1;  // last reader of the shared tiles
+      int kst = (c0 + k_at(it, tile_of(it, s, 0))) % SL;  // stage of the step's K; its V of the step before is one below
       const int r = it.dual ? row : s * 128 + row;
       // a warp without rows only keeps the barriers going
       const bool any_rows = (it.dual ? 0 : s * 128) + q4 * 32 < it.rows;
@@ -497,11 +506,13 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         if (!(ok = ok && wait_all(&s_full[s], ns))) continue;
         tc_fence_after();
         const int t = tile_of(it, s, i);
-        if (q4 == 0 && lane == 0 && releases) {
-          // S_i complete, and with it the PV of the step before
-          mbar_arrive(&empty[(c0 + k_at(it, t)) % SL]);
-          if (i > 0) mbar_arrive(&empty[(c0 + v_at(it, tile_of(it, s, i - 1))) % SL]);
+        // S_i complete, and with it the PV of the step before: K_i and V_i-1 are free
+        if (lane == 0 && releases) {
+          if (q4 == 0) mbar_arrive(&empty[kst]);
+          if (q4 == 1 && i > 0) mbar_arrive(&empty[kst ? kst - 1 : SL - 1]);
         }
+        kst += it.dual ? (t ? 4 : 3) : 2;
+        kst -= kst >= SL ? SL : 0;
         if (any_rows) {
           const int valid = limit - (it.k0 + t * 128);  // keys of this tile the row sees
           const bool mask = __any_sync(0xffffffffu, valid < 128);
@@ -525,7 +536,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
             return mx * p.scale_log2;
           };
           uint32_t pr[64];
-          auto exps = [&]() {
+          auto exps = [&](bool mixed) {
             // a row that has seen nothing yet keeps m = -inf: its exponentials are 2^(-inf - 0) = 0
             const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
             float sum = 0.f;
@@ -533,7 +544,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
             for (int ch = 0; ch < 4; ++ch) {
               uint32_t v[32], pp[16];
               load(ch, v);
-              sum += exp_block<32, BF16>(v, pp, p.scale_log2, neg_m);
+              sum += mixed ? exp_block_mixed<32, BF16>(v, pp, p.scale_log2, neg_m)
+                           : exp_block<32, BF16>(v, pp, p.scale_log2, neg_m);
 #pragma unroll
               for (int k = 0; k < 16; ++k) pr[ch * 16 + k] = pp[k];
             }
@@ -545,13 +557,17 @@ __global__ void __launch_bounds__(kThreadsD, 1)
             const float mx = tile_max();
             if (m_run == -INFINITY) m_run = mx;
           }
-          float ls = exps();
+          float ls;
+          if (mask || __any_sync(0xffffffffu, m_run == -INFINITY))
+            ls = exps(false);
+          else
+            ls = exps(true);
           if (__any_sync(0xffffffffu, !(ls <= ref_slack<BF16>()))) {
             const float m_new = fmaxf(m_run, tile_max());
             const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m_run - m_new);
             l_run *= alpha;
             m_run = m_new;
-            ls = exps();
+            ls = exps(false);
             if (i > 0) {
 #pragma unroll
               for (int ch = 0; ch < D / 32; ++ch) {
