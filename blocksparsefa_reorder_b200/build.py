@@ -25,7 +25,7 @@ BUILD_DIR = PKG / "_build"
 LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libbsattn_b200.so"
 SOURCES = ["api.cu", "preprocess.cu", "attn_simt.cu", "tma_maps.cu", "attn_tcp.cu", "attn_bwd.cu",
-           "plan_noalloc.cu", "qk_norm_rope.cu", "attn_dense.cu",
+           "plan_noalloc.cu", "qk_norm_rope.cu", "attn_dense.cu", "attn_few.cu",
            "attn_dense_bwd.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

@@ -42,6 +42,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "dense.h"
 #include "internal.h"
 #include "softmax.cuh"
 
@@ -60,17 +61,15 @@ constexpr int kRegsSplitD = kRegsIssueD + 2 * kRegsSoftmaxD + kRegsEpilogueD;
 static_assert(128 * kRegsSplitD <= kThreadsD * kRegsLaunchD, "register split");
 
 // One source of keys.  Row r of a unit is query (sequence, head, token):
-// with `seqs` sequences in a unit, r = (seq * G + g) * M + m.
+// r = (seq * G + g) * M + m.
 struct DensePart {
-  int units;       // seqs == 1: B * Hk, else Hk
-  int seqs;        // sequences whose rows one unit holds
-  int rows;        // seqs * G * M
+  int rows;        // of a unit: seqs * G * M
   int tiles;       // row tiles of a unit
   int splits;      // key ranges
   int chunk;       // key tiles of a range
   int keys;        // keys the tensors hold
   int items;       // units * tiles * splits
-  int shared_kv;   // the unit's K / V do not depend on the sequence
+  int shared_kv;   // a unit's keys serve every sequence (units: Hk, else B * Hk)
   int kb_mul;      // 0: K / V batch stride 0 (one copy for the batch)
   int vb_mul;
   int causal;      // query m of M sees keys below len - (M - 1 - m)
@@ -86,6 +85,7 @@ struct DenseParams {
   int lens_i64;
   int packed;      // query rows gathered by warps 2-3 (fewer than 128 queries a head)
   int dual;        // bit i: part i runs both streams over the same rows
+  int qb_mul;      // 0: the queries' batch stride is 0
   const uint8_t* q;
   int64_t qs_b, qs_h, qs_n;
   uint8_t* o;
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
   // set-up above touched this CTA's shared and tensor memory alone
   grid_dependency_wait();
 
-  const int total = p.part[0].items + (p.nparts > 1 ? p.part[1].items : 0);
+  const int total = p.part[0].items + p.part[1].items;
   auto wait = [&](uint64_t* bar, int n) { return mbar_wait(bar, n & 1, abort_flag, p.err, p.wait_ns); };
   auto wait_all = [&](uint64_t* bar, int n) { return __all_sync(0xffffffffu, wait(bar, n)) != 0; };
 
@@ -321,7 +321,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           mbar_arrive_expect_tx(q_full, nsub * C::TILE);
           for (int s = 0; s < nsub; ++s)
             for (int ch = 0; ch < C::NCHUNK; ++ch)
-              tma_load_4d(sQ + s * C::TILE + ch * C::CHUNK, &tmQ, q_full, ch * 64, it.m0 + s * 128, it.qh, it.qb);
+              tma_load_4d(sQ + s * C::TILE + ch * C::CHUNK, &tmQ, q_full, ch * 64, it.m0 + s * 128, it.qh,
+                          it.qb * p.qb_mul);
         }
         ++nq;
         const int ahead = it.dual ? 2 : 1;
@@ -540,14 +541,25 @@ __global__ void __launch_bounds__(kThreadsD, 1)
             // a row that has seen nothing yet keeps m = -inf: its exponentials are 2^(-inf - 0) = 0
             const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
             float sum = 0.f;
+            uint32_t buf[2][32];
+            tmem_ld32(s_base, buf[0]);
+            tmem_wait_ld32(buf[0]);
 #pragma unroll
             for (int ch = 0; ch < 4; ++ch) {
-              uint32_t v[32], pp[16];
-              load(ch, v);
+              // the next 32 columns come while these are exponentiated
+              uint32_t (&v)[32] = buf[ch & 1];
+              uint32_t pp[16];
+              if (ch < 3) tmem_ld32(s_base + (ch + 1) * 32, buf[(ch + 1) & 1]);
+              if (mask) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (ch * 32 + k >= valid) v[k] = __float_as_uint(-INFINITY);
+              }
               sum += mixed ? exp_block_mixed<32, BF16>(v, pp, p.scale_log2, neg_m)
                            : exp_block<32, BF16>(v, pp, p.scale_log2, neg_m);
 #pragma unroll
               for (int k = 0; k < 16; ++k) pr[ch * 16 + k] = pp[k];
+              if (ch < 3) tmem_wait_ld32(buf[(ch + 1) & 1]);
             }
             return sum;
           };
@@ -819,75 +831,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const JoinParams p) {
 // Host: splitting, workspace, launch.
 // ---------------------------------------------------------------------------
 constexpr int kSMs = 148;
-constexpr int kMaxSplits = 128;
-// An item's fixed cost in key tiles (query load, first scores, epilogue), and
-// what a second launch that joins costs, as measured (see the split rule).
-constexpr int kItemCost = 3;
-constexpr int kJoinCost = 3;
 
 size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
-
-struct Shape {
-  int units, rows, tiles, keys;
-  bool dual;
-};
-
-// One source of keys for `seqs` sequences a unit.
-Shape shape_of(int B, int H, int Hk, int M, int keys, bool shared_kv) {
-  Shape s;
-  const int G = H / Hk, seqs = shared_kv ? B : 1;
-  s.units = shared_kv ? Hk : B * Hk;
-  s.rows = seqs * G * M;
-  const bool packed = M < 128;
-  const int64_t one = packed ? s.rows : M;  // rows that can share a tile
-  s.dual = one <= 128;
-  const int per = s.dual ? 128 : 256;
-  s.tiles = static_cast<int>(packed ? (one + per - 1) / per : static_cast<int64_t>(seqs) * G * ((M + per - 1) / per));
-  s.keys = keys;
-  return s;
-}
-
-// Key tiles of a range, the same for all sources: the smallest of
-//   ceil(cost of all items / SMs) (every SM busy) or the longest item,
-// over all range lengths, with the join's cost once anything is split.
-int choose_chunk(const Shape* s, int n) {
-  int longest = 1;
-  for (int i = 0; i < n; ++i) longest = longest > (s[i].keys + 127) / 128 ? longest : (s[i].keys + 127) / 128;
-  int best = longest;
-  double best_cost = 1e30;
-  for (int c = longest; c >= 1; --c) {
-    double items = 0, work = 0;
-    int most = 0;
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int nk = (s[i].keys + 127) / 128;
-      const int splits = nk ? (nk + c - 1) / c : 1;
-      if (splits > kMaxSplits) ok = false;
-      const double per = static_cast<double>(s[i].units) * s[i].tiles;
-      // (a dual item does two key tiles at a time)
-      const double t = (s[i].dual ? (nk + 1) / 2 : nk) + static_cast<double>(splits) * kItemCost;
-      items += per * splits;
-      work += per * t;
-      const int one = (s[i].dual ? (c + 1) / 2 : c) + kItemCost;
-      if (nk && one > most) most = one;
-    }
-    if (!ok) break;
-    if (items > 2.0e9) break;
-    const double waves = static_cast<double>(static_cast<int64_t>((items + kSMs - 1) / kSMs));
-    double cost = work / kSMs;
-    // the last wave: whole items on part of the SMs
-    if (waves * most < 3.0 * cost && waves * most > cost) cost = waves * most;
-    if (cost < most) cost = most;
-    if (n > 1 || c < longest) cost += kJoinCost;
-    if (cost < best_cost * 0.999) best_cost = cost, best = c;
-  }
-  return best;
-}
 
 struct DenseCall {
   int B, H, Hk, M, D, dtype;
   bsa_tensor4d q, o;
-  int n;                      // sources
+  int n;                      // sources of keys
   bsa_tensor4d k[2], v[2];
   int keys[2];
   bool shared_kv[2], causal[2];
@@ -898,29 +848,110 @@ struct DenseCall {
   int32_t* err;
 };
 
-// Layout of the workspace: per split source its partial o, then its lse.
-struct DensePlan {
-  Shape s[2];
-  int chunk, splits[2];
-  bool join;
-  size_t o_off[2], lse_off[2], total;
+// How one source is computed.
+struct Source {
+  bool few;                   // attn_few.cu
+  bool dual;                  // both streams over the same rows
+  int units, rows, tiles;
+  int splits, chunk;          // key ranges; key tiles (few: keys) of each
+  size_t o_off, lse_off;      // partial results in the workspace
 };
+struct DensePlan {
+  Source s[2];
+  bool join;
+  size_t total;
+};
+
+Source source_of(const DenseCall& c, int i) {
+  Source s{};
+  const int G = c.H / c.Hk, seqs = c.shared_kv[i] ? c.B : 1;
+  s.units = c.shared_kv[i] ? c.Hk : c.B * c.Hk;
+  s.rows = seqs * G * c.M;
+  s.few = s.rows <= kFewRows;
+  const bool packed = c.M < 128;
+  const int one = packed ? s.rows : c.M;  // rows that can share a tile
+  s.dual = one <= 128;
+  const int per = s.dual ? 128 : 256;
+  s.tiles = packed ? (one + per - 1) / per : seqs * G * ((c.M + per - 1) / per);
+  s.splits = 1;
+  return s;
+}
+
+// The few-rows kernel: two CTAs an SM, whose time is their bytes.  Where the
+// units alone do not fill the SMs, or a range is so long that ragged lengths
+// would leave some of them busy alone at the end, the keys are split into about
+// eight ranges an SM of at least 256 keys (a warp's share is then two blocks of
+// 16).  (4 x 8 units of up to 65,536 keys: 4, 8, 16 ranges an SM 128, 122, 124
+// us; 256 units of 1,500 keys: one range 14 us, two and a join 17 us.)
+void split_few(Source* s, int keys) {
+  s->chunk = keys > 0 ? keys : 1;
+  if (s->units < kSMs || keys > 8192) {
+    const int64_t c = (static_cast<int64_t>(keys) * s->units + 8 * kSMs - 1) / (8 * kSMs);
+    s->chunk = static_cast<int>(c < 256 ? 256 : (c + 127) / 128 * 128);
+  }
+  s->splits = keys > 0 ? (keys + s->chunk - 1) / s->chunk : 1;
+}
+
+// The tensor-core kernel: one CTA an SM.  A step (one key tile of 256 rows, or
+// two of 128 rows) takes about 1.9 us, an item 4 us beside its steps, the join
+// 3 us and the partial results' way through memory.  The number of ranges is
+// the one of least
+//   waves x longest item + join
+// (16 heads x 4096 rows x 16,384 keys, 256 items: whole 548 us, halves 590 us;
+// 8 units of 256 rows x 32,768 keys: 18 ranges each).
+void split_dense(Source* s, const int* keys, int n, int D, bool must_join) {
+  int longest = 0;
+  for (int i = 0; i < n; ++i)
+    if (!s[i].few && (keys[i] + 127) / 128 > longest) longest = (keys[i] + 127) / 128;
+  int best = longest > 0 ? longest : 1;
+  double best_cost = 1e30;
+  const int most = longest < 128 ? longest : 128;
+  for (int k = 1; k <= most; ++k) {
+    const int c = (longest + k - 1) / k;
+    double work = 0, top = 0, bytes = 0, items = 0;
+    for (int i = 0; i < n; ++i) {
+      if (s[i].few) continue;
+      const int nk = (keys[i] + 127) / 128;
+      const int sp = nk ? (nk + c - 1) / c : 1;
+      const double per = static_cast<double>(s[i].units) * s[i].tiles * sp;
+      const int len = nk < c ? nk : c;
+      const double t = 1.9 * (s[i].dual ? (len + 1) / 2 : len) + 4.0;
+      work += per * t;
+      items += per;
+      top = t > top ? t : top;
+      bytes += static_cast<double>(s[i].units) * s[i].rows * sp * D * 8.0;
+    }
+    if (items > 2.0e9) break;
+    double cost = static_cast<double>(static_cast<int64_t>(work / (kSMs * top) + 0.999)) * top;
+    if (k > 1 || must_join) cost += 3.0 + bytes / 5.0e6;
+    if (cost < best_cost) best_cost = cost, best = c;
+  }
+  for (int i = 0; i < n; ++i) {
+    if (s[i].few) continue;
+    const int nk = (keys[i] + 127) / 128;
+    s[i].chunk = best;
+    s[i].splits = nk ? (nk + best - 1) / best : 1;
+  }
+}
 
 DensePlan plan_of(const DenseCall& c) {
   DensePlan pl{};
-  for (int i = 0; i < c.n; ++i) pl.s[i] = shape_of(c.B, c.H, c.Hk, c.M, c.keys[i], c.shared_kv[i]);
-  pl.chunk = choose_chunk(pl.s, c.n);
+  bool dense = false;
   for (int i = 0; i < c.n; ++i) {
-    const int nk = (c.keys[i] + 127) / 128;
-    pl.splits[i] = nk ? (nk + pl.chunk - 1) / pl.chunk : 1;
+    pl.s[i] = source_of(c, i);
+    if (pl.s[i].few)
+      split_few(&pl.s[i], c.keys[i]);
+    else
+      dense = true;
   }
-  pl.join = c.n > 1 || pl.splits[0] > 1;
+  if (dense) split_dense(pl.s, c.keys, c.n, c.D, c.n > 1);
+  pl.join = c.n > 1 || pl.s[0].splits > 1;
   size_t off = 0;
   for (int i = 0; pl.join && i < c.n; ++i) {
-    const size_t rows = static_cast<size_t>(pl.s[i].units) * pl.s[i].rows * pl.splits[i];
-    pl.o_off[i] = off;
+    const size_t rows = static_cast<size_t>(pl.s[i].units) * pl.s[i].rows * pl.s[i].splits;
+    pl.s[i].o_off = off;
     off += round256(rows * c.D * sizeof(float));
-    pl.lse_off[i] = off;
+    pl.s[i].lse_off = off;
     off += round256(rows * sizeof(float));
   }
   pl.total = off;
@@ -938,64 +969,86 @@ int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16
   return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, 128);
 }
 
+cudaLaunchConfig_t config(unsigned grid, int threads, int smem, cudaStream_t st, cudaLaunchAttribute* attr) {
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+float* part_o(const Source& s, uint8_t* ws) { return reinterpret_cast<float*>(ws + s.o_off); }
+float* part_lse(const Source& s, uint8_t* ws) { return reinterpret_cast<float*>(ws + s.lse_off); }
+
+int launch_few(const DenseCall& c, const DensePlan& pl, int i, uint8_t* ws, cudaStream_t st) {
+  const Source& s = pl.s[i];
+  FewParams p{};
+  p.units = s.units, p.rows = s.rows, p.splits = s.splits, p.chunk = s.chunk, p.keys = c.keys[i];
+  p.shared_kv = c.shared_kv[i], p.causal = c.causal[i];
+  p.H = c.H, p.Hk = c.Hk, p.G = c.H / c.Hk, p.M = c.M;
+  p.lens = c.lens[i], p.lens_i64 = c.lens_dtype == BSA_INDEX_I64;
+  p.q = static_cast<const uint8_t*>(c.q.data);
+  p.k = static_cast<const uint8_t*>(c.k[i].data);
+  p.v = static_cast<const uint8_t*>(c.v[i].data);
+  p.qs_b = c.q.stride_b, p.qs_h = c.q.stride_h, p.qs_n = c.q.stride_n;
+  p.ks_b = c.k[i].stride_b, p.ks_h = c.k[i].stride_h, p.ks_n = c.k[i].stride_n;
+  p.vs_b = c.v[i].stride_b, p.vs_h = c.v[i].stride_h, p.vs_n = c.v[i].stride_n;
+  p.o = static_cast<uint8_t*>(c.o.data);
+  p.os_b = c.o.stride_b, p.os_h = c.o.stride_h, p.os_n = c.o.stride_n;
+  p.lse = c.lse;
+  if (pl.join) p.part_o = part_o(s, ws), p.part_lse = part_lse(s, ws);
+  p.scale_log2 = c.sm_scale * 1.4426950408889634f;
+  p.err = c.err;
+  return launch_attn_few(p, c.D, c.dtype == BSA_DTYPE_BF16, st);
+}
+
 template <int D, bool BF16>
 int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_t st) {
   using C = DenseCfg<D>;
   auto kern = attn_dense_kernel<D, BF16>;
-  int dev = 0;
-  BSA_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return BSA_ERR_DEVICE;
-  static std::atomic<bool> ready[64] = {};
-  if (!ready[dev].load(std::memory_order_acquire)) {
+  static std::atomic<int> checked{0};  // 1 ok, 2 too few registers
+  if (!checked.load(std::memory_order_relaxed)) {
     cudaFuncAttributes fa;
     BSA_CUDA_CHECK(cudaFuncGetAttributes(&fa, kern));
     // with fewer registers at launch the split's increases would never be granted
-    if (fa.numRegs * kThreadsD < 128 * kRegsSplitD) return BSA_ERR_UNSUPPORTED;
-    BSA_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    ready[dev].store(true, std::memory_order_release);
+    checked.store(fa.numRegs * kThreadsD >= 128 * kRegsSplitD ? 1 : 2);
   }
+  if (checked.load(std::memory_order_relaxed) != 1) return BSA_ERR_UNSUPPORTED;
+  int r;
+  if ((r = opt_in_smem(reinterpret_cast<const void*>(kern), C::SMEM))) return r;
   DenseParams p{};
-  CUtensorMap mq, mk[2], mv[2];
-  int r, unused;
-  const bool packed = c.M < 128;
+  CUtensorMap mq{}, mk[2] = {}, mv[2] = {};
+  p.packed = c.M < 128;
   // (gathered query rows need no map; the kernel then never reads it)
-  bsa_tensor4d q = c.q;
-  if (packed)
-    mq = CUtensorMap{};
-  else if ((r = map_of(&mq, q, c.B, c.H, c.M, D, BF16, &unused)))
-    return r;
-  p.nparts = c.n;
+  if (!p.packed && (r = map_of(&mq, c.q, c.B, c.H, c.M, D, BF16, &p.qb_mul))) return r;
   for (int i = 0; i < c.n; ++i) {
-    DensePart& pt = p.part[i];
-    const Shape& s = pl.s[i];
-    pt.units = s.units;
-    pt.seqs = c.shared_kv[i] ? c.B : 1;
+    const Source& s = pl.s[i];
+    if (s.few) continue;
+    const int j = p.nparts++;
+    DensePart& pt = p.part[j];
     pt.rows = s.rows;
     pt.tiles = s.tiles;
-    pt.splits = pl.splits[i];
-    pt.chunk = pl.chunk;
+    pt.splits = s.splits;
+    pt.chunk = s.chunk;
     pt.keys = c.keys[i];
-    pt.items = s.units * s.tiles * pl.splits[i];
+    pt.items = s.units * s.tiles * s.splits;
     pt.shared_kv = c.shared_kv[i];
     pt.causal = c.causal[i];
     pt.lens = c.lens[i];
-    if (pl.join) {
-      pt.part_o = reinterpret_cast<float*>(ws + pl.o_off[i]);
-      pt.part_lse = reinterpret_cast<float*>(ws + pl.lse_off[i]);
-    }
-    p.dual |= s.dual ? 1 << i : 0;
-    if (c.keys[i]) {
-      const int kb = c.shared_kv[i] ? 1 : c.B;
-      if ((r = map_of(&mk[i], c.k[i], kb, c.Hk, c.keys[i], D, BF16, &pt.kb_mul))) return r;
-      if ((r = map_of(&mv[i], c.v[i], kb, c.Hk, c.keys[i], D, BF16, &pt.vb_mul))) return r;
-    } else {
-      mk[i] = mv[i] = CUtensorMap{};  // no key tile is ever loaded
-    }
+    if (pl.join) pt.part_o = part_o(s, ws), pt.part_lse = part_lse(s, ws);
+    p.dual |= s.dual ? 1 << j : 0;
+    if (!c.keys[i]) continue;  // no key tile is ever loaded
+    const int kb = c.shared_kv[i] ? 1 : c.B;
+    if ((r = map_of(&mk[j], c.k[i], kb, c.Hk, c.keys[i], D, BF16, &pt.kb_mul))) return r;
+    if ((r = map_of(&mv[j], c.v[i], kb, c.Hk, c.keys[i], D, BF16, &pt.vb_mul))) return r;
   }
-  if (c.n == 1) mk[1] = mk[0], mv[1] = mv[0];
   p.B = c.B, p.H = c.H, p.Hk = c.Hk, p.G = c.H / c.Hk, p.M = c.M;
   p.lens_i64 = c.lens_dtype == BSA_INDEX_I64;
-  p.packed = packed;
   p.q = static_cast<const uint8_t*>(c.q.data);
   p.qs_b = c.q.stride_b, p.qs_h = c.q.stride_h, p.qs_n = c.q.stride_n;
   p.o = static_cast<uint8_t*>(c.o.data);
@@ -1004,35 +1057,38 @@ int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStrea
   p.scale_log2 = c.sm_scale * 1.4426950408889634f;
   p.err = c.err;
   p.wait_ns = kWaitNs;
-  const int total = p.part[0].items + (c.n > 1 ? p.part[1].items : 0);
+  const int total = p.part[0].items + p.part[1].items;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(total < kSMs ? total : kSMs);
-  cfg.blockDim = dim3(kThreadsD);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  const cudaLaunchConfig_t cfg = config(total < kSMs ? total : kSMs, kThreadsD, C::SMEM, st, attr);
   BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq, mk[0], mv[0], mk[1], mv[1], p));
+  return BSA_OK;
+}
+
+template <int D, bool BF16>
+int launch_all(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_t st) {
+  int r;
+  bool dense = false;
+  for (int i = 0; i < c.n; ++i) dense = dense || !pl.s[i].few;
+  if (dense && (r = launch_dense<D, BF16>(c, pl, ws, st))) return r;
+  for (int i = 0; i < c.n; ++i)
+    if (pl.s[i].few && (r = launch_few(c, pl, i, ws, st))) return r;
   if (!pl.join) return BSA_OK;
   JoinParams j{};
   j.nsrc = c.n;
   for (int i = 0; i < c.n; ++i) {
-    j.src[i].o = p.part[i].part_o;
-    j.src[i].lse = p.part[i].part_lse;
-    j.src[i].splits = p.part[i].splits;
-    j.src[i].rows = p.part[i].rows;
-    j.src[i].shared_kv = p.part[i].shared_kv;
+    j.src[i].o = part_o(pl.s[i], ws);
+    j.src[i].lse = part_lse(pl.s[i], ws);
+    j.src[i].splits = pl.s[i].splits;
+    j.src[i].rows = pl.s[i].rows;
+    j.src[i].shared_kv = c.shared_kv[i];
   }
-  j.B = c.B, j.H = c.H, j.Hk = c.Hk, j.G = p.G, j.M = c.M;
-  j.o = p.o, j.os_b = p.os_b, j.os_h = p.os_h, j.os_n = p.os_n;
+  j.B = c.B, j.H = c.H, j.Hk = c.Hk, j.G = c.H / c.Hk, j.M = c.M;
+  j.o = static_cast<uint8_t*>(c.o.data);
+  j.os_b = c.o.stride_b, j.os_h = c.o.stride_h, j.os_n = c.o.stride_n;
   j.lse = c.lse;
   const int64_t rows = static_cast<int64_t>(c.B) * c.H * c.M;
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + 7) / 8));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = config(static_cast<unsigned>((rows + 7) / 8), 256, 0, st, attr);
   BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16>, j));
   return BSA_OK;
 }
@@ -1098,8 +1154,8 @@ int run(const DenseCall& c, void* ws, size_t bytes, cudaStream_t st) {
   if (reinterpret_cast<uintptr_t>(ws) % 16) return BSA_ERR_ALIGNMENT;
   uint8_t* w = static_cast<uint8_t*>(ws);
   const bool bf = c.dtype == BSA_DTYPE_BF16;
-  if (c.D == 128) return bf ? launch_dense<128, true>(c, pl, w, st) : launch_dense<128, false>(c, pl, w, st);
-  return bf ? launch_dense<64, true>(c, pl, w, st) : launch_dense<64, false>(c, pl, w, st);
+  if (c.D == 128) return bf ? launch_all<128, true>(c, pl, w, st) : launch_all<128, false>(c, pl, w, st);
+  return bf ? launch_all<64, true>(c, pl, w, st) : launch_all<64, false>(c, pl, w, st);
 }
 
 }  // namespace

@@ -161,7 +161,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int bh = item / p.q_tiles, t = item - bh * p.q_tiles;
   const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
 
@@ -212,39 +212,51 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
     }
     mbar_wait(q_full, 0, nullptr, nullptr, p.wait_ns);
     for (int i = j > ST ? j - ST : 0; i < j; ++i) mbar_wait(&kv_full[i % ST], (i / ST) & 1, nullptr, nullptr, p.wait_ns);
-  } else if (warp == 1 && lane == 0 && n > 0) {
-    // ------------------------------------------------------------ MMA issue
+  } else if (warp == 1 && n > 0) {
+    // -------------------- MMA issue (whole warp, one elected lane: see attn_dense.cu)
     constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
     constexpr uint32_t idesc_dq = make_idesc_f16(BF16, 128, D, false, true);
     constexpr int TS = C::TILE >> 4;
     const uint64_t qd = k_major(sQ), dod = k_major(sDO), kd = k_major(sK), vd = k_major(sV), kmn = mn_major(sK);
-    bool ok = wait(q_full, 0);
+    bool ok = wait_all(q_full, 0);
     auto issue_s = [&](int j) {
       const int st = j % ST;
-      if (!(ok = ok && wait(&kv_full[st], j / ST))) return;
+      if (!(ok = ok && wait_all(&kv_full[st], j / ST))) return;
       tc_fence_after();
-      mma_abt<D>(tmem + (j & 1) * 128, qd, kd + st * TS, idesc_s);
-      tc_commit(&s_full[j & 1]);
+      if (elect_one()) {
+        mma_abt<D>(tmem + (j & 1) * 128, qd, kd + st * TS, idesc_s);
+        tc_commit(&s_full[j & 1]);
+      }
+      __syncwarp();
     };
     auto issue_dp = [&](int j) {
-      mma_abt<D>(tmem + kDP, dod, vd + (j % ST) * TS, idesc_s);
-      tc_commit(dp_full);
+      if (elect_one()) {
+        mma_abt<D>(tmem + kDP, dod, vd + (j % ST) * TS, idesc_s);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
     };
     if (ok) issue_s(0);
     if (ok) issue_dp(0);
     if (ok && n > 1) issue_s(1);
     for (int j = 0; ok && j < n; ++j) {
-      if (!(ok = wait(ds_ready, j))) break;
+      if (!(ok = wait_all(ds_ready, j))) break;
       tc_fence_after();
       // dP's buffer is free (dS_j is written): step j+1 can go on
       if (j + 1 < n) issue_dp(j + 1);
-      mma_ab<D>(tmem + kDQ, tmem + (j & 1) * 128, kmn + (j % ST) * TS, idesc_dq, j == 0);
-      tc_commit(&kv_empty[j % ST]);
+      if (elect_one()) {
+        mma_ab<D>(tmem + kDQ, tmem + (j & 1) * 128, kmn + (j % ST) * TS, idesc_dq, j == 0);
+        tc_commit(&kv_empty[j % ST]);
+      }
+      __syncwarp();
       // over dS_j, which dQ_j (issued before) has read
       if (j + 2 < n) issue_s(j + 2);
     }
-    tc_commit(done);
-    mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
+    if (elect_one()) {
+      tc_commit(done);
+      mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
+    }
+    __syncwarp();
   } else if (warp >= 4) {
     // ------------------------------------------------- elementwise, epilogue
     const int q4 = warp & 3, half = (warp - 4) >> 2;
@@ -364,7 +376,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int bh = item / p.k_tiles, t = item - bh * p.k_tiles;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
 
@@ -415,39 +427,52 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     }
     mbar_wait(kv_full, 0, nullptr, nullptr, p.wait_ns);
     for (int k = i > ST ? i - ST : 0; k < i; ++k) mbar_wait(&qd_full[k % ST], (k / ST) & 1, nullptr, nullptr, p.wait_ns);
-  } else if (warp == 1 && lane == 0 && n > 0) {
-    // ------------------------------------------------------------ MMA issue
+  } else if (warp == 1 && n > 0) {
+    // -------------------- MMA issue (whole warp, one elected lane: see attn_dense.cu)
     constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
     constexpr uint32_t idesc_acc = make_idesc_f16(BF16, 128, D, false, true);
     constexpr int TS = C::TILE >> 4;
     const uint64_t kd = k_major(sK), vd = k_major(sV), qd = k_major(sQ), dod = k_major(sDO);
     const uint64_t qmn = mn_major(sQ), domn = mn_major(sDO);
-    bool ok = wait(kv_full, 0);
+    bool ok = wait_all(kv_full, 0);
     auto issue_s = [&](int i) {
-      if (!(ok = ok && wait(&qd_full[i % ST], i / ST))) return;
+      if (!(ok = ok && wait_all(&qd_full[i % ST], i / ST))) return;
       tc_fence_after();
-      mma_abt<D>(tmem, kd, qd + (i % ST) * TS, idesc_s);
-      tc_commit(s_full);
+      if (elect_one()) {
+        mma_abt<D>(tmem, kd, qd + (i % ST) * TS, idesc_s);
+        tc_commit(s_full);
+      }
+      __syncwarp();
     };
     auto issue_dp = [&](int i) {
-      mma_abt<D>(tmem + 128, vd, dod + (i % ST) * TS, idesc_s);
-      tc_commit(dp_full);
+      if (elect_one()) {
+        mma_abt<D>(tmem + 128, vd, dod + (i % ST) * TS, idesc_s);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
     };
     if (ok) issue_s(0);
     if (ok) issue_dp(0);
     for (int i = 0; ok && i < n; ++i) {
-      if (!(ok = wait(p_ready, i))) break;
+      if (!(ok = wait_all(p_ready, i))) break;
       tc_fence_after();
-      mma_ab<D>(tmem + 256, tmem, domn + (i % ST) * TS, idesc_acc, i == 0);
+      if (elect_one()) mma_ab<D>(tmem + 256, tmem, domn + (i % ST) * TS, idesc_acc, i == 0);
+      __syncwarp();
       if (i + 1 < n) issue_s(i + 1);  // over P_i^T, which dV_i has read
-      if (!(ok = ok && wait(ds_ready, i))) break;
+      if (!(ok = ok && wait_all(ds_ready, i))) break;
       tc_fence_after();
-      mma_ab<D>(tmem + 256 + D, tmem + 128, qmn + (i % ST) * TS, idesc_acc, i == 0);
-      tc_commit(&qd_empty[i % ST]);
+      if (elect_one()) {
+        mma_ab<D>(tmem + 256 + D, tmem + 128, qmn + (i % ST) * TS, idesc_acc, i == 0);
+        tc_commit(&qd_empty[i % ST]);
+      }
+      __syncwarp();
       if (i + 1 < n) issue_dp(i + 1);  // over dS_i^T
     }
-    tc_commit(done);
-    mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
+    if (elect_one()) {
+      tc_commit(done);
+      mbar_wait(done, 0, nullptr, nullptr, p.wait_ns);
+    }
+    __syncwarp();
   } else if (warp >= 4) {
     // ------------------------------------------------- elementwise, epilogue
     const int q4 = warp & 3, half = (warp - 4) >> 2;
