@@ -361,79 +361,58 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         const int n0 = steps_of(it, 0), n1 = steps_of(it, 1);
         const bool dual = it.dual;
         const int last_s = dual ? (it.nk - 1) & 1 : (n1 ? 1 : 0);  // stream of the item's last S and PV
-        auto issue_s = [&](int s, const Ring<SL>& k, bool last) {
-          tc_fence_after();
-          const uint64_t a = qd + (dual ? 0 : s * (C::TILE >> 4)), b = kd + k.st * (C::TILE >> 4);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const int off = (kk >> 2) * (C::CHUNK >> 4) + (kk & 3) * 2;  // 32 bytes inside a chunk's rows
-              tc_mma_ss(tmem + s * 128, a + off, b + off, idesc_qk, kk > 0 ? 1u : 0u);
-            }
-            tc_commit(&s_full[s]);
-            if (last && s == last_s) tc_commit(q_empty);
-          }
-          __syncwarp();
-        };
-        auto issue_pv = [&](int s, int& np, int& no, const Ring<SL>& v, bool first, bool last) {
-          if (first && no > 0 && !(ok = ok && wait_all(&o_empty[s], no - 1))) return;
-          if (!(ok = ok && wait_all(&p_ready[s], np))) return;
-          ++np;
-          tc_fence_after();
-          const uint64_t b = vd + v.st * (C::TILE >> 4);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              tc_mma_ts(tmem + C::O_COL + s * D, tmem + s * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_pv,
-                        (!first || kk > 0) ? 1u : 0u);
-            if (last) {
-              tc_commit(&o_final[s]);
-              // no later S of this stream tells the softmax that V is free
-              if (dual || s == last_s) tc_commit(&empty[v.st]);
-            }
-          }
-          __syncwarp();
-          if (last) ++no;
-        };
         if (!(ok = wait_all(q_full, nq))) break;
         ++nq;
-        Ring<SL> k = ring, v;
-        ring.next();
-        if (!landed(k)) break;
-        issue_s(0, k, n0 == 1);
-        if (n1 > 0) {
-          if (dual) {
-            k = ring;
-            ring.next();
-            if (!landed(k)) break;
-          }
-          issue_s(1, k, n1 == 1);
-        }
-        auto take_v = [&]() {
-          v = ring;
+        Ring<SL> k, v;
+        auto take = [&](Ring<SL>& r) {
+          r = ring;
           ring.next();
-          return landed(v);
+          return landed(r);
         };
-        auto take_k = [&]() {
-          k = ring;
-          ring.next();
-          return landed(k);
-        };
-        for (int i = 0; ok && i < n0; ++i) {
-          if (!take_v()) break;
-          issue_pv(0, np0, no0, v, i == 0, i == n0 - 1);
-          if (!ok) break;
-          if (i + 1 < n0) {
-            if (!take_k()) break;
-            issue_s(0, k, i + 2 == n0);
-          }
-          if (i < n1) {
-            if (dual && !take_v()) break;
-            issue_pv(1, np1, no1, v, i == 0, i == n1 - 1);
-            if (!ok) break;
-            if (i + 1 < n1) {
-              if (dual && !take_k()) break;
-              issue_s(1, k, i + 2 == n1);
+        // Step i of stream 0, then of stream 1: P_i V_i, S_i+1 (i = -1: the
+        // first S).  The loads are taken in the order they were issued; the
+        // second reader of a shared tile finds it landed.
+        for (int i = -1; ok && i < n0; ++i) {
+#pragma unroll 1
+          for (int s = 0; ok && s < 2; ++s) {
+            const int n = s ? n1 : n0;
+            if (i >= 0 && i < n) {
+              const bool last = i == n - 1;
+              if ((s == 0 || dual) && !take(v)) break;
+              const int np = s ? np1 : np0, no = s ? no1 : no0;
+              if (i == 0 && no > 0 && !(ok = wait_all(&o_empty[s], no - 1))) break;
+              if (!(ok = wait_all(&p_ready[s], np))) break;
+              (s ? np1 : np0) += 1;
+              (s ? no1 : no0) += last ? 1 : 0;
+              tc_fence_after();
+              const uint64_t b = vd + v.st * (C::TILE >> 4);
+              const uint32_t st = tmem + s * 128, ot = tmem + C::O_COL + s * D;
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                  tc_mma_ts(ot, st + kk * 8, b + kk * (16 * 128 >> 4), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+                if (last) {
+                  tc_commit(&o_final[s]);
+                  // no later S of this stream tells the softmax that V is free
+                  if (dual || s == last_s) tc_commit(&empty[v.st]);
+                }
+              }
+              __syncwarp();
+            }
+            if (i + 1 < n) {
+              if ((s == 0 || dual) && !take(k)) break;
+              tc_fence_after();
+              const uint64_t a = qd + (dual ? 0 : s * (C::TILE >> 4)), b = kd + k.st * (C::TILE >> 4);
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const int off = (kk >> 2) * (C::CHUNK >> 4) + (kk & 3) * 2;  // 32 bytes inside a chunk's rows
+                  tc_mma_ss(tmem + s * 128, a + off, b + off, idesc_qk, kk > 0 ? 1u : 0u);
+                }
+                tc_commit(&s_full[s]);
+                if (i + 2 == n && s == last_s) tc_commit(q_empty);
+              }
+              __syncwarp();
             }
           }
         }
@@ -454,16 +433,24 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         if (nq > 0) ok = ok && wait_all(q_empty, nq - 1);
         ++nq;
         if (!ok) continue;
-        // one 16-byte piece a lane: the D / 8 pieces of a row by neighbouring lanes
-        constexpr int PIECES = D / 8;
-        for (int x = (warp - 2) * 32 + lane; x < it.rows * PIECES; x += 64) {
-          const int r = x / PIECES, g = x - r * PIECES;
+        // The warps take 32 rows each in turn: a lane finds one row's
+        // place, then the D / 8 pieces of a row are copied by neighbouring lanes.
+        constexpr int PIECES = D / 8, PER = 32 / PIECES;  // rows a pass
+        const int piece = lane % PIECES, sub = lane / PIECES;
+        for (int base = (warp - 2) * 32; base < it.rows; base += 64) {
+          const int mine = base + lane;
           int b, h, m;
-          row_of(p, it, it.row0 + r, b, h, m);
-          const uint8_t* src = p.q + 2 * (b * p.qs_b + h * p.qs_h + m * p.qs_n + g * 8);
-          const int rr = r & 127;
-          cp_async16(smem_u32(sQ + (r >> 7) * C::TILE + (g >> 3) * C::CHUNK + rr * 128 + (((g & 7) ^ (rr & 7)) * 16)),
-                     src, 16);
+          row_of(p, it, it.row0 + min(mine, it.rows - 1), b, h, m);
+          const int64_t off = 2 * (b * p.qs_b + h * p.qs_h + m * p.qs_n);
+#pragma unroll 4
+          for (int x = 0; x < 32; x += PER) {
+            const int64_t at = __shfl_sync(0xffffffffu, off, x + sub);
+            const int r = base + x + sub, rr = r & 127;
+            if (r < it.rows)
+              cp_async16(smem_u32(sQ + (r >> 7) * C::TILE + (piece >> 3) * C::CHUNK + rr * 128 +
+                                  (((piece & 7) ^ (rr & 7)) * 16)),
+                         p.q + at + piece * 16, 16);
+          }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
@@ -668,21 +655,23 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         f1 *= inv;
         const float lse = nan ? NAN : (lt > 0.f ? mx + log2f(lt) : -INFINITY);
         int b = 0, h = 0, mm = 0;
-        row_of(p, it, it.row0 + (store ? r : 0), b, h, mm);
-        uint8_t* orow = p.o + 2 * (b * p.os_b + h * p.os_h + mm * p.os_n);
+        row_of(p, it, it.row0 + (r < it.rows ? r : 0), b, h, mm);
+        // a row's place in the result, or in the partial results
         const int64_t slot = (static_cast<int64_t>(it.unit) * pt.rows + it.row0 + r) * pt.splits + it.split;
-        float* prow = pt.part_o ? pt.part_o + slot * D : nullptr;
-        if (it.nk > 0) {
-#pragma unroll
+        uint8_t* const mine = pt.part_o ? reinterpret_cast<uint8_t*>(pt.part_o + slot * D)
+                                        : p.o + 2 * (b * p.os_b + h * p.os_h + mm * p.os_n);
+        const bool have = it.nk > 0;
+        if (have || !pt.part_o) {  // (a partial result without keys is only its lse)
+#pragma unroll 1
           for (int ch = 0; ch < D / 32; ++ch) {
             uint32_t v[32];
-            tmem_ld32(o_base + first * D + ch * 32, v);
-            tmem_wait_ld32(v);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float x = __uint_as_float(v[k]);
-              v[k] = __float_as_uint(l[0] > 0.f || nan ? x * f0 : 0.f);
+            if (have) {
+              tmem_ld32(o_base + first * D + ch * 32, v);
+              tmem_wait_ld32(v);
             }
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              v[k] = have && (l[0] > 0.f || nan) ? __float_as_uint(__uint_as_float(v[k]) * f0) : 0u;
             if (last - first == 2) {
               uint32_t u[32];
               tmem_ld32(o_base + D + ch * 32, u);
@@ -693,38 +682,46 @@ __global__ void __launch_bounds__(kThreadsD, 1)
                   v[k] = __float_as_uint(fmaf(__uint_as_float(u[k]), f1, __uint_as_float(v[k])));
               }
             }
-            if (ch == D / 32 - 1) {
+            if (have && ch == D / 32 - 1) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0)
                 for (int s = first; s < last; ++s) mbar_arrive(&o_empty[s]);
             }
-            if (store) {
-              if (prow) {
+            // 32 columns: 8 pieces of 16 bytes in fp32, 4 in 16 bits
+            const int row0 = ps * 128 + q4 * 32;
+            if (pt.part_o) {
+              uint4 x[8];
 #pragma unroll
-                for (int g = 0; g < 8; ++g)
-                  reinterpret_cast<uint4*>(prow)[ch * 8 + g] =
-                      make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-              } else {
+              for (int g = 0; g < 8; ++g) x[g] = make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+              transpose_pieces<8>(x);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                  uint4 x;
-                  x.x = pack2<BF16>(__uint_as_float(v[8 * g + 0]), __uint_as_float(v[8 * g + 1]));
-                  x.y = pack2<BF16>(__uint_as_float(v[8 * g + 2]), __uint_as_float(v[8 * g + 3]));
-                  x.z = pack2<BF16>(__uint_as_float(v[8 * g + 4]), __uint_as_float(v[8 * g + 5]));
-                  x.w = pack2<BF16>(__uint_as_float(v[8 * g + 6]), __uint_as_float(v[8 * g + 7]));
-                  reinterpret_cast<uint4*>(orow)[ch * 4 + g] = x;
-                }
+              for (int k = 0; k < 8; ++k) {
+                const int from = (lane & 24) + k;
+                uint8_t* dst = shfl_ptr(mine, from) + ch * 128 + (lane & 7) * 16;
+                if (ok && row0 + from < it.rows) *reinterpret_cast<uint4*>(dst) = x[k];
+              }
+            } else {
+              uint4 x[4];
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                x[g].x = pack2<BF16>(__uint_as_float(v[8 * g + 0]), __uint_as_float(v[8 * g + 1]));
+                x[g].y = pack2<BF16>(__uint_as_float(v[8 * g + 2]), __uint_as_float(v[8 * g + 3]));
+                x[g].z = pack2<BF16>(__uint_as_float(v[8 * g + 4]), __uint_as_float(v[8 * g + 5]));
+                x[g].w = pack2<BF16>(__uint_as_float(v[8 * g + 6]), __uint_as_float(v[8 * g + 7]));
+              }
+              transpose_pieces<4>(x);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int from = (lane & 28) + k;
+                uint8_t* dst = shfl_ptr(mine, from) + ch * 64 + (lane & 3) * 16;
+                if (ok && row0 + from < it.rows) *reinterpret_cast<uint4*>(dst) = x[k];
               }
             }
           }
-        } else if (store && !prow) {
-          // no key at all: o = 0 (a partial result is only its lse)
-#pragma unroll
-          for (int g = 0; g < D / 8; ++g) reinterpret_cast<uint4*>(orow)[g] = make_uint4(0, 0, 0, 0);
         }
         if (store) {
-          if (prow)
+          if (pt.part_o)
             pt.part_lse[slot] = lse;
           else if (p.lse)
             p.lse[(static_cast<int64_t>(b) * p.H + h) * p.M + mm] = lse;
@@ -742,8 +739,10 @@ __global__ void __launch_bounds__(kThreadsD, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Joins the partial results of an output row: one warp a row, D / 32 columns a
-// lane.  A partial result whose lse is -inf saw no key and its o is not read.
+// Joins the partial results of an output row: W warps a row, each D / 32
+// columns a lane over every W-th partial result.  One whose lse is -inf saw no
+// key and its o is not read.  W = 8 where there are few rows (128 rows of 37
+// partial results: 5 us, with one warp a row 20 us), else 1.
 // ---------------------------------------------------------------------------
 struct JoinSrc {
   const float* o;
@@ -752,69 +751,80 @@ struct JoinSrc {
 };
 struct JoinParams {
   JoinSrc src[2];
-  int nsrc;
   int B, H, Hk, G, M;
   uint8_t* o;
   int64_t os_b, os_h, os_n;
   float* lse;
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, int W>
 __global__ void __launch_bounds__(256) attn_join_kernel(const JoinParams p) {
   constexpr int V = D / 32;
+  __shared__ float part[W == 1 ? 1 : W][D + 1];
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(p.B) * p.H * p.M) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
+  if (row >= static_cast<int64_t>(p.B) * p.H * p.M) return;  // (W = 8: never)
   const int m = static_cast<int>(row % p.M);
   const int64_t bh = row / p.M;
   const int h = static_cast<int>(bh % p.H), b = static_cast<int>(bh / p.H);
   const int hk = h / p.G, g = h - hk * p.G;
-  // the running max and sums over both sources
-  float mx = -INFINITY, sum = 0.f, acc[V];
+  const float *ls[2], *os[2];
+  int n[2];
+  float mx = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const JoinSrc sr = p.src[s];
+    const int64_t r = sr.shared_kv ? static_cast<int64_t>(hk) * sr.rows + (static_cast<int64_t>(b) * p.G + g) * p.M + m
+                                   : (static_cast<int64_t>(b) * p.Hk + hk) * sr.rows + g * p.M + m;
+    n[s] = sr.splits;
+    ls[s] = sr.lse + r * sr.splits;
+    os[s] = sr.o + r * sr.splits * D + lane * V;
+    for (int k = lane; k < n[s]; k += 32) {
+      const float l = ls[s][k];
+      nan = nan || isnan(l);
+      mx = fmaxf(mx, l);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+  if (__any_sync(0xffffffffu, nan)) mx = NAN;
+  float sum = 0.f, acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const JoinSrc sr = p.src[s];
-    if (s >= p.nsrc) break;
-    const int64_t r = sr.shared_kv ? static_cast<int64_t>(hk) * sr.rows + (static_cast<int64_t>(b) * p.G + g) * p.M + m
-                                   : (static_cast<int64_t>(b) * p.Hk + hk) * sr.rows + g * p.M + m;
-    const float* ls = sr.lse + r * sr.splits;
-    const float* os = sr.o + r * sr.splits * D + lane * V;
-    for (int c = 0; c < sr.splits; c += 32) {
-      const int n = min(32, sr.splits - c);
-      const float mine = lane < n ? ls[c + lane] : -INFINITY;
-      float t = mine;
-      bool nan = isnan(mine);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
-      if (__any_sync(0xffffffffu, nan)) t = NAN;
-      if (t == -INFINITY) continue;
-      const float m_new = isnan(t) ? t : fmaxf(mx, t);
-      const float alpha = mx == -INFINITY ? 0.f : ex2_approx(mx - m_new);
-      mx = m_new;
-      sum *= alpha;
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] *= alpha;
-      const float wt = mine == -INFINITY ? 0.f : ex2_approx(mine - mx);
 #pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const float wk = __shfl_sync(0xffffffffu, wt, k);
-        if (wk == 0.f) continue;
-        sum += wk;
-        const float* src = os + static_cast<int64_t>(c + k) * D;
-        float x[V];
-        if constexpr (V == 4) {
-          const float4 f = *reinterpret_cast<const float4*>(src);
-          x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-        } else {
-          const float2 f = *reinterpret_cast<const float2*>(src);
-          x[0] = f.x, x[1] = f.y;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(wk, x[i], acc[i]);
+    for (int k = W == 1 ? 0 : warp; k < n[s]; k += W) {
+      const float l = ls[s][k];
+      const bool any = l != -INFINITY;
+      const float* src = os[s] + static_cast<int64_t>(k) * D;
+      float x[V];
+      if constexpr (V == 4) {
+        const float4 f = any ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+      } else {
+        const float2 f = any ? *reinterpret_cast<const float2*>(src) : make_float2(0.f, 0.f);
+        x[0] = f.x, x[1] = f.y;
       }
+      const float wt = any ? ex2_approx(l - mx) : 0.f;
+      sum += wt;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(wt, x[i], acc[i]);
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[warp][lane * V + i] = acc[i];
+    if (lane == 0) part[warp][D] = sum;
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      sum += part[w][D];
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] += part[w][lane * V + i];
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -867,7 +877,10 @@ Source source_of(const DenseCall& c, int i) {
   const int G = c.H / c.Hk, seqs = c.shared_kv[i] ? c.B : 1;
   s.units = c.shared_kv[i] ? c.Hk : c.B * c.Hk;
   s.rows = seqs * G * c.M;
-  s.few = s.rows <= kFewRows;
+  // 9 to 16 rows leave the few-rows kernel half the warps an SM: it wins on
+  // short ranges only (16 rows, 64 x 8 units of 512 keys 39 us against 48; 4 x 8
+  // units of 65,536 keys 199 against 181).
+  s.few = s.rows <= kFewRows / 2 || (s.rows <= kFewRows && c.keys[i] <= 8192);
   const bool packed = c.M < 128;
   const int one = packed ? s.rows : c.M;  // rows that can share a tile
   s.dual = one <= 128;
@@ -1073,8 +1086,7 @@ int launch_all(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_
   for (int i = 0; i < c.n; ++i)
     if (pl.s[i].few && (r = launch_few(c, pl, i, ws, st))) return r;
   if (!pl.join) return BSA_OK;
-  JoinParams j{};
-  j.nsrc = c.n;
+  JoinParams j{};  // (an absent second source has no partial results)
   for (int i = 0; i < c.n; ++i) {
     j.src[i].o = part_o(pl.s[i], ws);
     j.src[i].lse = part_lse(pl.s[i], ws);
@@ -1088,8 +1100,13 @@ int launch_all(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_
   j.lse = c.lse;
   const int64_t rows = static_cast<int64_t>(c.B) * c.H * c.M;
   cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = config(static_cast<unsigned>((rows + 7) / 8), 256, 0, st, attr);
-  BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16>, j));
+  if (rows <= 8 * kSMs) {
+    const cudaLaunchConfig_t cfg = config(static_cast<unsigned>(rows), 256, 0, st, attr);
+    BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16, 8>, j));
+  } else {
+    const cudaLaunchConfig_t cfg = config(static_cast<unsigned>((rows + 7) / 8), 256, 0, st, attr);
+    BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16, 1>, j));
+  }
   return BSA_OK;
 }
 

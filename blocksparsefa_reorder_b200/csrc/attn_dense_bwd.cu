@@ -86,28 +86,40 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// A 128 x 64-column part of an accumulator row (this thread's 32 columns at a
-// time) times `scale`, as 16-bit values; zeros where `zero`.
+// Half of an accumulator's columns (this thread's D / 2 of one row) times
+// `scale`, as 16-bit values; `row`: the row's place, `keep`: whether it is
+// stored, `zero`: as zeros.  8 lanes write 128 bytes of a row at D = 128.
 template <int D, bool BF16>
-__device__ __forceinline__ void store_half_row(uint32_t base, int half, float scale, uint8_t* row, bool store, bool zero) {
+__device__ __forceinline__ void store_half_row(uint32_t base, int half, float scale, uint8_t* row, bool keep, bool zero) {
+  const int lane = threadIdx.x & 31;
+  uint4 x[8];
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) {
-    const int col = half * (D / 2) + c * 32;
     uint32_t a[32];
-    tmem_ld32(base + col, a);
+    tmem_ld32(base + half * (D / 2) + c * 32, a);
     tmem_wait32(a);
-    if (store) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint4 v;
-        v.x = pack2<BF16>(__uint_as_float(a[8 * g + 0]) * scale, __uint_as_float(a[8 * g + 1]) * scale);
-        v.y = pack2<BF16>(__uint_as_float(a[8 * g + 2]) * scale, __uint_as_float(a[8 * g + 3]) * scale);
-        v.z = pack2<BF16>(__uint_as_float(a[8 * g + 4]) * scale, __uint_as_float(a[8 * g + 5]) * scale);
-        v.w = pack2<BF16>(__uint_as_float(a[8 * g + 6]) * scale, __uint_as_float(a[8 * g + 7]) * scale);
-        if (zero) v = make_uint4(0, 0, 0, 0);
-        reinterpret_cast<uint4*>(row)[col / 8 + g] = v;
-      }
+    for (int g = 0; g < 4; ++g) {
+      uint4& v = x[c * 4 + g];
+      v.x = pack2<BF16>(__uint_as_float(a[8 * g + 0]) * scale, __uint_as_float(a[8 * g + 1]) * scale);
+      v.y = pack2<BF16>(__uint_as_float(a[8 * g + 2]) * scale, __uint_as_float(a[8 * g + 3]) * scale);
+      v.z = pack2<BF16>(__uint_as_float(a[8 * g + 4]) * scale, __uint_as_float(a[8 * g + 5]) * scale);
+      v.w = pack2<BF16>(__uint_as_float(a[8 * g + 6]) * scale, __uint_as_float(a[8 * g + 7]) * scale);
+      if (zero) v = make_uint4(0, 0, 0, 0);
     }
+  }
+  if constexpr (D == 128) {
+    transpose_pieces<8>(x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int from = (lane & 24) + k;
+      uint8_t* dst = shfl_ptr(row, from);
+      const bool st = __shfl_sync(0xffffffffu, static_cast<int>(keep), from) != 0;
+      if (st) *reinterpret_cast<uint4*>(dst + half * D + (lane & 7) * 16) = x[k];
+    }
+  } else if (keep) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) reinterpret_cast<uint4*>(row)[half * 4 + g] = x[g];
   }
 }
 

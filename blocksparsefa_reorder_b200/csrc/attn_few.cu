@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
   constexpr int VP = D / 64;  // and of a V row
   constexpr int MT = D / 16;  // m tiles of O^T
   constexpr int ROWS = 8 * NR;
+  constexpr int UB = 128 / D;
   constexpr float kSlack = BF16 ? 30.f : 14.f;  // log2: p stays below 2^30 (bf16), 2^14 (fp16)
   extern __shared__ __align__(16) float fsm[];
   float* sm_o = fsm;                          // [kWarpsF][ROWS][D]
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
     l_run[n][0] = l_run[n][1] = 0.f;
   }
 
-  if (k0 + warp * 16 < k1) {
+  if (k0 + warp * 16 * UB < k1) {
     uint4 qf[NR][KP];
     int limit[NR][2];  // keys that rows 2c, 2c + 1 see
 #pragma unroll
@@ -131,78 +132,88 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
     }
     const uint8_t* kb = p.k + 2 * (b * p.ks_b + hk * p.ks_h + c * 8);
     const uint8_t* vb = p.v + 2 * (b * p.vs_b + hk * p.vs_h + g * 8);
-    for (int key = k0 + warp * 16; key < k1; key += kWarpsF * 16) {
-      const bool whole = key + 16 <= k1;
-      uint4 kf[2][KP], vf[4][VP];
+    // UB blocks of 16 keys at a time: at D = 64 two, for the same bytes in flight
+    for (int key0 = k0 + warp * 16 * UB; key0 < k1; key0 += kWarpsF * 16 * UB) {
+      const bool whole = key0 + 16 * UB <= k1;
+      uint4 kfs[UB][2][KP], vfs[UB][4][VP];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = key + g + 8 * h;
-        const uint8_t* src = kb + 2 * (row * p.ks_n);
+      for (int u = 0; u < UB; ++u) {
 #pragma unroll
-        for (int i = 0; i < KP; ++i) kf[h][i] = load16(src + i * 64, whole || row < k1);
+        for (int h = 0; h < 2; ++h) {
+          const int row = key0 + u * 16 + g + 8 * h;
+          const uint8_t* src = kb + 2 * (row * p.ks_n);
+#pragma unroll
+          for (int i = 0; i < KP; ++i) kfs[u][h][i] = load16(src + i * 64, whole || row < k1);
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int row = key0 + u * 16 + 2 * c + (h & 1) + 8 * (h >> 1);
+          const uint8_t* src = vb + 2 * (row * p.vs_n);
+#pragma unroll
+          for (int i = 0; i < VP; ++i) vfs[u][h][i] = load16(src + i * 128, whole || row < k1);
+        }
       }
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int row = key + 2 * c + (h & 1) + 8 * (h >> 1);
-        const uint8_t* src = vb + 2 * (row * p.vs_n);
+      for (int u = 0; u < UB; ++u) {
+        const int key = key0 + u * 16;
+        const uint4 (&kf)[2][KP] = kfs[u];
+        const uint4 (&vf)[4][VP] = vfs[u];
+        uint32_t pt[NR][2];
 #pragma unroll
-        for (int i = 0; i < VP; ++i) vf[h][i] = load16(src + i * 128, whole || row < k1);
-      }
-      uint32_t pt[NR][2];
+        for (int n = 0; n < NR; ++n) {
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < KP; ++i) {
+            mma_16816<BF16>(s, kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qf[n][i].x, qf[n][i].y);
+            mma_16816<BF16>(s, kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qf[n][i].z, qf[n][i].w);
+          }
+          // s[2 h + e]: key g + 8 h, row 2c + e
+          float x[4];
+          bool over = false;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-          mma_16816<BF16>(s, kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qf[n][i].x, qf[n][i].y);
-          mma_16816<BF16>(s, kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qf[n][i].z, qf[n][i].w);
-        }
-        // s[2 h + e]: key g + 8 h, row 2c + e
-        float x[4];
-        bool over = false;
+          for (int t = 0; t < 4; ++t) {
+            const int e = t & 1;
+            x[t] = key + g + 8 * (t >> 1) < limit[n][e] ? s[t] * p.scale_log2 : -INFINITY;
+            over = over || (x[t] - m_run[n][e] > kSlack);
+          }
+          if (__any_sync(0xffffffffu, over)) {
+            // a new reference point: the block's max of each row, over the 8 lanes that hold its keys
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int e = t & 1;
-          x[t] = key + g + 8 * (t >> 1) < limit[n][e] ? s[t] * p.scale_log2 : -INFINITY;
-          over = over || (x[t] - m_run[n][e] > kSlack);
-        }
-        if (__any_sync(0xffffffffu, over)) {
-          // a new reference point: the block's max of each row, over the 8 lanes that hold its keys
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(x[e], x[2 + e]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              mx = fmaxf(mx, m_run[n][e]);
+              const float alpha = mx == -INFINITY ? 1.f : ex2_approx(m_run[n][e] - mx);
+              m_run[n][e] = mx;
+              l_run[n][e] *= alpha;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(x[e], x[2 + e]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            mx = fmaxf(mx, m_run[n][e]);
-            const float alpha = mx == -INFINITY ? 1.f : ex2_approx(m_run[n][e] - mx);
-            m_run[n][e] = mx;
-            l_run[n][e] *= alpha;
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-              acc[n][j][e] *= alpha;
-              acc[n][j][2 + e] *= alpha;
+              for (int j = 0; j < MT; ++j) {
+                acc[n][j][e] *= alpha;
+                acc[n][j][2 + e] *= alpha;
+              }
             }
           }
+          float pr[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int e = t & 1;
+            pr[t] = ex2_approx(x[t] - (m_run[n][e] == -INFINITY ? 0.f : m_run[n][e]));
+            l_run[n][e] += pr[t];
+          }
+          pt[n][0] = movmatrix_trans(pack2<BF16>(pr[0], pr[1]));
+          pt[n][1] = movmatrix_trans(pack2<BF16>(pr[2], pr[3]));
         }
-        float pr[4];
+        // m tile j: rows g and g + 8 are dims g 8 + j and 64 + g 8 + j (D 128), g 8 + 2j and g 8 + 2j + 1 (D 64)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int e = t & 1;
-          pr[t] = ex2_approx(x[t] - (m_run[n][e] == -INFINITY ? 0.f : m_run[n][e]));
-          l_run[n][e] += pr[t];
+        for (int j = 0; j < MT; ++j) {
+          const int e0 = VP == 2 ? j : 2 * j, e1 = VP == 2 ? j : 2 * j + 1, hi = VP - 1;
+          const uint32_t a0 = pair_at(vf[0][0], vf[1][0], e0), a1 = pair_at(vf[0][hi], vf[1][hi], e1);
+          const uint32_t a2 = pair_at(vf[2][0], vf[3][0], e0), a3 = pair_at(vf[2][hi], vf[3][hi], e1);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) mma_16816<BF16>(acc[n][j], a0, a1, a2, a3, pt[n][0], pt[n][1]);
         }
-        pt[n][0] = movmatrix_trans(pack2<BF16>(pr[0], pr[1]));
-        pt[n][1] = movmatrix_trans(pack2<BF16>(pr[2], pr[3]));
-      }
-      // m tile j: rows g and g + 8 are dims g 8 + j and 64 + g 8 + j (D 128), g 8 + 2j and g 8 + 2j + 1 (D 64)
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int e0 = VP == 2 ? j : 2 * j, e1 = VP == 2 ? j : 2 * j + 1, hi = VP - 1;
-        const uint32_t a0 = pair_at(vf[0][0], vf[1][0], e0), a1 = pair_at(vf[0][hi], vf[1][hi], e1);
-        const uint32_t a2 = pair_at(vf[2][0], vf[3][0], e0), a3 = pair_at(vf[2][hi], vf[3][hi], e1);
-#pragma unroll
-        for (int n = 0; n < NR; ++n) mma_16816<BF16>(acc[n][j], a0, a1, a2, a3, pt[n][0], pt[n][1]);
       }
     }
   }

@@ -36,6 +36,19 @@ template <> __device__ __forceinline__ uint32_t pack2<false>(float lo, float hi)
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// The inverse.
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (BF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  }
+}
+
 __device__ __forceinline__ void set_err(int32_t* flag, int32_t bits) {
   if (flag) atomicOr(flag, bits);
 }
@@ -244,6 +257,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
 // 16 lanes, split in column halves between the two half-warps: threads 0-15
 // access lanes [taddr.lane, +16) at columns [taddr.col, +N), threads 16-31
 // the same lanes at columns [taddr.col + OFF, +N); thread i holds N
@@ -303,6 +326,35 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(bool bf16, int M, int N, b
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn_major ? 1u : 0u) << 15) |
          ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// Transposes N x N pieces of 16 bytes among N neighbouring lanes: lane j of the
+// N gives pieces 0 .. N-1 of its row and gets piece j of rows 0 .. N-1.  A row
+// a lane otherwise stores in 16-byte steps a row apart, every step touching 32
+// lines; after this N lanes write 16 N bytes of one row.
+template <int N>
+__device__ __forceinline__ void transpose_pieces(uint4 (&b)[N]) {
+  const int j = threadIdx.x & (N - 1);
+#pragma unroll
+  for (int s = 1; s < N; s <<= 1) {
+    const bool up = (j & s) != 0;
+#pragma unroll
+    for (int a = 0; a < N; ++a) {
+      if (a & s) continue;
+      uint4 x = up ? b[a] : b[a | s];
+      x.x = __shfl_xor_sync(0xffffffffu, x.x, s);
+      x.y = __shfl_xor_sync(0xffffffffu, x.y, s);
+      x.z = __shfl_xor_sync(0xffffffffu, x.z, s);
+      x.w = __shfl_xor_sync(0xffffffffu, x.w, s);
+      if (up)
+        b[a] = x;
+      else
+        b[a | s] = x;
+    }
+  }
+}
+__device__ __forceinline__ uint8_t* shfl_ptr(uint8_t* p, int lane) {
+  return reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), lane));
 }
 
 __device__ __forceinline__ float ex2_approx(float x) {

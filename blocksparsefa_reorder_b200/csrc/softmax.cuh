@@ -103,11 +103,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // nearest integer (adding 1.5 2^23 leaves n in the low bits of the sum), 2^f
 // by the degree-4 polynomial of least relative error on [-1/2, 1/2] (2.6e-6,
 // fitted by Remez exchange; its mean error is 1.4e-8), 2^n from n's bits in
-// the exponent field.  Values below 2^-126 give 2^-126; NaN stays NaN.
+// the exponent field.  Values below 2^-126 give 0 (exactly, for -inf: the
+// exponent field is 0); NaN stays NaN.
 __device__ __forceinline__ uint64_t ex2_fma_x2(uint64_t x) {
   float x0, x1;
   f32x2_unpack(x, x0, x1);
-  x = f32x2_pack(max_nan(x0, -126.f), max_nan(x1, -126.f));
+  x = f32x2_pack(max_nan(x0, -127.f), max_nan(x1, -127.f));
   constexpr float kMagic = 12582912.f + 127.f;  // the exponent's bias with it
   const uint64_t t = f32x2_add(x, f32x2_pack(kMagic, kMagic));
   const uint64_t n = f32x2_add(t, f32x2_pack(-kMagic, -kMagic));
@@ -122,8 +123,7 @@ __device__ __forceinline__ uint64_t ex2_fma_x2(uint64_t x) {
   return f32x2_mul(p, f32x2_pack(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
 }
 
-// exp_block with a quarter of the exponentials on the FMA pipe (for scores
-// none of which is masked: a masked one needs its exact 0).
+// exp_block with a quarter of the exponentials on the FMA pipe.
 template <int BN, bool BF16>
 __device__ __forceinline__ float exp_block_mixed(const uint32_t (&sr)[BN], uint32_t (&pr)[BN / 2], float scale_log2,
                                                  float neg_m) {
