@@ -8,11 +8,12 @@ there is no CPU or library fallback for any entry point.
 from __future__ import annotations
 
 import ctypes
-import struct
+import importlib.util
 import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libbsattn_b200.so"
+NATIVE_PATH = LIB_PATH.parent / "_bsattn_torch.so"
 
 OK = 0
 STATUS_NAMES = {
@@ -54,23 +55,6 @@ class BwdArgs(ctypes.Structure):
                 ("plan", Plan), ("plan_t", Plan), ("err_flag", ctypes.c_void_p)]
 
 
-# Argument structures of the entry points that are called once a token: packed
-# in one step (a quarter of the time of filling a ctypes.Structure field by
-# field) in the C declaration's order; "Pqqq" is a bsa_tensor4d, a trailing
-# "0q" the C compiler's padding.
-_T4 = "Pqqq"
-# B H Hk N D R dtype weight_dtype | q k q_out k_out dq_out dk_out | q_weight k_weight cos sin | table_stride |
-# table_len pos_dtype | positions | pos_stride_b | eps interleaved | dq_weight dk_weight err_flag
-ROPE_ARGS = struct.Struct("@8i" + 6 * _T4 + "4Pq2iPqfi3P")
-# B H Hk M N D dtype lens_dtype | q o k v | k_lens lse err_flag | sm_scale
-CROSS_ARGS = struct.Struct("@8i" + 4 * _T4 + "3Pf0q")
-# B H Hk M N D dtype lens_dtype | q k v o dout dq dk dv | k_lens lse delta err_flag | sm_scale
-CROSS_BWD_ARGS = struct.Struct("@8i" + 8 * _T4 + "4Pf0q")
-# B H Hk T P C D dtype lens_dtype | q o k_prefix v_prefix k v | lens lse err_flag | sm_scale
-PREFIX_ARGS = struct.Struct("@9i" + 6 * _T4 + "3Pf0q")
-NO_TENSOR = (0, 0, 0, 0)
-
-
 class BsaError(RuntimeError):
     """A C-ABI call returned a non-zero bsa_status."""
 
@@ -99,6 +83,7 @@ PROTOS = {
     "bsa_fwd_reordered": ([ctypes.POINTER(FwdArgs), _vp, _vp, _i32, _vp, _sz, _vp], ctypes.c_int),
     "bsa_test_arm_wait_timeout": ([ctypes.c_uint32], ctypes.c_int),
     "bsa_bwd": ([ctypes.POINTER(BwdArgs), _vp], ctypes.c_int),
+    # (called from csrc/bind.cpp, which fills the argument structures)
     "bsa_qk_norm_rope": ([_vp, _vp], ctypes.c_int),
     "bsa_qk_norm_rope_bwd_workspace_bytes": ([_vp, ctypes.POINTER(_sz)], ctypes.c_int),
     "bsa_qk_norm_rope_bwd": ([_vp, _vp, _sz, _vp], ctypes.c_int),
@@ -132,6 +117,29 @@ def lib():
                     raise RuntimeError(f"{LIB_PATH}: ABI version {handle.bsa_abi_version()} != {ABI_VERSION}")
                 _lib = handle
     return _lib
+
+
+_native = None
+
+
+def native():
+    """The native host side of the per-token operators (``csrc/bind.cpp``),
+    loaded once per process; it links the library above."""
+    global _native
+    if _native is None:
+        lib()
+        with _lock:
+            if _native is None:
+                if not NATIVE_PATH.exists():
+                    raise RuntimeError(f"{NATIVE_PATH} is missing: build the CUDA extension first "
+                                       "(python -m blocksparsefa_reorder_b200.build)")
+                import torch  # noqa: F401  (the module links libtorch)
+
+                spec = importlib.util.spec_from_file_location("_bsattn_torch", NATIVE_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _native = module
+    return _native
 
 
 def status_string(status: int) -> str:

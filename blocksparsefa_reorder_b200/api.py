@@ -13,7 +13,6 @@ moves to new position ``i``; the output comes back in the original order.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from typing import Optional
@@ -28,19 +27,6 @@ _KERNELS = {"auto": _lib.KERNEL_AUTO, "simt": _lib.KERNEL_SIMT, "tcgen05": _lib.
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Context in which `device` is the current one (no work when it already is)."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def raw_stream(device: torch.device) -> int:
-    """The current stream's handle, without building a stream object for it."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _require_cuda(t, name: str) -> None:
