@@ -17,18 +17,20 @@
 //
 // A CTA runs two streams, each with its own softmax warpgroup, S and O
 // columns in tensor memory:
-//  * rows above 128: stream s takes rows 128 s .. 128 s + 127 of a 256-row
-//    tile, and both read each K / V tile once from shared memory;
-//  * at most 128 rows: both streams hold the same rows, stream s takes the key
-//    tiles of parity s, and the epilogue joins the two.
+//  * a tile of two subtiles (up to 128 rows each): stream s takes subtile s, and
+//    both read each K / V tile once from shared memory;
+//  * a unit of one subtile: both streams hold the same rows, stream s takes the
+//    key tiles of parity s, and the epilogue joins the two.
+// A subtile is a box of tokens x query heads x sequences, one TMA load.
 // While one stream's softmax runs, the tensor cores work for the other.
 // Per stream: S_i = Q K_i^T into TMEM, softmax (one row a thread) writes P_i as
 // 16-bit pairs over S_i, then O += P_i V_i, then S_i+1; so S_i+1 seen complete
 // means PV_i complete, and the softmax may rescale O and hand back the stages
 // of V_i and K_i+1 without any further commit.
-// Roles: warp 0 TMA producer; warp 1 one thread issues tcgen05.mma; warps
-// 2-3 gather query rows of several heads (or sequences) into one tile where a
-// head has fewer than 128; warpgroups 1, 2 softmax of streams 0, 1; warpgroup 3 epilogue.
+// Roles: warp 0 TMA producer; warp 1 issues tcgen05.mma (whole warp, one elected
+// lane: with the operands in uniform registers a group of 8 takes 230 cycles to
+// issue, from a diverged thread 560); warpgroups 1, 2 softmax of streams 0, 1;
+// warpgroup 3 epilogue.
 //
 // Bound: 4 rows keys D flops against the tensor rate and, row by row, the 16
 // exponentials a clock of an SM (as many cycles as the products at D = 128);
@@ -61,17 +63,24 @@ constexpr int kRegsSplitD = kRegsIssueD + 2 * kRegsSoftmaxD + kRegsEpilogueD;
 static_assert(128 * kRegsSplitD <= kThreadsD * kRegsLaunchD, "register split");
 
 // One source of keys.  Row r of a unit is query (sequence, head, token):
-// r = (seq * G + g) * M + m.
+// r = (seq * G + g) * M + m.  Its rows lie in subtiles of mt tokens x gh heads x
+// nb sequences, the tokens fastest.
 struct DensePart {
   int rows;        // of a unit: seqs * G * M
-  int tiles;       // row tiles of a unit
+  int seqs;        // sequences of a unit
+  int mt, gh, nb;  // a subtile's tokens, heads, sequences
+  int nm, ng;      // subtiles along the tokens and the heads of a unit
+  int subs;        // subtiles of a unit
+  int tiles;       // row tiles of a unit: two subtiles each (dual: one)
   int splits;      // key ranges
   int chunk;       // key tiles of a range
   int keys;        // keys the tensors hold
   int items;       // units * tiles * splits
   int shared_kv;   // a unit's keys serve every sequence (units: Hk, else B * Hk)
+  int dual;        // one subtile: both streams run over its rows
   int kb_mul;      // 0: K / V batch stride 0 (one copy for the batch)
   int vb_mul;
+  int qb_mul;      // 0: the queries' batch stride is 0
   int causal;      // query m of M sees keys below len - (M - 1 - m)
   const void* lens;  // [B] valid keys, or null (all)
   float* part_o;   // partial results, or null: this part is the whole result
@@ -83,11 +92,6 @@ struct DenseParams {
   int nparts;
   int B, H, Hk, G, M;
   int lens_i64;
-  int packed;      // query rows gathered by warps 2-3 (fewer than 128 queries a head)
-  int dual;        // bit i: part i runs both streams over the same rows
-  int qb_mul;      // 0: the queries' batch stride is 0
-  const uint8_t* q;
-  int64_t qs_b, qs_h, qs_n;
   uint8_t* o;
   int64_t os_b, os_h, os_n;
   float* lse;
@@ -112,14 +116,13 @@ struct DenseCfg {
 
 // One item as every role derives it from its number.
 struct Item {
-  int part, unit, tile, split;
+  int part, unit, split;
   int nk;       // key tiles to do
   int k0;       // first key
   int len;      // valid keys of the unit (all its sequences alike, but for causal rows)
-  int rows;     // rows of the tile: 1 .. 256 (dual: 1 .. 128)
+  int sub0;     // first subtile
+  int nsub;     // 1 or 2
   int b, hk;    // K / V coordinates (b: of the only sequence)
-  int row0;     // packed: first row of the unit in the tile
-  int qb, qh, m0;  // not packed: the tile's query sequence, head and first token
   bool dual;
 };
 
@@ -139,8 +142,10 @@ __device__ __forceinline__ void get_item(const DenseParams& p, int w, Item& it) 
   it.unit = w / per_unit;
   w -= it.unit * per_unit;
   it.split = w / pt.tiles;  // neighbouring CTAs: the same keys, so K / V come from L2
-  it.tile = w - it.split * pt.tiles;
-  it.dual = (p.dual >> it.part) & 1;
+  const int tile = w - it.split * pt.tiles;
+  it.dual = pt.dual != 0;
+  it.sub0 = 2 * tile;
+  it.nsub = min(2, pt.subs - it.sub0);
   if (pt.shared_kv) {
     it.b = 0;
     it.hk = it.unit;
@@ -153,30 +158,26 @@ __device__ __forceinline__ void get_item(const DenseParams& p, int w, Item& it) 
   it.k0 = it.split * pt.chunk * 128;
   const int left = it.len - it.k0;
   it.nk = left <= 0 ? 0 : min(pt.chunk, (left + 127) / 128);
-  const int per = it.dual ? 128 : 256;
-  if (p.packed) {
-    it.row0 = it.tile * per;
-    it.rows = min(per, pt.rows - it.row0);
-    it.qb = it.qh = it.m0 = 0;
-  } else {
-    const int mt = (p.M + per - 1) / per;
-    const int hh = it.tile / mt;  // seq * G + g
-    it.m0 = (it.tile - hh * mt) * per;
-    it.rows = min(per, p.M - it.m0);
-    const int sq = hh / p.G;
-    it.qb = pt.shared_kv ? sq : it.b;
-    it.qh = it.hk * p.G + (hh - sq * p.G);
-    it.row0 = hh * p.M + it.m0;
-  }
 }
 
-// (sequence, head, token) of row `r` of the unit.
-__device__ __forceinline__ void row_of(const DenseParams& p, const Item& it, int r, int& b, int& h, int& m) {
-  const int sg = r / p.M;
-  m = r - sg * p.M;
-  const int sq = sg / p.G;
-  h = it.hk * p.G + (sg - sq * p.G);
-  b = p.part[it.part].shared_kv ? sq : it.b;
+// First token, head (of the group) and sequence (of the unit) of a subtile.
+__device__ __forceinline__ void origin_of(const DensePart& pt, int sub, int& m0, int& g0, int& s0) {
+  const int q = sub / pt.nm, r = q / pt.ng;
+  m0 = (sub - q * pt.nm) * pt.mt;
+  g0 = (q - r * pt.ng) * pt.gh;
+  s0 = r * pt.nb;
+}
+
+// Row `rl` of subtile `sub`: its head of the group, token and sequence of the
+// unit; false where the subtile has no such row.
+__device__ __forceinline__ bool row_of(const DenseParams& p, const DensePart& pt, int sub, int rl, int& sq, int& g, int& m) {
+  int m0, g0, s0;
+  origin_of(pt, sub, m0, g0, s0);
+  const int q = rl / pt.mt, r = q / pt.gh;
+  m = m0 + rl - q * pt.mt;
+  g = g0 + q - r * pt.gh;
+  sq = s0 + r;
+  return r < pt.nb && m < p.M && g < p.G && sq < pt.seqs;
 }
 
 // Stage positions of K_t and V_t in the item's sequence of 2 nk loads (the
@@ -187,7 +188,7 @@ __device__ __forceinline__ int v_at(const Item& it, int t) {
 }
 // steps of stream s, and the key tile of its i-th step
 __device__ __forceinline__ int steps_of(const Item& it, int s) {
-  return it.dual ? (it.nk - s + 1) / 2 : (it.rows > 128 * s ? it.nk : 0);
+  return it.dual ? (it.nk - s + 1) / 2 : (s < it.nsub ? it.nk : 0);
 }
 __device__ __forceinline__ int tile_of(const Item& it, int s, int i) { return it.dual ? 2 * i + s : i; }
 
@@ -200,10 +201,6 @@ struct Ring {
     if (++st == SL) st = 0, ph ^= 1;
   }
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 
 // The values loaded by tcgen05.ld may be used from here on: they pass through
 // the wait, so that no use of them can move ahead of it.
@@ -220,9 +217,9 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreadsD, 1)
-    attn_dense_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK0,
-                      const __grid_constant__ CUtensorMap tmV0, const __grid_constant__ CUtensorMap tmK1,
-                      const __grid_constant__ CUtensorMap tmV1, const __grid_constant__ DenseParams p) {
+    attn_dense_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant__ CUtensorMap tmK0,
+                      const __grid_constant__ CUtensorMap tmV0, const __grid_constant__ CUtensorMap tmQ1,
+                      const __grid_constant__ CUtensorMap tmK1, const __grid_constant__ CUtensorMap tmV1, const __grid_constant__ DenseParams p) {
   using C = DenseCfg<D>;
   constexpr int SL = C::SLOTS;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -256,7 +253,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(q_full, p.packed ? 2 : 1);
+    mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -289,7 +286,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
     regs_dec<kRegsIssueD>();
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ producer
-      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmQ0);
       tma_prefetch_desc(&tmK0);
       tma_prefetch_desc(&tmV0);
       int c = 0;      // loads so far
@@ -315,14 +312,16 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         };
         if (!(ok = load(false, 0))) break;
         if (it.dual && it.nk > 1 && !(ok = load(false, 1))) break;
-        if (!p.packed) {
-          if (nq > 0 && !(ok = wait(q_empty, nq - 1))) break;
-          const int nsub = it.rows > 128 ? 2 : 1;
-          mbar_arrive_expect_tx(q_full, nsub * C::TILE);
-          for (int s = 0; s < nsub; ++s)
-            for (int ch = 0; ch < C::NCHUNK; ++ch)
-              tma_load_4d(sQ + s * C::TILE + ch * C::CHUNK, &tmQ, q_full, ch * 64, it.m0 + s * 128, it.qh,
-                          it.qb * p.qb_mul);
+        if (nq > 0 && !(ok = wait(q_empty, nq - 1))) break;
+        const int box = pt.mt * pt.gh * pt.nb * 128;  // bytes of one 64-column chunk
+        mbar_arrive_expect_tx(q_full, it.nsub * C::NCHUNK * box);
+        for (int s = 0; s < it.nsub; ++s) {
+          int m0, g0, s0;
+          origin_of(pt, it.sub0 + s, m0, g0, s0);
+          const int qb = (pt.shared_kv ? s0 : it.b) * pt.qb_mul;
+          for (int ch = 0; ch < C::NCHUNK; ++ch)
+            tma_load_4d(sQ + s * C::TILE + ch * C::CHUNK, it.part ? &tmQ1 : &tmQ0, q_full, ch * 64, m0,
+                        it.hk * p.G + g0, qb);
         }
         ++nq;
         const int ahead = it.dual ? 2 : 1;
@@ -335,7 +334,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       allow_dependents();
       // every load issued lands before the CTA exits
       for (int i = c > SL ? c - SL : 0; i < c; ++i) mbar_wait(&full[i % SL], (i / SL) & 1, nullptr, nullptr, p.wait_ns);
-      if (!p.packed && nq > 0) mbar_wait(q_full, (nq - 1) & 1, nullptr, nullptr, p.wait_ns);
+      if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, nullptr, nullptr, p.wait_ns);
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issue
       // One thread, with nothing between the MMAs but adding to descriptors:
@@ -422,41 +421,6 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         mbar_wait(drain, 0, nullptr, nullptr, p.wait_ns);
       }
       __syncwarp();
-    } else if (warp >= 2 && p.packed) {
-      // ------------------------------------------------------ query rows of several heads
-      int nq = 0;
-      bool ok = true;
-      for (int w = blockIdx.x; w < total; w += gridDim.x) {
-        Item it;
-        get_item(p, w, it);
-        if (it.nk == 0) continue;
-        if (nq > 0) ok = ok && wait_all(q_empty, nq - 1);
-        ++nq;
-        if (!ok) continue;
-        // The warps take 32 rows each in turn: a lane finds one row's
-        // place, then the D / 8 pieces of a row are copied by neighbouring lanes.
-        constexpr int PIECES = D / 8, PER = 32 / PIECES;  // rows a pass
-        const int piece = lane % PIECES, sub = lane / PIECES;
-        for (int base = (warp - 2) * 32; base < it.rows; base += 64) {
-          const int mine = base + lane;
-          int b, h, m;
-          row_of(p, it, it.row0 + min(mine, it.rows - 1), b, h, m);
-          const int64_t off = 2 * (b * p.qs_b + h * p.qs_h + m * p.qs_n);
-#pragma unroll 4
-          for (int x = 0; x < 32; x += PER) {
-            const int64_t at = __shfl_sync(0xffffffffu, off, x + sub);
-            const int r = base + x + sub, rr = r & 127;
-            if (r < it.rows)
-              cp_async16(smem_u32(sQ + (r >> 7) * C::TILE + (piece >> 3) * C::CHUNK + rr * 128 +
-                                  (((piece & 7) ^ (rr & 7)) * 16)),
-                         p.q + at + piece * 16, 16);
-          }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-      }
     }
   } else if (warp < 12) {
     regs_inc<kRegsSoftmaxD>();
@@ -479,16 +443,14 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         c0 += 2 * it.nk;
         continue;
       }
-      const bool releases = it.dual || it.rows <= 128 || s == 1;  // last reader of the shared tiles
+      const DensePart& pt = p.part[it.part];
+      const bool releases = it.dual || it.nsub == 1 || s == 1;  // last reader of the shared tiles
       int kst = (c0 + k_at(it, tile_of(it, s, 0))) % SL;  // stage of the step's K; its V of the step before is one below
-      const int r = it.dual ? row : s * 128 + row;
       // a warp without rows only keeps the barriers going
-      const bool any_rows = (it.dual ? 0 : s * 128) + q4 * 32 < it.rows;
-      int limit = r < it.rows ? it.len : 0;  // keys this row sees
-      if (p.part[it.part].causal && r < it.rows) {
-        const int m = (it.row0 + r) % p.M;
-        limit = max(0, it.len - (p.M - 1 - m));
-      }
+      const bool any_rows = q4 * 32 < pt.mt * pt.gh * pt.nb;
+      int sq, g, m;
+      int limit = row_of(p, pt, it.sub0 + (it.dual ? 0 : s), row, sq, g, m) ? it.len : 0;  // keys this row sees
+      if (pt.causal) limit = max(0, limit - (p.M - 1 - m));
       float m_run = -INFINITY, l_run = 0.f;
       for (int i = 0; i < n; ++i, ++ns) {
         if (!(ok = ok && wait_all(&s_full[s], ns))) continue;
@@ -624,7 +586,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       get_item(p, w, it);
       const DensePart& pt = p.part[it.part];
       const int nst = it.nk == 0 ? 0 : (steps_of(it, 1) > 0 ? 2 : 1);  // streams with an O
-      const int passes = it.dual || it.rows <= 128 ? 1 : 2;
+      const int passes = it.dual ? 1 : it.nsub;
       for (int ps = 0; ps < passes; ++ps) {
         // streams whose O make up this pass's rows: [first, last)
         const int first = it.dual ? 0 : ps, last = it.nk == 0 ? first : (it.dual ? nst : ps + 1);
@@ -641,8 +603,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           ++ni[s];
         }
         if (ok) tc_fence_after();
-        const int r = ps * 128 + row;
-        const bool store = ok && r < it.rows;
+        int sq, g, mm;
+        const bool store = row_of(p, pt, it.sub0 + ps, row, sq, g, mm) && ok;
         // weights of the streams' sums: 2^(m_s - max) / l, 0 for a stream without any key
         const float mx = fmaxf(l[0] > 0.f ? m[0] : -INFINITY, l[1] > 0.f ? m[1] : -INFINITY);
         float f0 = l[0] > 0.f ? ex2_approx(m[0] - mx) : 0.f;
@@ -654,12 +616,13 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         f0 *= inv;
         f1 *= inv;
         const float lse = nan ? NAN : (lt > 0.f ? mx + log2f(lt) : -INFINITY);
-        int b = 0, h = 0, mm = 0;
-        row_of(p, it, it.row0 + (r < it.rows ? r : 0), b, h, mm);
         // a row's place in the result, or in the partial results
-        const int64_t slot = (static_cast<int64_t>(it.unit) * pt.rows + it.row0 + r) * pt.splits + it.split;
-        uint8_t* const mine = pt.part_o ? reinterpret_cast<uint8_t*>(pt.part_o + slot * D)
-                                        : p.o + 2 * (b * p.os_b + h * p.os_h + mm * p.os_n);
+        const int b = pt.shared_kv ? sq : it.b, h = it.hk * p.G + g;
+        const int64_t slot =
+            (static_cast<int64_t>(it.unit) * pt.rows + (static_cast<int64_t>(sq) * p.G + g) * p.M + mm) * pt.splits + it.split;
+        uint8_t* const mine = !store ? nullptr
+                              : pt.part_o ? reinterpret_cast<uint8_t*>(pt.part_o + slot * D)
+                                          : p.o + 2 * (b * p.os_b + h * p.os_h + mm * p.os_n);
         const bool have = it.nk > 0;
         if (have || !pt.part_o) {  // (a partial result without keys is only its lse)
 #pragma unroll 1
@@ -689,7 +652,6 @@ __global__ void __launch_bounds__(kThreadsD, 1)
                 for (int s = first; s < last; ++s) mbar_arrive(&o_empty[s]);
             }
             // 32 columns: 8 pieces of 16 bytes in fp32, 4 in 16 bits
-            const int row0 = ps * 128 + q4 * 32;
             if (pt.part_o) {
               uint4 x[8];
 #pragma unroll
@@ -698,8 +660,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 const int from = (lane & 24) + k;
-                uint8_t* dst = shfl_ptr(mine, from) + ch * 128 + (lane & 7) * 16;
-                if (ok && row0 + from < it.rows) *reinterpret_cast<uint4*>(dst) = x[k];
+                uint8_t* dst = shfl_ptr(mine, from);
+                if (dst) *reinterpret_cast<uint4*>(dst + ch * 128 + (lane & 7) * 16) = x[k];
               }
             } else {
               uint4 x[4];
@@ -714,8 +676,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const int from = (lane & 28) + k;
-                uint8_t* dst = shfl_ptr(mine, from) + ch * 64 + (lane & 3) * 16;
-                if (ok && row0 + from < it.rows) *reinterpret_cast<uint4*>(dst) = x[k];
+                uint8_t* dst = shfl_ptr(mine, from);
+                if (dst) *reinterpret_cast<uint4*>(dst + ch * 64 + (lane & 3) * 16) = x[k];
               }
             }
           }
@@ -862,7 +824,8 @@ struct DenseCall {
 struct Source {
   bool few;                   // attn_few.cu
   bool dual;                  // both streams over the same rows
-  int units, rows, tiles;
+  int units, rows, seqs;
+  int mt, gh, nb, nm, ng, subs, tiles;  // as in DensePart
   int splits, chunk;          // key ranges; key tiles (few: keys) of each
   size_t o_off, lse_off;      // partial results in the workspace
 };
@@ -874,18 +837,28 @@ struct DensePlan {
 
 Source source_of(const DenseCall& c, int i) {
   Source s{};
-  const int G = c.H / c.Hk, seqs = c.shared_kv[i] ? c.B : 1;
+  const int G = c.H / c.Hk;
+  s.seqs = c.shared_kv[i] ? c.B : 1;
   s.units = c.shared_kv[i] ? c.Hk : c.B * c.Hk;
-  s.rows = seqs * G * c.M;
+  s.rows = s.seqs * G * c.M;
   // 9 to 16 rows leave the few-rows kernel half the warps an SM: it wins on
   // short ranges only (16 rows, 64 x 8 units of 512 keys 39 us against 48; 4 x 8
   // units of 65,536 keys 199 against 181).
   s.few = s.rows <= kFewRows / 2 || (s.rows <= kFewRows && c.keys[i] <= 8192);
-  const bool packed = c.M < 128;
-  const int one = packed ? s.rows : c.M;  // rows that can share a tile
-  s.dual = one <= 128;
-  const int per = s.dual ? 128 : 256;
-  s.tiles = packed ? (one + per - 1) / per : seqs * G * ((c.M + per - 1) / per);
+  // The subtile shape with the fewest subtiles: the tokens in equal parts of at
+  // most 128, as many heads as fit beside them, then as many sequences.
+  s.subs = INT32_MAX;
+  for (int parts = (c.M + 127) / 128, tries = 0; tries < 8 && parts <= c.M; ++parts, ++tries) {
+    const int mt = c.M >= 128 && tries == 0 ? 128 : (c.M + parts - 1) / parts;
+    const int gh = 128 / mt < G ? 128 / mt : G;
+    const int fit = 128 / (mt * gh);
+    const int nb = gh < G || (c.B > 1 && c.q.stride_b == 0) ? 1 : fit < s.seqs ? fit : s.seqs;
+    const int nm = (c.M + mt - 1) / mt, ng = (G + gh - 1) / gh, ns = (s.seqs + nb - 1) / nb;
+    if (static_cast<int64_t>(nm) * ng * ns >= s.subs) continue;
+    s.mt = mt, s.gh = gh, s.nb = nb, s.nm = nm, s.ng = ng, s.subs = nm * ng * ns;
+  }
+  s.dual = s.subs == 1;
+  s.tiles = (s.subs + 1) / 2;
   s.splits = 1;
   return s;
 }
@@ -972,14 +945,15 @@ DensePlan plan_of(const DenseCall& c) {
 }
 
 // A tensor map's batch dimension of 1 where the batch shares one copy.
-int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul) {
+int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul, int rows = 128, int heads = 1,
+           int batch = 1) {
   const bool one = B == 1 || t.stride_b == 0;
   *mul = one ? 0 : 1;
   // a dimension of length 1 has no stride of its own
   if (one) t.stride_b = 8;
   if (H == 1) t.stride_h = 8;
   if (N == 1) t.stride_n = 8;
-  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, 128);
+  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, rows, heads, batch);
 }
 
 cudaLaunchConfig_t config(unsigned grid, int threads, int smem, cudaStream_t st, cudaLaunchAttribute* attr) {
@@ -1035,17 +1009,16 @@ int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStrea
   int r;
   if ((r = opt_in_smem(reinterpret_cast<const void*>(kern), C::SMEM))) return r;
   DenseParams p{};
-  CUtensorMap mq{}, mk[2] = {}, mv[2] = {};
-  p.packed = c.M < 128;
-  // (gathered query rows need no map; the kernel then never reads it)
-  if (!p.packed && (r = map_of(&mq, c.q, c.B, c.H, c.M, D, BF16, &p.qb_mul))) return r;
+  CUtensorMap mq[2] = {}, mk[2] = {}, mv[2] = {};
   for (int i = 0; i < c.n; ++i) {
     const Source& s = pl.s[i];
     if (s.few) continue;
     const int j = p.nparts++;
     DensePart& pt = p.part[j];
-    pt.rows = s.rows;
+    pt.rows = s.rows, pt.seqs = s.seqs;
+    pt.mt = s.mt, pt.gh = s.gh, pt.nb = s.nb, pt.nm = s.nm, pt.ng = s.ng, pt.subs = s.subs;
     pt.tiles = s.tiles;
+    pt.dual = s.dual;
     pt.splits = s.splits;
     pt.chunk = s.chunk;
     pt.keys = c.keys[i];
@@ -1054,7 +1027,7 @@ int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStrea
     pt.causal = c.causal[i];
     pt.lens = c.lens[i];
     if (pl.join) pt.part_o = part_o(s, ws), pt.part_lse = part_lse(s, ws);
-    p.dual |= s.dual ? 1 << j : 0;
+    if ((r = map_of(&mq[j], c.q, c.B, c.H, c.M, D, BF16, &pt.qb_mul, s.mt, s.gh, s.nb))) return r;
     if (!c.keys[i]) continue;  // no key tile is ever loaded
     const int kb = c.shared_kv[i] ? 1 : c.B;
     if ((r = map_of(&mk[j], c.k[i], kb, c.Hk, c.keys[i], D, BF16, &pt.kb_mul))) return r;
@@ -1062,8 +1035,6 @@ int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStrea
   }
   p.B = c.B, p.H = c.H, p.Hk = c.Hk, p.G = c.H / c.Hk, p.M = c.M;
   p.lens_i64 = c.lens_dtype == BSA_INDEX_I64;
-  p.q = static_cast<const uint8_t*>(c.q.data);
-  p.qs_b = c.q.stride_b, p.qs_h = c.q.stride_h, p.qs_n = c.q.stride_n;
   p.o = static_cast<uint8_t*>(c.o.data);
   p.os_b = c.o.stride_b, p.os_h = c.o.stride_h, p.os_n = c.o.stride_n;
   p.lse = c.lse;
@@ -1073,7 +1044,7 @@ int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStrea
   const int total = p.part[0].items + p.part[1].items;
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = config(total < kSMs ? total : kSMs, kThreadsD, C::SMEM, st, attr);
-  BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq, mk[0], mv[0], mk[1], mv[1], p));
+  BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq[0], mk[0], mv[0], mq[1], mk[1], mv[1], p));
   return BSA_OK;
 }
 

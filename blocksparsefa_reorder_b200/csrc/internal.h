@@ -40,9 +40,11 @@ int launch_bwd_delta(const bsa_tensor4d& o, const bsa_tensor4d& dout, float* del
 
 // tma_maps.cu: whether the tcgen05 path takes these arguments (bf16 / fp16,
 // D 64 or 128, BLOCK 64 or 128, 16-byte-aligned rows), and the 4-D TMA map
-// over a [B, H, N, D] 16-bit tensor, box 64 x rows, 128-byte swizzle.
+// over a [B, H, N, D] 16-bit tensor, box 64 x rows (x heads x batch), 128-byte
+// swizzle.
 bool attn_tc_supported(const bsa_fwd_args* a);
-int make_tensor_map_4d(CUtensorMap* m, const bsa_tensor4d& t, int B, int H, int N, int D, bool bf16, int rows);
+int make_tensor_map_4d(CUtensorMap* m, const bsa_tensor4d& t, int B, int H, int N, int D, bool bf16, int rows,
+                       int box_h = 1, int box_b = 1);
 
 // attn_tcp.cu: the persistent tcgen05 attention forward
 // q_perm (optional, bsa_index_dtype perm_dtype): gather Q rows from and

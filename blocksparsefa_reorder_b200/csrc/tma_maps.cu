@@ -28,10 +28,11 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
 
 }  // namespace
 
-// 4-D map over [B, H, N, D] (TMA order: D, N, H, B), box = 64 x rows, 128B
-// swizzle; strides are the caller's, so [B,H,N,D] and [B,N,H,D] memory both
+// 4-D map over [B, H, N, D] (TMA order: D, N, H, B), box = 64 x rows (x heads x
+// batch, in that order), 128B swizzle; strides are the caller's, so [B,H,N,D] and [B,N,H,D] memory both
 // work without a copy.
-int make_tensor_map_4d(CUtensorMap* m, const bsa_tensor4d& tdesc, int B, int H, int N, int D, bool bf16, int rows) {
+int make_tensor_map_4d(CUtensorMap* m, const bsa_tensor4d& tdesc, int B, int H, int N, int D, bool bf16, int rows,
+                       int box_h, int box_b) {
   auto enc = get_encode_fn();
   if (!enc) return BSA_ERR_CUDA;
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(H),
@@ -39,7 +40,8 @@ int make_tensor_map_4d(CUtensorMap* m, const bsa_tensor4d& tdesc, int B, int H, 
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(tdesc.stride_n) * 2,
                                  static_cast<cuuint64_t>(tdesc.stride_h) * 2,
                                  static_cast<cuuint64_t>(tdesc.stride_b) * 2};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(box_h),
+                             static_cast<cuuint32_t>(box_b)};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, tdesc.data, dims,
                    strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

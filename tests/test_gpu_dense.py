@@ -159,6 +159,33 @@ def test_cross_layouts_and_expanded_batch():
     _check_o(cross_attention(q, wide_k, wide_v), None, _cross_ref(q, wide_k, wide_v, None, 1 / 8))
 
 
+@pytest.mark.parametrize("M,G", [(1, 24), (3, 50), (40, 6), (65, 8), (100, 4), (129, 4), (43, 3)])
+def test_cross_tiles_of_tokens_heads_and_sequences(M, G):
+    """Row tiles that hold several heads, some of them cut; queries expanded over
+    the batch."""
+    g = torch.Generator(device="cuda").manual_seed(M + G)
+    B, Hk, N, D = 2, 2, 300, 64
+    k, v = _rand((B, Hk, N, D), BF, g), _rand((B, Hk, N, D), BF, g)
+    for q in (_rand((B, Hk * G, M, D), BF, g), _rand((1, Hk * G, M, D), BF, g).expand(B, -1, -1, -1)):
+        o, lse = cross_attention(q, k, v, return_lse=True)
+        _check_o(o, lse, _cross_ref(q, k, v, None, 1 / 8))
+
+
+@pytest.mark.parametrize("B,T,G", [(37, 1, 8), (13, 5, 3), (9, 30, 2), (5, 50, 3), (3, 129, 2)])
+def test_prefix_tiles_of_tokens_heads_and_sequences(B, T, G):
+    g = torch.Generator(device="cuda").manual_seed(B + T + G)
+    Hk, P, C, D = 2, 333, T + 3, 64
+    q = _rand((B, Hk * G, T, D), HF, g)
+    kp, vp = _rand((Hk, P, D), HF, g), _rand((Hk, P, D), HF, g)
+    k, v = _rand((B, Hk, C, D), HF, g), _rand((B, Hk, C, D), HF, g)
+    o, lse = shared_prefix_attention(q, kp, vp, k, v, return_lse=True)
+    t = torch.arange(T, device="cuda")
+    own = (torch.arange(C, device="cuda") < (C - (T - 1 - t)[:, None])).expand(B, T, C)
+    seen = torch.cat((torch.ones(B, T, P, dtype=torch.bool, device="cuda"), own), -1)[:, None].expand(B, Hk * G, T, P + C)
+    kk, vv = torch.cat((kp.expand(B, -1, -1, -1), k), 2), torch.cat((vp.expand(B, -1, -1, -1), v), 2)
+    _check_o(o, lse, _attend(q, _heads(kk, Hk * G), _heads(vv, Hk * G), seen, 1 / 8))
+
+
 def test_cross_empty_and_out_of_range_lengths():
     g = torch.Generator(device="cuda").manual_seed(6)
     q, k, v = _rand((2, 2, 5, 64), BF, g), _rand((2, 2, 70, 64), BF, g), _rand((2, 2, 70, 64), BF, g)
