@@ -104,10 +104,24 @@ struct Turn {
   bool on;      // this lane's elements are rotated
 };
 
-template <bool IL>
-__device__ __forceinline__ void other_half(const float (&x)[8], const Turn& t, float (&o)[8]) {
+// The other halves of a row's pairs: from the lane's own values, or from the
+// partner lane's, shuffled as they were loaded (a 16-bit pair a shuffle).
+template <typename T, bool IL>
+__device__ __forceinline__ void other_half(const Vec8<T>& raw, const float (&x)[8], int partner, float (&o)[8]) {
+  if constexpr (IL) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = IL ? x[i ^ 1] : __shfl_sync(0xffffffffu, x[i], t.partner);
+    for (int i = 0; i < 8; ++i) o[i] = x[i ^ 1];
+  } else {
+    Vec8<T> r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+      r.v[i].x = __shfl_sync(0xffffffffu, raw.v[i].x, partner);
+      r.v[i].y = __shfl_sync(0xffffffffu, raw.v[i].y, partner);
+      r.v[i].z = __shfl_sync(0xffffffffu, raw.v[i].z, partner);
+      r.v[i].w = __shfl_sync(0xffffffffu, raw.v[i].w, partner);
+    }
+    unpack8<T>(r, o);
+  }
 }
 
 // The angles of element group `l` (8 elements) at table row `pos`.
@@ -163,11 +177,13 @@ __device__ __forceinline__ bool token_pos(const RopeParams& p, int64_t b, int64_
   return p.R == 0 || (pos >= 0 && pos < p.table_len);
 }
 
-// U rows (heads of one token) are loaded before the first is used: 4 x 16
-// bytes in flight a thread.
+// U rows (heads of one token) are in flight while U are computed: loads of the
+// first ones go out before the position and its table row are known, and four
+// blocks an SM keep 64 KB on the way.  (16 + 16 heads x 16,384 tokens x 128, bf16,
+// 277 MB: 65 us with the loads behind the table and three blocks an SM.)
 template <typename T, int LPR, bool IL>
-__global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const RopeParams p) {
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;
+__global__ void __launch_bounds__(kThreads, 4) rope_fwd_kernel(const RopeParams p) {
+  constexpr int U = sizeof(T) == 4 ? 1 : 2;
   constexpr int E = sizeof(T);
   const int lane = threadIdx.x & 31, l = lane % LPR;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * (kThreads / LPR) + threadIdx.x / LPR;
@@ -178,20 +194,33 @@ __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const RopeParams p) 
   const bool live = token < p.tokens;
   const bool in = live && l * 8 < p.D;
   const int64_t b = live ? token / p.N : 0, n = live ? token - b * p.N : 0;
+  const uint8_t* xp = sd.x + E * (b * sd.xs_b + n * sd.xs_n + l * 8);
+  uint8_t* yp = sd.y + E * (b * sd.ys_b + n * sd.ys_n + l * 8);
+  Vec8<T> next[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) next[u] = in && h0 + u < h1 ? load8<T>(xp + E * ((h0 + u) * sd.xs_h)) : zero8<T>();
   int64_t pos = 0;
   const bool valid = live && token_pos(p, b, n, pos);
   if (live && !valid && l == 0) set_err(p.err, BSA_DEVERR_COORD);
   Turn t;
   load_turn<IL>(p, l, lane, pos, valid, t);
-  float w[8];
-  load_weight<T>(sd.w, p.w_f32, l, in, w);
-  const uint8_t* xp = sd.x + E * (b * sd.xs_b + n * sd.xs_n + l * 8);
-  uint8_t* yp = sd.y + E * (b * sd.ys_b + n * sd.ys_n + l * 8);
+  // y = r (x o A + other half o B): weights and angles in one factor each
+  float A[8], B[8];
+  load_weight<T>(sd.w, p.w_f32, l, in, A);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    B[i] = t.s[i] * (IL ? A[i ^ 1] : __shfl_sync(0xffffffffu, A[i], t.partner));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) A[i] *= t.c[i];
+  const float inv_d = 1.f / static_cast<float>(p.D);
   for (int h = h0; h < h1; h += U) {
     Vec8<T> raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      raw[u] = in && h + u < h1 ? load8<T>(xp + E * ((h + u) * sd.xs_h)) : zero8<T>();
+    for (int u = 0; u < U; ++u) {
+      raw[u] = next[u];
+      next[u] = in && h + U + u < h1 ? load8<T>(xp + E * ((h + U + u) * sd.xs_h)) : zero8<T>();
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float x[8], o[8];
@@ -200,18 +229,15 @@ __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const RopeParams p) 
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
       ss = group_sum<LPR>(ss);
-      const float r = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
-      other_half<IL>(x, t, o);
+      // (a position outside the table: NaN rather than a row that looks right)
+      const float r = valid ? rsqrtf(fmaf(ss, inv_d, p.eps)) : NAN;
+      other_half<T, IL>(raw[u], x, t.partner, o);
       if (t.on) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], t.c[i], o[i] * t.s[i]);
-      }
-      // a position outside the table: NaN rather than a row that looks right
-      if (!valid) {
+        for (int i = 0; i < 8; ++i) x[i] = r * fmaf(x[i], A[i], o[i] * B[i]);
+      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = NAN;
+        for (int i = 0; i < 8; ++i) x[i] = r * (x[i] * A[i]);
       }
       if (in && h + u < h1) store8<T>(yp + E * ((h + u) * sd.ys_h), x);
     }
@@ -223,8 +249,7 @@ __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const RopeParams p) 
 // block adds its groups in a fixed order and writes one row of `partial`.
 // grid.y: 0 = queries, 1 = keys.
 template <typename T, int LPR, bool IL>
-__global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const RopeParams p) {
-  constexpr int U = 2;
+__global__ void __launch_bounds__(kThreads, 3) rope_bwd_kernel(const RopeParams p) {
   constexpr int E = sizeof(T);
   constexpr int GP = kThreads / LPR;
   __shared__ float sums[GP][LPR * 8 + 4];
@@ -235,6 +260,7 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const RopeParams p) 
   load_weight<T>(sd.w, p.w_f32, l, cols, w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[i] = 0.f;
+  const float inv_d = 1.f / static_cast<float>(p.D);
   const int chunks = (sd.heads + p.chunk - 1) / p.chunk;
   const int64_t items = p.tokens * chunks;
   // whole blocks stay in the loop together (the shuffles name every lane)
@@ -246,52 +272,48 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const RopeParams p) 
     const int64_t b = token / p.N, n = token - b * p.N;
     const int h0 = static_cast<int>(ck) * p.chunk, h1 = min(h0 + p.chunk, sd.heads);
     const bool in = live && cols;
+    const uint8_t* xp = sd.x + E * (b * sd.xs_b + n * sd.xs_n + l * 8);
+    const uint8_t* dp = sd.dy + E * (b * sd.ds_b + n * sd.ds_n + l * 8);
+    uint8_t* yp = sd.y + E * (b * sd.ys_b + n * sd.ys_n + l * 8);
+    Vec8<T> nx = in ? load8<T>(xp + E * (h0 * sd.xs_h)) : zero8<T>();
+    Vec8<T> nd = in ? load8<T>(dp + E * (h0 * sd.ds_h)) : zero8<T>();
     int64_t pos = 0;
     const bool valid = live && token_pos(p, b, n, pos);
     if (live && !valid && l == 0) set_err(p.err, BSA_DEVERR_COORD);
     Turn t;
     load_turn<IL>(p, l, lane, pos, valid, t);
-    const uint8_t* xp = sd.x + E * (b * sd.xs_b + n * sd.xs_n + l * 8);
-    const uint8_t* dp = sd.dy + E * (b * sd.ds_b + n * sd.ds_n + l * 8);
-    uint8_t* yp = sd.y + E * (b * sd.ys_b + n * sd.ys_n + l * 8);
-    for (int hh = 0; hh < p.chunk; hh += U) {
+    for (int hh = 0; hh < p.chunk; ++hh) {
       const int h = h0 + hh;
-      Vec8<T> rx[U], rd[U];
+      const Vec8<T> rx = nx, rd = nd;
+      const bool more = in && hh + 1 < p.chunk && h + 1 < h1;
+      nx = more ? load8<T>(xp + E * ((h + 1) * sd.xs_h)) : zero8<T>();
+      nd = more ? load8<T>(dp + E * ((h + 1) * sd.ds_h)) : zero8<T>();
+      float x[8], g[8], o[8];
+      unpack8<T>(rx, x);
+      unpack8<T>(rd, g);
+      other_half<T, IL>(rd, g, t.partner, o);
+      if (t.on) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool ok = in && h + u < h1;
-        rx[u] = ok ? load8<T>(xp + E * ((h + u) * sd.xs_h)) : zero8<T>();
-        rd[u] = ok ? load8<T>(dp + E * ((h + u) * sd.ds_h)) : zero8<T>();
+        for (int i = 0; i < 8; ++i) g[i] = fmaf(g[i], t.c[i], -o[i] * t.s[i]);
       }
+      float ss = 0.f, dot = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[8], g[8], o[8];
-        unpack8<T>(rx[u], x);
-        unpack8<T>(rd[u], g);
-        other_half<IL>(g, t, o);
-        if (t.on) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = fmaf(g[i], t.c[i], -o[i] * t.s[i]);
-        }
-        float ss = 0.f, dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss = fmaf(x[i], x[i], ss);
-          dot = fmaf(g[i] * w[i], x[i], dot);
-        }
-        ss = group_sum<LPR>(ss);
-        dot = group_sum<LPR>(dot);
-        const float r = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
-        const float m = dot * r / static_cast<float>(p.D);  // mean(u o n)
-        const bool ok = in && h + u < h1;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float nn = x[i] * r;
-          if (ok) dw[i] = fmaf(g[i], nn, dw[i]);
-          x[i] = valid ? r * (g[i] * w[i] - nn * m) : NAN;
-        }
-        if (ok) store8<T>(yp + E * ((h + u) * sd.ys_h), x);
+      for (int i = 0; i < 8; ++i) {
+        ss = fmaf(x[i], x[i], ss);
+        dot = fmaf(g[i] * w[i], x[i], dot);
       }
+      ss = group_sum<LPR>(ss);
+      dot = group_sum<LPR>(dot);
+      const float r = rsqrtf(fmaf(ss, inv_d, p.eps));
+      const float m = dot * r * inv_d;  // mean(u o n)
+      const bool ok = in && h < h1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float nn = x[i] * r;
+        if (ok) dw[i] = fmaf(g[i], nn, dw[i]);
+        x[i] = valid ? r * (g[i] * w[i] - nn * m) : NAN;
+      }
+      if (ok) store8<T>(yp + E * (h * sd.ys_h), x);
     }
   }
   if (!p.partial) return;
