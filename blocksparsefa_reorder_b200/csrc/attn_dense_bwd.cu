@@ -53,11 +53,14 @@ struct DBwdCfg {
   static constexpr int NCHUNK = D / 64;
   static constexpr int CHUNK = 128 * 128;
   static constexpr int TILE = 128 * D * 2;
-  static constexpr int STAGES = D == 128 ? 2 : 4;  // of the two streamed tensors
+  // Stages of the two streamed tensors: the first (K, resp. Q) is held until
+  // the step's last product, the second until its first.
+  static constexpr int SA = D == 128 ? 3 : 5, SB = D == 128 ? 2 : 5;
   static constexpr int BAR_BYTES = 256;
   static constexpr int STATS = 2 * 2 * 128 * 4;
-  static constexpr int SMEM = (2 + 2 * STAGES) * TILE + BAR_BYTES + STATS;
+  static constexpr int SMEM = (2 + SA + SB) * TILE + BAR_BYTES + STATS;
   static_assert(SMEM <= 232448, "shared memory budget");
+  static_assert((2 * (SA + SB) + 8) * 8 + 8 <= BAR_BYTES, "barriers");
 };
 
 __device__ __forceinline__ int bwd_len(const DBwdParams& p, int b) {
@@ -129,6 +132,19 @@ __device__ __forceinline__ void zero_half_row(int half, uint8_t* row) {
   for (int g = 0; g < D / 16; ++g) reinterpret_cast<uint4*>(row)[half * (D / 16) + g] = make_uint4(0, 0, 0, 0);
 }
 
+// Two exponentials, on the FMA pipe or on the special function unit: half of
+// them each way, as a step's 64 a thread keep the unit busy for 1,024 cycles.
+__device__ __forceinline__ void ex2_pair(uint64_t x, bool fma, float& p0, float& p1) {
+  if (fma) {
+    f32x2_unpack(ex2_fma_x2(x), p0, p1);
+  } else {
+    float x0, x1;
+    f32x2_unpack(x, x0, x1);
+    p0 = ex2_approx(x0);
+    p1 = ex2_approx(x1);
+  }
+}
+
 // C (+)= A B^T of two 128 x D shared-memory tiles (K-major descriptors)
 template <int D>
 __device__ __forceinline__ void mma_abt(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
@@ -157,16 +173,18 @@ template <int D, bool BF16>
 __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmDO,
                         const DBwdParams& p, uint8_t* smem, int item) {
   using C = DBwdCfg<D>;
-  constexpr int ST = C::STAGES;
+  constexpr int SA = C::SA, SB = C::SB;
   uint8_t* sQ = smem;
   uint8_t* sDO = sQ + C::TILE;
-  uint8_t* sK = sDO + C::TILE;      // [ST]
-  uint8_t* sV = sK + ST * C::TILE;  // [ST]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * C::TILE);
+  uint8_t* sK = sDO + C::TILE;      // [SA]
+  uint8_t* sV = sK + SA * C::TILE;  // [SB]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + SB * C::TILE);
   uint64_t* q_full = bars;
-  uint64_t* kv_full = bars + 1;            // [ST]
-  uint64_t* kv_empty = kv_full + ST;       // [ST] dQ_j (the last reader) completed
-  uint64_t* s_full = kv_empty + ST;        // [2]
+  uint64_t* k_full = bars + 1;          // [SA]
+  uint64_t* k_empty = k_full + SA;      // [SA] dQ_j (its last reader) completed
+  uint64_t* v_full = k_empty + SA;      // [SB]
+  uint64_t* v_empty = v_full + SB;      // [SB] dP_j completed
+  uint64_t* s_full = v_empty + SB;      // [2]
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_ready = dp_full + 1;        // 8 elementwise warps
   uint64_t* done = ds_ready + 1;
@@ -179,9 +197,13 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+    for (int i = 0; i < SA; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < SB; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
     mbar_init(dp_full, 1);
@@ -212,18 +234,23 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
       tma_load_4d(sQ + c * C::CHUNK, &tmQ, q_full, c * 64, t * 128, h, b * p.qb_mul);
       tma_load_4d(sDO + c * C::CHUNK, &tmDO, q_full, c * 64, t * 128, h, b * p.db_mul);
     }
-    int j = 0;
-    for (; j < n; ++j) {
-      const int st = j % ST;
-      if (j >= ST && !wait(&kv_empty[st], j / ST - 1)) break;
-      mbar_arrive_expect_tx(&kv_full[st], 2 * C::TILE);
-      for (int c = 0; c < C::NCHUNK; ++c) {
-        tma_load_4d(sK + st * C::TILE + c * C::CHUNK, &tmK, &kv_full[st], c * 64, j * 128, hk, b * p.kb_mul);
-        tma_load_4d(sV + st * C::TILE + c * C::CHUNK, &tmV, &kv_full[st], c * 64, j * 128, hk, b * p.vb_mul);
-      }
+    int nk = 0, nv = 0;  // loads issued
+    for (int j = 0; j < n; ++j) {
+      const int a = j % SA, v = j % SB;
+      if (j >= SA && !wait(&k_empty[a], j / SA - 1)) break;
+      mbar_arrive_expect_tx(&k_full[a], C::TILE);
+      for (int c = 0; c < C::NCHUNK; ++c)
+        tma_load_4d(sK + a * C::TILE + c * C::CHUNK, &tmK, &k_full[a], c * 64, j * 128, hk, b * p.kb_mul);
+      ++nk;
+      if (j >= SB && !wait(&v_empty[v], j / SB - 1)) break;
+      mbar_arrive_expect_tx(&v_full[v], C::TILE);
+      for (int c = 0; c < C::NCHUNK; ++c)
+        tma_load_4d(sV + v * C::TILE + c * C::CHUNK, &tmV, &v_full[v], c * 64, j * 128, hk, b * p.vb_mul);
+      ++nv;
     }
     mbar_wait(q_full, 0, nullptr, nullptr, p.wait_ns);
-    for (int i = j > ST ? j - ST : 0; i < j; ++i) mbar_wait(&kv_full[i % ST], (i / ST) & 1, nullptr, nullptr, p.wait_ns);
+    for (int i = nk > SA ? nk - SA : 0; i < nk; ++i) mbar_wait(&k_full[i % SA], (i / SA) & 1, nullptr, nullptr, p.wait_ns);
+    for (int i = nv > SB ? nv - SB : 0; i < nv; ++i) mbar_wait(&v_full[i % SB], (i / SB) & 1, nullptr, nullptr, p.wait_ns);
   } else if (warp == 1 && n > 0) {
     // -------------------- MMA issue (whole warp, one elected lane: see attn_dense.cu)
     constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
@@ -232,8 +259,8 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
     const uint64_t qd = k_major(sQ), dod = k_major(sDO), kd = k_major(sK), vd = k_major(sV), kmn = mn_major(sK);
     bool ok = wait_all(q_full, 0);
     auto issue_s = [&](int j) {
-      const int st = j % ST;
-      if (!(ok = ok && wait_all(&kv_full[st], j / ST))) return;
+      const int st = j % SA;
+      if (!(ok = ok && wait_all(&k_full[st], j / SA))) return;
       tc_fence_after();
       if (elect_one()) {
         mma_abt<D>(tmem + (j & 1) * 128, qd, kd + st * TS, idesc_s);
@@ -242,9 +269,13 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
       __syncwarp();
     };
     auto issue_dp = [&](int j) {
+      const int st = j % SB;
+      if (!(ok = ok && wait_all(&v_full[st], j / SB))) return;
+      tc_fence_after();
       if (elect_one()) {
-        mma_abt<D>(tmem + kDP, dod, vd + (j % ST) * TS, idesc_s);
+        mma_abt<D>(tmem + kDP, dod, vd + st * TS, idesc_s);
         tc_commit(dp_full);
+        tc_commit(&v_empty[st]);
       }
       __syncwarp();
     };
@@ -256,9 +287,10 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
       tc_fence_after();
       // dP's buffer is free (dS_j is written): step j+1 can go on
       if (j + 1 < n) issue_dp(j + 1);
+      if (!ok) break;
       if (elect_one()) {
-        mma_ab<D>(tmem + kDQ, tmem + (j & 1) * 128, kmn + (j % ST) * TS, idesc_dq, j == 0);
-        tc_commit(&kv_empty[j % ST]);
+        mma_ab<D>(tmem + kDQ, tmem + (j & 1) * 128, kmn + (j % SA) * TS, idesc_dq, j == 0);
+        tc_commit(&k_empty[j % SA]);
       }
       __syncwarp();
       // over dS_j, which dQ_j (issued before) has read
@@ -300,10 +332,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const uint64_t x = f32x2_fma(f32x2_pack(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc2, nl2);
-            float x0, x1;
-            f32x2_unpack(x, x0, x1);
-            pv[c * 32 + k] = ex2_approx(x0);
-            pv[c * 32 + k + 1] = ex2_approx(x1);
+            ex2_pair(x, (k & 2) != 0, pv[c * 32 + k], pv[c * 32 + k + 1]);
           }
         }
         if (!(ok = wait_all(dp_full, j))) break;
@@ -332,7 +361,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
         if (j == n - 1 && (len & 127)) {
           // K rows past the length: zero before dS K may start, for dS = 0 times
           // what lies there (S_j, the tile's other reader, is complete)
-          uint8_t* kt = sK + (j % ST) * C::TILE;
+          uint8_t* kt = sK + (j % SA) * C::TILE;
           for (int x = (len & 127) * 8 + (threadIdx.x - 128); x < 128 * 8; x += 256) {
 #pragma unroll
             for (int c = 0; c < C::NCHUNK; ++c)
@@ -369,18 +398,20 @@ template <int D, bool BF16>
 __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmDO,
                           const DBwdParams& p, uint8_t* smem, int item) {
   using C = DBwdCfg<D>;
-  constexpr int ST = C::STAGES;
+  constexpr int SA = C::SA, SB = C::SB;
   uint8_t* sK = smem;
   uint8_t* sV = sK + C::TILE;
-  uint8_t* sQ = sV + C::TILE;        // [ST]
-  uint8_t* sDO = sQ + ST * C::TILE;  // [ST]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sDO + ST * C::TILE);
+  uint8_t* sQ = sV + C::TILE;        // [SA]
+  uint8_t* sDO = sQ + SA * C::TILE;  // [SB]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sDO + SB * C::TILE);
   float* col_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + C::BAR_BYTES);  // [2][128]
   float* col_dlt = col_lse + 256;                                                                 // [2][128]
   uint64_t* kv_full = bars;
-  uint64_t* qd_full = bars + 1;         // [ST]
-  uint64_t* qd_empty = qd_full + ST;    // [ST] dK_i (the last reader) completed
-  uint64_t* s_full = qd_empty + ST;
+  uint64_t* q_full = bars + 1;          // [SA]
+  uint64_t* q_empty = q_full + SA;      // [SA] dK_i (its last reader) completed
+  uint64_t* do_full = q_empty + SA;     // [SB]
+  uint64_t* do_empty = do_full + SB;    // [SB] dV_i completed (dP_i was issued before)
+  uint64_t* s_full = do_empty + SB;
   uint64_t* dp_full = s_full + 1;
   uint64_t* p_ready = dp_full + 1;      // 8 elementwise warps wrote P^T
   uint64_t* ds_ready = p_ready + 1;     // 8 elementwise warps wrote dS^T
@@ -394,9 +425,13 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&qd_full[i], 1);
-      mbar_init(&qd_empty[i], 1);
+    for (int i = 0; i < SA; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < SB; ++i) {
+      mbar_init(&do_full[i], 1);
+      mbar_init(&do_empty[i], 1);
     }
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
@@ -427,18 +462,23 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
       tma_load_4d(sK + c * C::CHUNK, &tmK, kv_full, c * 64, t * 128, hk, b * p.kb_mul);
       tma_load_4d(sV + c * C::CHUNK, &tmV, kv_full, c * 64, t * 128, hk, b * p.vb_mul);
     }
-    int i = 0;
-    for (; i < n; ++i) {
-      const int st = i % ST, g = i / p.q_tiles, qt = i - g * p.q_tiles;
-      if (i >= ST && !wait(&qd_empty[st], i / ST - 1)) break;
-      mbar_arrive_expect_tx(&qd_full[st], 2 * C::TILE);
-      for (int c = 0; c < C::NCHUNK; ++c) {
-        tma_load_4d(sQ + st * C::TILE + c * C::CHUNK, &tmQ, &qd_full[st], c * 64, qt * 128, hk * p.G + g, b * p.qb_mul);
-        tma_load_4d(sDO + st * C::TILE + c * C::CHUNK, &tmDO, &qd_full[st], c * 64, qt * 128, hk * p.G + g, b * p.db_mul);
-      }
+    int nq = 0, nd = 0;  // loads issued
+    for (int i = 0; i < n; ++i) {
+      const int a = i % SA, o = i % SB, g = i / p.q_tiles, qt = i - g * p.q_tiles;
+      if (i >= SA && !wait(&q_empty[a], i / SA - 1)) break;
+      mbar_arrive_expect_tx(&q_full[a], C::TILE);
+      for (int c = 0; c < C::NCHUNK; ++c)
+        tma_load_4d(sQ + a * C::TILE + c * C::CHUNK, &tmQ, &q_full[a], c * 64, qt * 128, hk * p.G + g, b * p.qb_mul);
+      ++nq;
+      if (i >= SB && !wait(&do_empty[o], i / SB - 1)) break;
+      mbar_arrive_expect_tx(&do_full[o], C::TILE);
+      for (int c = 0; c < C::NCHUNK; ++c)
+        tma_load_4d(sDO + o * C::TILE + c * C::CHUNK, &tmDO, &do_full[o], c * 64, qt * 128, hk * p.G + g, b * p.db_mul);
+      ++nd;
     }
     mbar_wait(kv_full, 0, nullptr, nullptr, p.wait_ns);
-    for (int k = i > ST ? i - ST : 0; k < i; ++k) mbar_wait(&qd_full[k % ST], (k / ST) & 1, nullptr, nullptr, p.wait_ns);
+    for (int k = nq > SA ? nq - SA : 0; k < nq; ++k) mbar_wait(&q_full[k % SA], (k / SA) & 1, nullptr, nullptr, p.wait_ns);
+    for (int k = nd > SB ? nd - SB : 0; k < nd; ++k) mbar_wait(&do_full[k % SB], (k / SB) & 1, nullptr, nullptr, p.wait_ns);
   } else if (warp == 1 && n > 0) {
     // -------------------- MMA issue (whole warp, one elected lane: see attn_dense.cu)
     constexpr uint32_t idesc_s = make_idesc_f16(BF16, 128, 128, false, false);
@@ -448,17 +488,19 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     const uint64_t qmn = mn_major(sQ), domn = mn_major(sDO);
     bool ok = wait_all(kv_full, 0);
     auto issue_s = [&](int i) {
-      if (!(ok = ok && wait_all(&qd_full[i % ST], i / ST))) return;
+      if (!(ok = ok && wait_all(&q_full[i % SA], i / SA))) return;
       tc_fence_after();
       if (elect_one()) {
-        mma_abt<D>(tmem, kd, qd + (i % ST) * TS, idesc_s);
+        mma_abt<D>(tmem, kd, qd + (i % SA) * TS, idesc_s);
         tc_commit(s_full);
       }
       __syncwarp();
     };
     auto issue_dp = [&](int i) {
+      if (!(ok = ok && wait_all(&do_full[i % SB], i / SB))) return;
+      tc_fence_after();
       if (elect_one()) {
-        mma_abt<D>(tmem + 128, vd, dod + (i % ST) * TS, idesc_s);
+        mma_abt<D>(tmem + 128, vd, dod + (i % SB) * TS, idesc_s);
         tc_commit(dp_full);
       }
       __syncwarp();
@@ -468,14 +510,17 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     for (int i = 0; ok && i < n; ++i) {
       if (!(ok = wait_all(p_ready, i))) break;
       tc_fence_after();
-      if (elect_one()) mma_ab<D>(tmem + 256, tmem, domn + (i % ST) * TS, idesc_acc, i == 0);
+      if (elect_one()) {
+        mma_ab<D>(tmem + 256, tmem, domn + (i % SB) * TS, idesc_acc, i == 0);
+        tc_commit(&do_empty[i % SB]);
+      }
       __syncwarp();
       if (i + 1 < n) issue_s(i + 1);  // over P_i^T, which dV_i has read
       if (!(ok = ok && wait_all(ds_ready, i))) break;
       tc_fence_after();
       if (elect_one()) {
-        mma_ab<D>(tmem + 256 + D, tmem + 128, qmn + (i % ST) * TS, idesc_acc, i == 0);
-        tc_commit(&qd_empty[i % ST]);
+        mma_ab<D>(tmem + 256 + D, tmem + 128, qmn + (i % SA) * TS, idesc_acc, i == 0);
+        tc_commit(&q_empty[i % SA]);
       }
       __syncwarp();
       if (i + 1 < n) issue_dp(i + 1);  // over dS_i^T
@@ -532,10 +577,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
             const float2 nl = *reinterpret_cast<const float2*>(lb + c * 32 + k);
             const uint64_t x =
                 f32x2_fma(f32x2_pack(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc2, f32x2_pack(nl.x, nl.y));
-            float x0, x1;
-            f32x2_unpack(x, x0, x1);
-            pv[c * 32 + k] = ex2_approx(x0);
-            pv[c * 32 + k + 1] = ex2_approx(x1);
+            ex2_pair(x, (k & 2) != 0, pv[c * 32 + k], pv[c * 32 + k + 1]);
             pt[k / 2] = pack2<BF16>(pv[c * 32 + k], pv[c * 32 + k + 1]);
           }
           tmem_st16(lane_base + half * 64 + c * 16, pt);
