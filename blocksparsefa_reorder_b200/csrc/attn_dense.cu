@@ -587,6 +587,26 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       const DensePart& pt = p.part[it.part];
       const int nst = it.nk == 0 ? 0 : (steps_of(it, 1) > 0 ? 2 : 1);  // streams with an O
       const int passes = it.dual ? 1 : it.nsub;
+      // this thread's rows' places in the result or in the partial results (null:
+      // no such row) and their lse's, found while the item is computed
+      auto place = [&](int ps, uint8_t*& dst, float*& dst_lse) {
+        int sq, g, mm;
+        const bool in = row_of(p, pt, it.sub0 + ps, row, sq, g, mm);
+        const int b = pt.shared_kv ? sq : it.b, h = it.hk * p.G + g;
+        const int64_t slot =
+            (static_cast<int64_t>(it.unit) * pt.rows + (static_cast<int64_t>(sq) * p.G + g) * p.M + mm) * pt.splits + it.split;
+        dst = !in          ? nullptr
+              : pt.part_o ? reinterpret_cast<uint8_t*>(pt.part_o + slot * D)
+                          : p.o + 2 * (b * p.os_b + h * p.os_h + mm * p.os_n);
+        dst_lse = !in          ? nullptr
+                  : pt.part_o ? pt.part_lse + slot
+                  : p.lse     ? p.lse + (static_cast<int64_t>(b) * p.H + h) * p.M + mm
+                              : nullptr;
+      };
+      uint8_t *dst0, *dst1 = nullptr;
+      float *lse0, *lse1 = nullptr;
+      place(0, dst0, lse0);
+      if (passes > 1) place(1, dst1, lse1);
       for (int ps = 0; ps < passes; ++ps) {
         // streams whose O make up this pass's rows: [first, last)
         const int first = it.dual ? 0 : ps, last = it.nk == 0 ? first : (it.dual ? nst : ps + 1);
@@ -603,8 +623,6 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           ++ni[s];
         }
         if (ok) tc_fence_after();
-        int sq, g, mm;
-        const bool store = row_of(p, pt, it.sub0 + ps, row, sq, g, mm) && ok;
         // weights of the streams' sums: 2^(m_s - max) / l, 0 for a stream without any key
         const float mx = fmaxf(l[0] > 0.f ? m[0] : -INFINITY, l[1] > 0.f ? m[1] : -INFINITY);
         float f0 = l[0] > 0.f ? ex2_approx(m[0] - mx) : 0.f;
@@ -616,13 +634,9 @@ __global__ void __launch_bounds__(kThreadsD, 1)
         f0 *= inv;
         f1 *= inv;
         const float lse = nan ? NAN : (lt > 0.f ? mx + log2f(lt) : -INFINITY);
-        // a row's place in the result, or in the partial results
-        const int b = pt.shared_kv ? sq : it.b, h = it.hk * p.G + g;
-        const int64_t slot =
-            (static_cast<int64_t>(it.unit) * pt.rows + (static_cast<int64_t>(sq) * p.G + g) * p.M + mm) * pt.splits + it.split;
-        uint8_t* const mine = !store ? nullptr
-                              : pt.part_o ? reinterpret_cast<uint8_t*>(pt.part_o + slot * D)
-                                          : p.o + 2 * (b * p.os_b + h * p.os_h + mm * p.os_n);
+        uint8_t* const mine = ok ? (ps ? dst1 : dst0) : nullptr;
+        float* const mine_lse = ps ? lse1 : lse0;
+        if (ok && mine_lse) *mine_lse = lse;
         const bool have = it.nk > 0;
         if (have || !pt.part_o) {  // (a partial result without keys is only its lse)
 #pragma unroll 1
@@ -681,12 +695,6 @@ __global__ void __launch_bounds__(kThreadsD, 1)
               }
             }
           }
-        }
-        if (store) {
-          if (pt.part_o)
-            pt.part_lse[slot] = lse;
-          else if (p.lse)
-            p.lse[(static_cast<int64_t>(b) * p.H + h) * p.M + mm] = lse;
         }
       }
     }
@@ -1071,7 +1079,7 @@ int launch_all(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_
   j.lse = c.lse;
   const int64_t rows = static_cast<int64_t>(c.B) * c.H * c.M;
   cudaLaunchAttribute attr[1];
-  if (rows <= 8 * kSMs) {
+  if (pl.s[0].splits + (c.n > 1 ? pl.s[1].splits : 0) >= 8) {
     const cudaLaunchConfig_t cfg = config(static_cast<unsigned>(rows), 256, 0, st, attr);
     BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16, 8>, j));
   } else {
