@@ -980,7 +980,7 @@ cudaLaunchConfig_t config(unsigned grid, int threads, int smem, cudaStream_t st,
 float* part_o(const Source& s, uint8_t* ws) { return reinterpret_cast<float*>(ws + s.o_off); }
 float* part_lse(const Source& s, uint8_t* ws) { return reinterpret_cast<float*>(ws + s.lse_off); }
 
-int launch_few(const DenseCall& c, const DensePlan& pl, int i, uint8_t* ws, cudaStream_t st) {
+int launch_few(const DenseCall& c, const DensePlan& pl, int i, bool late, uint8_t* ws, cudaStream_t st) {
   const Source& s = pl.s[i];
   FewParams p{};
   p.units = s.units, p.rows = s.rows, p.splits = s.splits, p.chunk = s.chunk, p.keys = c.keys[i];
@@ -998,6 +998,7 @@ int launch_few(const DenseCall& c, const DensePlan& pl, int i, uint8_t* ws, cuda
   p.lse = c.lse;
   if (pl.join) p.part_o = part_o(s, ws), p.part_lse = part_lse(s, ws);
   p.scale_log2 = c.sm_scale * 1.4426950408889634f;
+  p.late = late;
   p.err = c.err;
   return launch_attn_few(p, c.D, c.dtype == BSA_DTYPE_BF16, st);
 }
@@ -1062,8 +1063,12 @@ int launch_all(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_
   bool dense = false;
   for (int i = 0; i < c.n; ++i) dense = dense || !pl.s[i].few;
   if (dense && (r = launch_dense<D, BF16>(c, pl, ws, st))) return r;
-  for (int i = 0; i < c.n; ++i)
-    if (pl.s[i].few && (r = launch_few(c, pl, i, ws, st))) return r;
+  bool late = dense;
+  for (int i = 0; i < c.n; ++i) {
+    if (!pl.s[i].few) continue;
+    if ((r = launch_few(c, pl, i, late, ws, st))) return r;
+    late = true;
+  }
   if (!pl.join) return BSA_OK;
   JoinParams j{};  // (an absent second source has no partial results)
   for (int i = 0; i < c.n; ++i) {

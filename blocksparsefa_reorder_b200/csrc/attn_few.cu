@@ -78,7 +78,11 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
   float* sm_l = sm_m + kWarpsF * ROWS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int unit = blockIdx.x / p.splits, split = blockIdx.x - unit * p.splits;
-  grid_dependency_wait();
+  // Behind the kernel of the call's other source there is nothing to wait for
+  // (that kernel waited for what the inputs need before it let this one start),
+  // but the end of this grid has to mean the end of both for the join, so it
+  // waits last.
+  if (!p.late) grid_dependency_wait();
   allow_dependents();
   const int b = p.shared_kv ? 0 : unit / p.Hk, hk = p.shared_kv ? unit : unit - b * p.Hk;
   int len = p.keys;
@@ -291,6 +295,7 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
       if (col == 0 && p.lse) p.lse[(static_cast<int64_t>(rb) * p.H + rh) * p.M + rm] = lse;
     }
   }
+  if (p.late) grid_dependency_wait();
 }
 
 template <int D, bool BF16, int NR>

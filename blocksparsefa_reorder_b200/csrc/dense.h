@@ -33,6 +33,7 @@ struct FewParams {
   float* part_o;  // partial results, or null: this is the whole result
   float* part_lse;
   float scale_log2;
+  int late;       // launched behind the other source's kernel of the same call: see attn_few.cu
   int32_t* err;
 };
 int launch_attn_few(const FewParams& p, int D, bool bf16, cudaStream_t st);
