@@ -35,7 +35,9 @@ constexpr int kThreadsB = 384;
 
 struct DBwdParams {
   int B, H, Hk, G, M, N;
-  int q_tiles, k_tiles;
+  // A query tile holds mt tokens of gh heads of a group (a divisor of G), the
+  // tokens fastest: nm along the tokens, q_tiles in all for a key / value head.
+  int mt, gh, nm, q_tiles, k_tiles;
   int qb_mul, kb_mul, vb_mul, db_mul;  // 0: the tensor's batch stride is 0
   const void* lens;
   int lens_i64;
@@ -69,6 +71,15 @@ __device__ __forceinline__ int bwd_len(const DBwdParams& p, int b) {
                                : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.lens) + b));
   if (l < 0 || l > p.N) set_err(p.err, BSA_DEVERR_COORD);
   return static_cast<int>(l < 0 ? 0 : l > p.N ? p.N : l);
+}
+
+// Row `rl` of query tile t of a group: its head of the group and token; false
+// where the tile has no such row.
+__device__ __forceinline__ bool query_of(const DBwdParams& p, int t, int rl, int& g, int& m) {
+  const int gi = t / p.nm, q = rl / p.mt;
+  m = (t - gi * p.nm) * p.mt + rl - q * p.mt;
+  g = gi * p.gh + q;
+  return q < p.gh && m < p.M;
 }
 
 // -lse as the exponent's offset; a row without any weight (lse -inf) and a row
@@ -166,7 +177,7 @@ __device__ __forceinline__ uint64_t k_major(const void* t) { return make_sw128_d
 __device__ __forceinline__ uint64_t mn_major(const void* t) { return make_sw128_desc(smem_u32(t), 128 * 128, 1024); }
 
 // ---------------------------------------------------------------------------
-// dQ: one CTA per 128 query rows of one head, over the key tiles.
+// dQ: one CTA per query tile, over the key tiles.
 // TMEM: S_j / dS_j [128 (j & 1), +128), dP [256, 384), dQ [384, 384 + D).
 // ---------------------------------------------------------------------------
 template <int D, bool BF16>
@@ -193,7 +204,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int bh = item / p.q_tiles, t = item - bh * p.q_tiles;
-  const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -229,10 +240,11 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
 
   if (warp == 0 && lane == 0 && n > 0) {
     // ------------------------------------------------------------- producer
-    mbar_arrive_expect_tx(q_full, 2 * C::TILE);
+    mbar_arrive_expect_tx(q_full, 2 * C::NCHUNK * p.mt * p.gh * 128);
+    const int gi = t / p.nm, m0 = (t - gi * p.nm) * p.mt, h0 = hk * p.G + gi * p.gh;
     for (int c = 0; c < C::NCHUNK; ++c) {
-      tma_load_4d(sQ + c * C::CHUNK, &tmQ, q_full, c * 64, t * 128, h, b * p.qb_mul);
-      tma_load_4d(sDO + c * C::CHUNK, &tmDO, q_full, c * 64, t * 128, h, b * p.db_mul);
+      tma_load_4d(sQ + c * C::CHUNK, &tmQ, q_full, c * 64, m0, h0, b * p.qb_mul);
+      tma_load_4d(sDO + c * C::CHUNK, &tmDO, q_full, c * 64, m0, h0, b * p.db_mul);
     }
     int nk = 0, nv = 0;  // loads issued
     for (int j = 0; j < n; ++j) {
@@ -306,13 +318,14 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
     const int q4 = warp & 3, half = (warp - 4) >> 2;
     const int row = q4 * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
-    const int grow = t * 128 + row;
-    const bool live = grow < p.M;
-    uint8_t* orow = p.dq + 2 * (b * p.dq_b + h * p.dq_h + static_cast<int64_t>(grow) * p.dq_n);
+    int g, m;
+    const bool live = query_of(p, t, row, g, m);
+    const int h = hk * p.G + g;
+    uint8_t* orow = p.dq + 2 * (b * p.dq_b + h * p.dq_h + static_cast<int64_t>(m) * p.dq_n);
     if (n == 0) {
       if (live) zero_half_row<D>(half, orow);
     } else {
-      const int64_t ri = (static_cast<int64_t>(b) * p.H + h) * p.M + grow;
+      const int64_t ri = (static_cast<int64_t>(b) * p.H + h) * p.M + m;
       const float neg_lse = neg_lse_of(p, live, ri);
       const float dlt = live ? __ldg(&p.delta[ri]) : 0.f;
       const uint64_t sc2 = f32x2_pack(p.scale_log2, p.scale_log2), nl2 = f32x2_pack(neg_lse, neg_lse);
@@ -423,6 +436,13 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
   const int bh = item / p.k_tiles, t = item - bh * p.k_tiles;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
 
+  // Rows of a tile that no load fills: zero in every stage, so that their P = 0
+  // and dS = 0 meet finite values in the sums over the queries.
+  for (int x = p.mt * p.gh * 8 + threadIdx.x; x < 128 * 8; x += kThreadsB)
+    for (int st = 0; st < SA + SB; ++st)
+      for (int c = 0; c < C::NCHUNK; ++c)
+        *reinterpret_cast<uint4*>(sQ + st * C::TILE + c * C::CHUNK + x * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < SA; ++i) {
@@ -451,7 +471,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
   const int len = bwd_len(p, b);
-  const int n = t * 128 < len ? p.G * p.q_tiles : 0;  // steps: query tiles of all heads of the group
+  const int n = t * 128 < len ? p.q_tiles : 0;  // steps: query tiles of the whole group
   auto wait = [&](uint64_t* bar, int k) { return mbar_wait(bar, k & 1, abort_flag, p.err, p.wait_ns); };
   auto wait_all = [&](uint64_t* bar, int k) { return __all_sync(0xffffffffu, wait(bar, k)) != 0; };
 
@@ -464,16 +484,18 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     }
     int nq = 0, nd = 0;  // loads issued
     for (int i = 0; i < n; ++i) {
-      const int a = i % SA, o = i % SB, g = i / p.q_tiles, qt = i - g * p.q_tiles;
+      const int a = i % SA, o = i % SB;
+      const int gi = i / p.nm, m0 = (i - gi * p.nm) * p.mt, h0 = hk * p.G + gi * p.gh;
+      const int bytes = C::NCHUNK * p.mt * p.gh * 128;
       if (i >= SA && !wait(&q_empty[a], i / SA - 1)) break;
-      mbar_arrive_expect_tx(&q_full[a], C::TILE);
+      mbar_arrive_expect_tx(&q_full[a], bytes);
       for (int c = 0; c < C::NCHUNK; ++c)
-        tma_load_4d(sQ + a * C::TILE + c * C::CHUNK, &tmQ, &q_full[a], c * 64, qt * 128, hk * p.G + g, b * p.qb_mul);
+        tma_load_4d(sQ + a * C::TILE + c * C::CHUNK, &tmQ, &q_full[a], c * 64, m0, h0, b * p.qb_mul);
       ++nq;
       if (i >= SB && !wait(&do_empty[o], i / SB - 1)) break;
-      mbar_arrive_expect_tx(&do_full[o], C::TILE);
+      mbar_arrive_expect_tx(&do_full[o], bytes);
       for (int c = 0; c < C::NCHUNK; ++c)
-        tma_load_4d(sDO + o * C::TILE + c * C::CHUNK, &tmDO, &do_full[o], c * 64, qt * 128, hk * p.G + g, b * p.db_mul);
+        tma_load_4d(sDO + o * C::TILE + c * C::CHUNK, &tmDO, &do_full[o], c * 64, m0, h0, b * p.db_mul);
       ++nd;
     }
     mbar_wait(kv_full, 0, nullptr, nullptr, p.wait_ns);
@@ -549,9 +571,9 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
       // the first warpgroup stages -lse, the second -Delta, of the step's 128
       // query rows; the value of the next step is fetched a step ahead
       auto fetch = [&](int i) -> float {
-        const int g = i / p.q_tiles, qrow = (i - g * p.q_tiles) * 128 + row;
-        const int64_t at = (static_cast<int64_t>(b) * p.H + hk * p.G + g) * p.M + qrow;
-        const bool in = i < n && qrow < p.M;
+        int g, m;
+        const bool in = query_of(p, i, row, g, m);
+        const int64_t at = (static_cast<int64_t>(b) * p.H + hk * p.G + g) * p.M + m;
         return half == 0 ? neg_lse_of(p, in, at) : (in ? -__ldg(&p.delta[at]) : 0.f);
       };
       float next = fetch(0);
@@ -646,13 +668,13 @@ __global__ void __launch_bounds__(kThreadsB, 1)
     dq_tile<D, BF16>(tmQ, tmK, tmV, tmDO, p, smem, item - kv_items);
 }
 
-int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul) {
+int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul, int rows = 128, int heads = 1) {
   const bool one = B == 1 || t.stride_b == 0;
   *mul = one ? 0 : 1;
   if (one) t.stride_b = 8;
   if (H == 1) t.stride_h = 8;
   if (N == 1) t.stride_n = 8;
-  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, 128);
+  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, rows, heads);
 }
 
 template <int D, bool BF16>
@@ -670,15 +692,26 @@ int launch_t(const bsa_cross_bwd_args* a, cudaStream_t st) {
   DBwdParams p{};
   CUtensorMap mq, mk{}, mv{}, mdo;
   int r;
-  if ((r = map_of(&mq, a->q, a->B, a->H, a->M, D, BF16, &p.qb_mul))) return r;
-  if ((r = map_of(&mdo, a->dout, a->B, a->H, a->M, D, BF16, &p.db_mul))) return r;
+  // The tile shape with the fewest query tiles (8 tokens of 8 heads in one tile
+  // instead of eight): the tokens in equal parts, then heads that divide a group.
+  const int G = a->H / a->Hk;
+  p.q_tiles = INT32_MAX;
+  for (int parts = (a->M + 127) / 128, tries = 0; tries < 8 && parts <= a->M; ++parts, ++tries) {
+    const int mt = a->M >= 128 && tries == 0 ? 128 : (a->M + parts - 1) / parts;
+    int gh = 128 / mt < G ? 128 / mt : G;
+    while (G % gh) --gh;
+    const int nm = (a->M + mt - 1) / mt;
+    if (static_cast<int64_t>(nm) * (G / gh) >= p.q_tiles) continue;
+    p.mt = mt, p.gh = gh, p.nm = nm, p.q_tiles = nm * (G / gh);
+  }
+  if ((r = map_of(&mq, a->q, a->B, a->H, a->M, D, BF16, &p.qb_mul, p.mt, p.gh))) return r;
+  if ((r = map_of(&mdo, a->dout, a->B, a->H, a->M, D, BF16, &p.db_mul, p.mt, p.gh))) return r;
   if (a->N > 0) {
     if ((r = map_of(&mk, a->k, a->B, a->Hk, a->N, D, BF16, &p.kb_mul))) return r;
     if ((r = map_of(&mv, a->v, a->B, a->Hk, a->N, D, BF16, &p.vb_mul))) return r;
   }
   if ((r = launch_bwd_delta(a->o, a->dout, a->delta, a->B, a->H, a->M, D, BF16, st))) return r;
-  p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.G = a->H / a->Hk, p.M = a->M, p.N = a->N;
-  p.q_tiles = (a->M + 127) / 128;
+  p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.G = G, p.M = a->M, p.N = a->N;
   p.k_tiles = (a->N + 127) / 128;
   p.lens = a->k_lens;
   p.lens_i64 = a->lens_dtype == BSA_INDEX_I64;
@@ -692,7 +725,7 @@ int launch_t(const bsa_cross_bwd_args* a, cudaStream_t st) {
   p.err = a->err_flag;
   p.wait_ns = kWaitNs;
   const int64_t items =
-      static_cast<int64_t>(p.B) * p.Hk * p.k_tiles + static_cast<int64_t>(p.B) * p.H * p.q_tiles;
+      static_cast<int64_t>(p.B) * p.Hk * (static_cast<int64_t>(p.k_tiles) + p.q_tiles);
   if (items > INT32_MAX) return BSA_ERR_UNSUPPORTED;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

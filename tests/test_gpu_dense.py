@@ -224,7 +224,8 @@ def _grads_ref(q, k, v, do, lens, scale):
 BWD = [
     (1, 1, 1, 1, 1, None), (2, 4, 2, 5, 130, [130, 1]), (3, 6, 2, 129, 257, [0, 128, 200]),
     (1, 4, 1, 300, 1000, [999]), (2, 2, 2, 256, 128, None), (2, 6, 3, 257, 385, [385, 384]),
-    (1, 8, 2, 640, 64, [33]), (1, 2, 2, 1000, 1531, None),
+    (1, 8, 2, 640, 64, [33]), (1, 2, 2, 1000, 1531, None), (2, 12, 1, 3, 200, [200, 7]), (1, 12, 2, 40, 300, None),
+    (2, 8, 1, 65, 150, [150, 129]), (1, 5, 1, 129, 130, None),
 ]
 
 
