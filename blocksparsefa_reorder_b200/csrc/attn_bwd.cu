@@ -104,8 +104,9 @@ __device__ __forceinline__ void zero_row(uint8_t* row) {
 
 // Delta[b, h, n] = sum_d dO[n, d] * O[n, d] in fp32: each row read by D / 8
 // lanes with 16-byte loads (two rows per warp at D = 128, four at D = 64).
+// `rest` (optional, laid out as O) holds what O's rounding left.
 template <bool BF16, int D>
-__global__ void __launch_bounds__(256) bwd_delta_kernel(const uint8_t* o, int64_t o_b, int64_t o_h, int64_t o_n,
+__global__ void __launch_bounds__(256) bwd_delta_kernel(const uint8_t* o, const uint8_t* rest, int64_t o_b, int64_t o_h, int64_t o_n,
                                                         const uint8_t* dout, int64_t d_b, int64_t d_h, int64_t d_n,
                                                         float* delta, int B, int H, int N) {
   constexpr int LPR = D / 8;  // lanes per row
@@ -116,19 +117,20 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const uint8_t* o, int64_
   if (live) {
     const int64_t bh = r / N, n = r - bh * N, b = bh / H, h = bh - b * H;
     const int d = (lane % LPR) * 8;
-    const uint4 ov = *reinterpret_cast<const uint4*>(o + 2 * (b * o_b + h * o_h + n * o_n + d));
+    const int64_t at = 2 * (b * o_b + h * o_h + n * o_n + d);
+    const uint4 ov = *reinterpret_cast<const uint4*>(o + at);
     const uint4 dv = *reinterpret_cast<const uint4*>(dout + 2 * (b * d_b + h * d_h + n * d_n + d));
-    const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, dw[4] = {dv.x, dv.y, dv.z, dv.w};
+    const uint4 rv = rest ? *reinterpret_cast<const uint4*>(rest + at) : make_uint4(0, 0, 0, 0);
+    const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, dw[4] = {dv.x, dv.y, dv.z, dv.w}, rw[4] = {rv.x, rv.y, rv.z, rv.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       float o0, o1, d0, d1;
-      if constexpr (BF16) {
-        o0 = __uint_as_float(ow[k] << 16), o1 = __uint_as_float(ow[k] & 0xFFFF0000u);
-        d0 = __uint_as_float(dw[k] << 16), d1 = __uint_as_float(dw[k] & 0xFFFF0000u);
-      } else {
-        const __half2 oh = *reinterpret_cast<const __half2*>(&ow[k]);
-        const __half2 dh = *reinterpret_cast<const __half2*>(&dw[k]);
-        o0 = __low2float(oh), o1 = __high2float(oh), d0 = __low2float(dh), d1 = __high2float(dh);
+      unpack2<BF16>(ow[k], o0, o1);
+      unpack2<BF16>(dw[k], d0, d1);
+      if (rest) {
+        float r0, r1;
+        unpack2<BF16>(rw[k], r0, r1);
+        o0 += r0, o1 += r1;
       }
       acc = fmaf(o0, d0, fmaf(o1, d1, acc));
     }
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
 }  // namespace
 
-int launch_bwd_delta(const bsa_tensor4d& o, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
+int launch_bwd_delta(const bsa_tensor4d& o, const void* rest, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
                      bool bf16, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(B) * H * N;
   const int64_t rows_per_block = 8 * (32 / (D / 8));
@@ -576,7 +578,7 @@ int launch_bwd_delta(const bsa_tensor4d& o, const bsa_tensor4d& dout, float* del
 #define BSA_DELTA_CASE(BF_, D_)                                                                                     \
   if (bf16 == BF_ && D == D_)                                                                                      \
     bwd_delta_kernel<BF_, D_><<<grid, 256, 0, st>>>(                                                               \
-        static_cast<const uint8_t*>(o.data), o.stride_b, o.stride_h, o.stride_n,                                   \
+        static_cast<const uint8_t*>(o.data), static_cast<const uint8_t*>(rest), o.stride_b, o.stride_h, o.stride_n, \
         static_cast<const uint8_t*>(dout.data), dout.stride_b, dout.stride_h, dout.stride_n, delta, B, H, N);
   BSA_DELTA_CASE(true, 128)
   BSA_DELTA_CASE(false, 128)
@@ -618,7 +620,7 @@ int launch_bwd_t(const bsa_bwd_args* a, cudaStream_t st) {
   if ((r = make_tensor_map_4d(&mv_s, a->v, a->B, a->H, a->N, D, BF16, BN))) return r;
   if ((r = make_tensor_map_4d(&mdo_s, a->dout, a->B, a->H, a->N, D, BF16, BN))) return r;
 
-  if ((r = launch_bwd_delta(a->o, a->dout, a->delta, a->B, a->H, a->N, D, BF16, st))) return r;
+  if ((r = launch_bwd_delta(a->o, nullptr, a->dout, a->delta, a->B, a->H, a->N, D, BF16, st))) return r;
 
   BwdParams p{};
   p.H = a->H;

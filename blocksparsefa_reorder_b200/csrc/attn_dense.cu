@@ -93,6 +93,7 @@ struct DenseParams {
   int B, H, Hk, G, M;
   int lens_i64;
   uint8_t* o;
+  uint8_t* o_rest;  // optional, laid out as o: what rounding left
   int64_t os_b, os_h, os_n;
   float* lse;
   float scale_log2;
@@ -678,20 +679,31 @@ __global__ void __launch_bounds__(kThreadsD, 1)
                 if (dst) *reinterpret_cast<uint4*>(dst + ch * 128 + (lane & 7) * 16) = x[k];
               }
             } else {
-              uint4 x[4];
+              // once for o and, where asked for, once for what its rounding left
+#pragma unroll 1
+              for (int turn = 0; turn < (p.o_rest ? 2 : 1); ++turn) {
+                const int64_t to = turn ? p.o_rest - p.o : 0;
+                uint4 x[4];
 #pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                x[g].x = pack2<BF16>(__uint_as_float(v[8 * g + 0]), __uint_as_float(v[8 * g + 1]));
-                x[g].y = pack2<BF16>(__uint_as_float(v[8 * g + 2]), __uint_as_float(v[8 * g + 3]));
-                x[g].z = pack2<BF16>(__uint_as_float(v[8 * g + 4]), __uint_as_float(v[8 * g + 5]));
-                x[g].w = pack2<BF16>(__uint_as_float(v[8 * g + 6]), __uint_as_float(v[8 * g + 7]));
-              }
-              transpose_pieces<4>(x);
+                for (int g = 0; g < 4; ++g) {
+                  uint32_t* y = reinterpret_cast<uint32_t*>(&x[g]);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int from = (lane & 28) + k;
-                uint8_t* dst = shfl_ptr(mine, from);
-                if (dst) *reinterpret_cast<uint4*>(dst + ch * 64 + (lane & 3) * 16) = x[k];
+                  for (int k = 0; k < 4; ++k) {
+                    float& lo = reinterpret_cast<float&>(v[8 * g + 2 * k]);
+                    float& hi = reinterpret_cast<float&>(v[8 * g + 2 * k + 1]);
+                    y[k] = pack2<BF16>(lo, hi);
+                    float a, b;
+                    unpack2<BF16>(y[k], a, b);
+                    lo -= a, hi -= b;
+                  }
+                }
+                transpose_pieces<4>(x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const int from = (lane & 28) + k;
+                  uint8_t* dst = shfl_ptr(mine, from);
+                  if (dst) *reinterpret_cast<uint4*>(dst + to + ch * 64 + (lane & 3) * 16) = x[k];
+                }
               }
             }
           }
@@ -723,6 +735,7 @@ struct JoinParams {
   JoinSrc src[2];
   int B, H, Hk, G, M;
   uint8_t* o;
+  uint8_t* o_rest;
   int64_t os_b, os_h, os_n;
   float* lse;
 };
@@ -798,12 +811,22 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const JoinParams p) {
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint8_t* dst = p.o + 2 * (b * p.os_b + h * p.os_h + m * p.os_n + lane * V);
-  if constexpr (V == 4)
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
+  const int64_t at = 2 * (b * p.os_b + h * p.os_h + m * p.os_n + lane * V);
+  uint32_t x[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) x[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  auto store = [&](uint8_t* dst) {
+    if constexpr (V == 4)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(x[0], x[1]);
+    else
+      *reinterpret_cast<uint32_t*>(dst) = x[0];
+  };
+  store(p.o + at);
+  if (p.o_rest) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) x[i] = pack2_rest<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv, x[i]);
+    store(p.o_rest + at);
+  }
   if (lane == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : mx + log2f(sum);
 }
 
@@ -825,6 +848,7 @@ struct DenseCall {
   int lens_dtype;
   float sm_scale;
   float* lse;
+  void* o_rest;
   int32_t* err;
 };
 
@@ -996,6 +1020,7 @@ int launch_few(const DenseCall& c, const DensePlan& pl, int i, bool late, uint8_
   p.o = static_cast<uint8_t*>(c.o.data);
   p.os_b = c.o.stride_b, p.os_h = c.o.stride_h, p.os_n = c.o.stride_n;
   p.lse = c.lse;
+  p.o_rest = static_cast<uint8_t*>(c.o_rest);
   if (pl.join) p.part_o = part_o(s, ws), p.part_lse = part_lse(s, ws);
   p.scale_log2 = c.sm_scale * 1.4426950408889634f;
   p.late = late;
@@ -1047,6 +1072,7 @@ int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStrea
   p.o = static_cast<uint8_t*>(c.o.data);
   p.os_b = c.o.stride_b, p.os_h = c.o.stride_h, p.os_n = c.o.stride_n;
   p.lse = c.lse;
+  p.o_rest = static_cast<uint8_t*>(c.o_rest);
   p.scale_log2 = c.sm_scale * 1.4426950408889634f;
   p.err = c.err;
   p.wait_ns = kWaitNs;
@@ -1082,6 +1108,7 @@ int launch_all(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_
   j.o = static_cast<uint8_t*>(c.o.data);
   j.os_b = c.o.stride_b, j.os_h = c.o.stride_h, j.os_n = c.o.stride_n;
   j.lse = c.lse;
+  j.o_rest = static_cast<uint8_t*>(c.o_rest);
   const int64_t rows = static_cast<int64_t>(c.B) * c.H * c.M;
   cudaLaunchAttribute attr[1];
   if (pl.s[0].splits + (c.n > 1 ? pl.s[1].splits : 0) >= 8) {
@@ -1107,6 +1134,7 @@ int validate(const DenseCall& c) {
   if (c.D != 64 && c.D != 128) return BSA_ERR_UNSUPPORTED;
   if (!(c.sm_scale > 0.f) || !(c.sm_scale < INFINITY)) return BSA_ERR_UNSUPPORTED;
   if (!c.q.data || !c.o.data) return BSA_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(c.o_rest) % 16) return BSA_ERR_ALIGNMENT;
   // row and item numbers are 32-bit
   if (static_cast<int64_t>(c.B) * c.H * c.M > INT32_MAX / 2) return BSA_ERR_UNSUPPORTED;
   if (!aligned(c.q, c.B, c.H, c.M) || !aligned(c.o, c.B, c.H, c.M)) return BSA_ERR_ALIGNMENT;
@@ -1133,7 +1161,7 @@ DenseCall call_of(const bsa_cross_args* a) {
   c.n = 1;
   c.k[0] = a->k, c.v[0] = a->v, c.keys[0] = a->N;
   c.lens[0] = a->k_lens, c.lens_dtype = a->lens_dtype;
-  c.sm_scale = a->sm_scale, c.lse = a->lse, c.err = a->err_flag;
+  c.sm_scale = a->sm_scale, c.lse = a->lse, c.o_rest = a->o_rest, c.err = a->err_flag;
   return c;
 }
 

@@ -710,7 +710,7 @@ int launch_t(const bsa_cross_bwd_args* a, cudaStream_t st) {
     if ((r = map_of(&mk, a->k, a->B, a->Hk, a->N, D, BF16, &p.kb_mul))) return r;
     if ((r = map_of(&mv, a->v, a->B, a->Hk, a->N, D, BF16, &p.vb_mul))) return r;
   }
-  if ((r = launch_bwd_delta(a->o, a->dout, a->delta, a->B, a->H, a->M, D, BF16, st))) return r;
+  if ((r = launch_bwd_delta(a->o, a->o_rest, a->dout, a->delta, a->B, a->H, a->M, D, BF16, st))) return r;
   p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.G = G, p.M = a->M, p.N = a->N;
   p.k_tiles = (a->N + 127) / 128;
   p.lens = a->k_lens;
@@ -756,6 +756,7 @@ int cross_bwd_validate(const bsa_cross_bwd_args* a) {
   if (a->D != 64 && a->D != 128) return BSA_ERR_UNSUPPORTED;
   if (!(a->sm_scale > 0.f) || !(a->sm_scale < INFINITY)) return BSA_ERR_UNSUPPORTED;
   if (!a->lse || !a->delta) return BSA_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(a->o_rest) % 16) return BSA_ERR_ALIGNMENT;
   if (static_cast<int64_t>(a->B) * a->H * a->M > INT32_MAX / 2 || a->N > INT32_MAX - 65536) return BSA_ERR_UNSUPPORTED;
   const bsa_tensor4d* qs[] = {&a->q, &a->o, &a->dout, &a->dq};
   const bsa_tensor4d* ks[] = {&a->k, &a->v, &a->dk, &a->dv};

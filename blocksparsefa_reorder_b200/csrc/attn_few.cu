@@ -291,7 +291,15 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
       x.y = pack2<BF16>(o[2] * inv, o[3] * inv);
       x.z = pack2<BF16>(o[4] * inv, o[5] * inv);
       x.w = pack2<BF16>(o[6] * inv, o[7] * inv);
-      *reinterpret_cast<uint4*>(p.o + 2 * (rb * p.os_b + rh * p.os_h + rm * p.os_n + col)) = x;
+      const int64_t at = 2 * (rb * p.os_b + rh * p.os_h + rm * p.os_n + col);
+      *reinterpret_cast<uint4*>(p.o + at) = x;
+      if (p.o_rest) {
+        x.x = pack2_rest<BF16>(o[0] * inv, o[1] * inv, x.x);
+        x.y = pack2_rest<BF16>(o[2] * inv, o[3] * inv, x.y);
+        x.z = pack2_rest<BF16>(o[4] * inv, o[5] * inv, x.z);
+        x.w = pack2_rest<BF16>(o[6] * inv, o[7] * inv, x.w);
+        *reinterpret_cast<uint4*>(p.o_rest + at) = x;
+      }
       if (col == 0 && p.lse) p.lse[(static_cast<int64_t>(rb) * p.H + rh) * p.M + rm] = lse;
     }
   }

@@ -356,13 +356,18 @@ void cross_shapes(const Tensor& q, const Tensor& k, const Tensor& v) {
 
 std::tuple<Tensor, OptTensor> cross_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& k_lens,
                                             const std::optional<double>& sm_scale, bool return_lse, const OptTensor& out,
-                                            const OptTensor& lse_out, const OptTensor& err) {
+                                            const OptTensor& lse_out, const OptTensor& o_rest, const OptTensor& err) {
   cross_shapes(q_, k_, v_);
   bsa_cross_args a{};
   a.lens_dtype = lens_dtype(k_lens, q_, "k_lens");
   a.sm_scale = scale_of(sm_scale, q_.size(3));
   const Tensor o = output(out, q_, "out");
   const OptTensor lse = lse_output(return_lse, lse_out, q_);
+  if (o_rest) {
+    output(o_rest, q_, "o_rest");
+    TORCH_CHECK_VALUE(o_rest->strides() == o.strides(), "o_rest must be laid out as the output");
+    a.o_rest = o_rest->data_ptr();
+  }
   if (q_.numel() == 0) return {o, lse};
   const Tensor q = spread(q_, true), k = spread(k_), v = spread(v_);
   a.B = dim(q.size(0), "B"), a.H = dim(q.size(1), "H"), a.Hk = dim(k.size(1), "Hk"), a.M = dim(q.size(2), "M");
@@ -377,7 +382,8 @@ std::tuple<Tensor, OptTensor> cross_forward(const Tensor& q_, const Tensor& k_, 
 
 std::tuple<Tensor, Tensor, Tensor> cross_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o_,
                                                   const Tensor& lse, const Tensor& dout_, const OptTensor& k_lens,
-                                                  const std::optional<double>& sm_scale, const OptTensor& err) {
+                                                  const std::optional<double>& sm_scale, const OptTensor& o_rest,
+                                                  const OptTensor& err) {
   cross_shapes(q_, k_, v_);
   like_q(o_, q_, "o");
   like_q(dout_, q_, "dout");
@@ -387,11 +393,17 @@ std::tuple<Tensor, Tensor, Tensor> cross_backward(const Tensor& q_, const Tensor
                         lse.device() == q_.device(),
                     "lse must be the forward's contiguous float32 [B, H, M] LSE");
   bsa_cross_bwd_args a{};
+  if (o_rest) {
+    output(o_rest, q_, "o_rest");
+    TORCH_CHECK_VALUE(o_rest->strides() == o_.strides(), "o_rest must be laid out as o");
+    a.o_rest = o_rest->data_ptr();
+  }
   a.lens_dtype = lens_dtype(k_lens, q_, "k_lens");
   a.sm_scale = scale_of(sm_scale, q_.size(3));
   Tensor dq = contiguous_like(q_), dk = contiguous_like(k_), dv = contiguous_like(v_);
   if (q_.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
-  const Tensor q = spread(q_, true), k = spread(k_), v = spread(v_), o = spread(o_, true), dout = spread(dout_, true);
+  const Tensor q = spread(q_, true), k = spread(k_), v = spread(v_), dout = spread(dout_, true);
+  const Tensor o = o_rest ? o_ : spread(o_, true);
   const Tensor delta = at::empty(lse.sizes(), lse.options());
   a.B = dim(q.size(0), "B"), a.H = dim(q.size(1), "H"), a.Hk = dim(k.size(1), "Hk"), a.M = dim(q.size(2), "M");
   a.N = dim(k.size(2), "N"), a.D = dim(q.size(3), "D"), a.dtype = dtype_of(q.scalar_type());
@@ -409,8 +421,9 @@ std::tuple<Tensor, Tensor, Tensor> cross_backward(const Tensor& q_, const Tensor
 struct CrossFn : torch::autograd::Function<CrossFn> {
   static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, const OptTensor& k_lens,
                         std::optional<double> sm_scale) {
-    auto [o, lse] = cross_forward(q, k, v, k_lens, sm_scale, true, {}, {}, {});
-    ctx->save_for_backward({q, k, v, o, *lse, or_none(k_lens)});
+    const Tensor rest = q.is_cuda() ? contiguous_like(q) : Tensor();
+    auto [o, lse] = cross_forward(q, k, v, k_lens, sm_scale, true, {}, {}, if_defined(rest), {});
+    ctx->save_for_backward({q, k, v, o, *lse, rest, or_none(k_lens)});
     ctx->saved_data["scale"] = sm_scale;
     return o;
   }
@@ -418,7 +431,7 @@ struct CrossFn : torch::autograd::Function<CrossFn> {
     once("cross_attention");
     const auto s = ctx->get_saved_variables();
     const auto scale = ctx->saved_data["scale"].toOptional<double>();
-    auto [dq, dk, dv] = cross_backward(s[0], s[1], s[2], s[3], s[4], rows(g[0]), if_defined(s[5]), scale, {});
+    auto [dq, dk, dv] = cross_backward(s[0], s[1], s[2], s[3], s[4], rows(g[0]), if_defined(s[6]), scale, if_defined(s[5]), {});
     return {dq, dk, dv, Tensor(), Tensor()};
   }
 };

@@ -49,6 +49,14 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
   }
 }
 
+// What packing two floats left of them, packed.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t packed) {
+  float a, b;
+  unpack2<BF16>(packed, a, b);
+  return pack2<BF16>(lo - a, hi - b);
+}
+
 __device__ __forceinline__ void set_err(int32_t* flag, int32_t bits) {
   if (flag) atomicOr(flag, bits);
 }

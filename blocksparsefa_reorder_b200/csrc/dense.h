@@ -29,6 +29,7 @@ struct FewParams {
   int64_t qs_b, qs_h, qs_n, ks_b, ks_h, ks_n, vs_b, vs_h, vs_n;
   uint8_t* o;
   int64_t os_b, os_h, os_n;
+  uint8_t* o_rest;  // optional, laid out as o: what rounding left
   float* lse;
   float* part_o;  // partial results, or null: this is the whole result
   float* part_lse;

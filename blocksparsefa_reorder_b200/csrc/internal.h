@@ -34,8 +34,9 @@ int launch_permute_rows(bsa_tensor4d dst, bsa_tensor4d src, int B, int H, int N,
 int launch_attn_simt(const bsa_fwd_args* a, cudaStream_t st);
 // The backward kernels (attn_bwd.cu): Delta, dQ, dK / dV; arguments validated.
 int launch_attn_bwd(const bsa_bwd_args* a, cudaStream_t st);
-// Delta = rowsum(dout o o) per query row, contiguous fp32 [B, H, N] (D 64 / 128).
-int launch_bwd_delta(const bsa_tensor4d& o, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
+// Delta = rowsum(dout o (o + rest)) per query row, contiguous fp32 [B, H, N] (D 64
+// / 128); rest (optional, laid out as o): what o's rounding left.
+int launch_bwd_delta(const bsa_tensor4d& o, const void* rest, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
                      bool bf16, cudaStream_t st);
 
 // tma_maps.cu: whether the tcgen05 path takes these arguments (bf16 / fp16,

@@ -30,7 +30,8 @@ def _error_word(check_errors: bool, q):
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, k_lens: Optional[torch.Tensor] = None,
                     sm_scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
-                    lse_out: Optional[torch.Tensor] = None, check_errors: bool = False):
+                    lse_out: Optional[torch.Tensor] = None, o_rest: Optional[torch.Tensor] = None,
+                    check_errors: bool = False):
     """Attention of M queries over N keys of another sequence.
 
     ``o = softmax(q k^T * sm_scale over keys j < k_lens[b]) v`` per (b, h).
@@ -44,25 +45,30 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, k_lens
     into the result, NaN included.  Lengths outside [0, N] are clamped, and an
     error with ``check_errors`` (which synchronises).
     return_lse: also return the row log-sum-exp in log2 units, ``[B, H, M]``.
+    o_rest: optional tensor laid out as the output that receives what rounding
+    left of the result (fp32 result - o), for :func:`cross_attention_backward`.
     """
     err = _error_word(check_errors, q)
-    o, lse = _lib.native().cross_attention(q, k, v, k_lens, sm_scale, return_lse, out, lse_out, err)
+    o, lse = _lib.native().cross_attention(q, k, v, k_lens, sm_scale, return_lse, out, lse_out, o_rest, err)
     _check_err(err, "cross_attention")
     return (o, lse) if return_lse else o
 
 
 def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                              dout: torch.Tensor, *, k_lens: Optional[torch.Tensor] = None,
-                             sm_scale: Optional[float] = None, check_errors: bool = False):
+                             sm_scale: Optional[float] = None, o_rest: Optional[torch.Tensor] = None,
+                             check_errors: bool = False):
     """Gradients of :func:`cross_attention`: ``dq, dk, dv`` for the output
     gradient ``dout``, from the forward's ``o`` and log2 ``lse``.
 
     dk and dv are summed over the query heads of each key / value head and are
     zero behind ``k_lens[b]``; every gradient row is written by one CTA (no
-    atomics, deterministic).
+    atomics, deterministic).  o_rest: the forward's, so that ``rowsum(dout o)``
+    is formed from the unrounded output; without it o's rounding is in dq and dk
+    (over few keys as much of it as their own).
     """
     err = _error_word(check_errors, q)
-    g = _lib.native().cross_attention_backward(q, k, v, o, lse, dout, k_lens, sm_scale, err)
+    g = _lib.native().cross_attention_backward(q, k, v, o, lse, dout, k_lens, sm_scale, o_rest, err)
     _check_err(err, "cross_attention_backward")
     return g
 

@@ -297,6 +297,8 @@ typedef struct bsa_cross_args {
   bsa_tensor4d q, o, k, v;
   const void* k_lens;       /* optional [B]                                        */
   float* lse;               /* optional contiguous [B, H, M], log2 units           */
+  void* o_rest;             /* optional, laid out as o: what rounding left of the
+                               result, fp32 result - o, in o's type                */
   int32_t* err_flag;
   float sm_scale;
 } bsa_cross_args;
@@ -315,6 +317,8 @@ typedef struct bsa_cross_bwd_args {
   bsa_tensor4d dq, dk, dv;  /* outputs                                             */
   const void* k_lens;       /* the forward's                                       */
   const float* lse;         /* the forward's contiguous [B, H, M]                  */
+  const void* o_rest;       /* the forward's, or NULL: Delta is formed from o +
+                               o_rest, so that o's rounding is not in dq and dk    */
   float* delta;
   int32_t* err_flag;
   float sm_scale;

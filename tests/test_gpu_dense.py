@@ -255,6 +255,26 @@ def test_cross_gradient_matches_formula(c, D, dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("M,N,G", [(3, 20, 2), (40, 20, 2), (40, 5000, 2), (200, 300, 1), (3, 9000, 1)])
+def test_cross_rounding_rest(M, N, G, dtype):
+    """o + o_rest is the result to twice the bits (rounding left u^2 |o|), whichever
+    kernel writes it, and the gradient holds its bound with it."""
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    q, do = _rand((2, 2 * G, M, 64), dtype, g), _rand((2, 2 * G, M, 64), dtype, g)
+    k, v = _rand((2, 2, N, 64), dtype, g), _rand((2, 2, N, 64), dtype, g)
+    rest = torch.full_like(q, math.nan)
+    o, lse = cross_attention(q, k, v, return_lse=True, o_rest=rest)
+    assert torch.equal(o, cross_attention(q, k, v))
+    ro, _, A, _ = _cross_ref(q, k, v, None, 1 / 8)
+    u = _u(dtype)
+    assert (rest.double().abs() <= u * o.double().abs() * 1.01 + 2.0 ** -24).all()
+    assert ((o.double() + rest.double() - ro).abs() <= (u + E) * A + 2 * u * u * ro.abs() + 2.0 ** -24).all()
+    got = cross_attention_backward(q, k, v, o, lse, do, o_rest=rest)
+    ref, bound = _grads_ref(q, k, v, do, None, 1 / 8)
+    assert all(((x.double() - r).abs() <= t).all() for x, r, t in zip(got, ref, bound))
+
+
 def test_cross_gradient_matches_differences():
     """Central differences of the 64-bit definition along random directions."""
     g = torch.Generator(device="cuda").manual_seed(8)
@@ -291,8 +311,9 @@ def test_cross_autograd_expanded_and_shared():
     ones = torch.ones_like(q)
     kd, vd = (t.detach().expand(B, -1, -1, -1).contiguous() for t in (k, v))
     with torch.no_grad():
-        ob, lb = cross_attention(q, kd, vd, k_lens=ln, return_lse=True)
-        dq, dk, dv = cross_attention_backward(q, kd, vd, ob, lb, ones, k_lens=ln)
+        rest = torch.empty_like(q)
+        ob, lb = cross_attention(q, kd, vd, k_lens=ln, return_lse=True, o_rest=rest)
+        dq, dk, dv = cross_attention_backward(q, kd, vd, ob, lb, ones, k_lens=ln, o_rest=rest)
     assert torch.equal(o, ob) and torch.equal(q.grad, dq)
     for got, parts in ((k.grad, dk), (v.grad, dv)):
         assert got.shape == (1, Hk, N, D)
