@@ -1,7 +1,7 @@
 """Command line with the reference's ``main.py`` interface (``main.py:102-167``).
 
     python -m blocksparsefa_reorder_b200 pattern.mtx [--block-size 128] [--head-dim 128]
-        [--num-heads 1] [--row-reorder rows.txt] [--col-reorder cols.txt] [--mode B200]
+        [--num-heads 1] [--row-reorder rows.txt] [--col-reorder cols.txt] [--mode B200] [--qk-norm-rope]
 
 Same positional pattern file, options, defaults and argument checks as the
 reference; ``--mode B200`` (the default here) runs this library: read the
@@ -46,6 +46,8 @@ def parse_args(argv: Optional[list] = None):
                    help="Optional input file for column reorderings (default: None).")
     p.add_argument("--mode", type=str, choices=["B200", *REFERENCE_MODES], default="B200",
                    help="Attention backend (default: B200, this library).")
+    p.add_argument("--qk-norm-rope", action="store_true",
+                   help="Also time the forward with the norm and rotation of q and k in front (B200 mode).")
     ns = p.parse_args(argv)
     if ns.matrix_mtx.suffix.lower() != ".mtx":
         p.error("Input matrix file must have .mtx extension.")
@@ -55,7 +57,7 @@ def parse_args(argv: Optional[list] = None):
     if ns.block_size not in (64, 128):
         p.error("--block-size must be 64 or 128 for the B200 kernels.")
     return Args(matrix_mtx=ns.matrix_mtx, block_size=ns.block_size, head_dim=ns.head_dim, num_heads=ns.num_heads,
-                row_reorder=ns.row_reorder, col_reorder=ns.col_reorder, mode=ns.mode)
+                row_reorder=ns.row_reorder, col_reorder=ns.col_reorder, mode=ns.mode, qk_norm_rope=ns.qk_norm_rope)
 
 
 def run_sparse_attention_reordering_test(args, device: str = "cuda:0") -> None:
@@ -71,7 +73,8 @@ def run_sparse_attention_reordering_test(args, device: str = "cuda:0") -> None:
     block_mask, seq_len = generate_blockmask_from_mtx_coords(
         rows_idx, cols_idx, seq_len, args.block_size, batch_size=1, nheads=args.num_heads, device=device,
         row_perm=row_perm, col_perm=col_perm)
-    run_experiments_B200(args, block_mask, seq_len, row_perm=row_perm, col_perm=col_perm, device=device)
+    run_experiments_B200(args, block_mask, seq_len, row_perm=row_perm, col_perm=col_perm, device=device,
+                         qk_norm_rope=args.qk_norm_rope)
 
 
 def main(argv: Optional[list] = None) -> int:

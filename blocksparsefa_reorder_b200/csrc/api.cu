@@ -298,8 +298,10 @@ extern "C" int bsa_cross_fwd_workspace_bytes(const bsa_cross_args* a, size_t* by
 extern "C" int bsa_cross_fwd(const bsa_cross_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = cross_validate(a);
   if (rc) return rc;
+  const size_t need = cross_workspace(a);
+  if (need && (!workspace || workspace_bytes < need)) return BSA_ERR_WORKSPACE;
   if ((rc = check_device())) return rc;
-  return launch_cross(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  return launch_cross(a, workspace, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int bsa_cross_bwd(const bsa_cross_bwd_args* a, void* stream) {
@@ -320,6 +322,8 @@ extern "C" int bsa_prefix_fwd_workspace_bytes(const bsa_prefix_args* a, size_t* 
 extern "C" int bsa_prefix_fwd(const bsa_prefix_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = prefix_validate(a);
   if (rc) return rc;
+  const size_t need = prefix_workspace(a);
+  if (need && (!workspace || workspace_bytes < need)) return BSA_ERR_WORKSPACE;
   if ((rc = check_device())) return rc;
-  return launch_prefix(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  return launch_prefix(a, workspace, static_cast<cudaStream_t>(stream));
 }

@@ -1177,10 +1177,10 @@ DenseCall call_of(const bsa_prefix_args* a) {
   return c;
 }
 
-int run(const DenseCall& c, void* ws, size_t bytes, cudaStream_t st) {
-  const DensePlan pl = plan_of(c);
-  if (pl.total && (!ws || bytes < pl.total)) return BSA_ERR_WORKSPACE;
+// (the caller checked that `ws` holds plan_of(c).total bytes)
+int run(const DenseCall& c, void* ws, cudaStream_t st) {
   if (reinterpret_cast<uintptr_t>(ws) % 16) return BSA_ERR_ALIGNMENT;
+  const DensePlan pl = plan_of(c);
   uint8_t* w = static_cast<uint8_t*>(ws);
   const bool bf = c.dtype == BSA_DTYPE_BF16;
   if (c.D == 128) return bf ? launch_all<128, true>(c, pl, w, st) : launch_all<128, false>(c, pl, w, st);
@@ -1191,13 +1191,9 @@ int run(const DenseCall& c, void* ws, size_t bytes, cudaStream_t st) {
 
 int cross_validate(const bsa_cross_args* a) { return a ? validate(call_of(a)) : BSA_ERR_INVALID_ARG; }
 size_t cross_workspace(const bsa_cross_args* a) { return plan_of(call_of(a)).total; }
-int launch_cross(const bsa_cross_args* a, void* ws, size_t bytes, cudaStream_t st) {
-  return run(call_of(a), ws, bytes, st);
-}
+int launch_cross(const bsa_cross_args* a, void* ws, cudaStream_t st) { return run(call_of(a), ws, st); }
 int prefix_validate(const bsa_prefix_args* a) { return a ? validate(call_of(a)) : BSA_ERR_INVALID_ARG; }
 size_t prefix_workspace(const bsa_prefix_args* a) { return plan_of(call_of(a)).total; }
-int launch_prefix(const bsa_prefix_args* a, void* ws, size_t bytes, cudaStream_t st) {
-  return run(call_of(a), ws, bytes, st);
-}
+int launch_prefix(const bsa_prefix_args* a, void* ws, cudaStream_t st) { return run(call_of(a), ws, st); }
 
 }  // namespace bsa

@@ -251,41 +251,45 @@ void once(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its gradient has none (create_graph)");
 }
 
+// Outputs and incoming gradients: those of q and k that are there, in that order.
 struct RopeFn : torch::autograd::Function<RopeFn> {
-  static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight,
-                               const OptTensor& positions, const OptTensor& cos, const OptTensor& sin, double eps,
-                               bool interleaved) {
-    const RopeIn in{if_defined(q), if_defined(k), if_defined(q_weight), if_defined(k_weight), positions, cos, sin, eps,
-                    interleaved};
-    auto [oq, ok] = rope_forward(in, {}, {}, {});
-    ctx->save_for_backward({q, k, q_weight, k_weight, or_none(positions), or_none(cos), or_none(sin)});
+  static variable_list forward(AutogradContext* ctx, const OptTensor& q, const OptTensor& k, const OptTensor& q_weight,
+                               const OptTensor& k_weight, const OptTensor& positions, const OptTensor& cos,
+                               const OptTensor& sin, double eps, bool interleaved) {
+    auto [oq, ok] = rope_forward({q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved}, {}, {}, {});
+    ctx->save_for_backward({or_none(q), or_none(k), or_none(q_weight), or_none(k_weight), or_none(positions), or_none(cos),
+                            or_none(sin)});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["interleaved"] = interleaved;
     ctx->set_materialize_grads(false);
-    return {or_none(oq), or_none(ok)};
+    variable_list out;
+    if (oq) out.push_back(*oq);
+    if (ok) out.push_back(*ok);
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     once("qk_norm_rope");
     const auto s = ctx->get_saved_variables();
-    const bool hq = g[0].defined(), hk = g[1].defined();
+    // a side that is absent, or whose output took no part, has no gradient
+    const Tensor gq = s[0].defined() ? g[0] : Tensor(), gk = s[1].defined() ? g[s[0].defined() ? 1 : 0] : Tensor();
+    const bool hq = gq.defined(), hk = gk.defined();
     variable_list out(9);
     if (!hq && !hk) return out;
-    // a side whose output took no part has no gradient
     RopeIn in{hq ? if_defined(s[0]) : OptTensor(), hk ? if_defined(s[1]) : OptTensor(),
               hq ? if_defined(s[2]) : OptTensor(), hk ? if_defined(s[3]) : OptTensor(), if_defined(s[4]),
               if_defined(s[5]), if_defined(s[6]), ctx->saved_data["eps"].toDouble(),
               ctx->saved_data["interleaved"].toBool()};
-    auto [dq, dk, dwq, dwk] = rope_backward(in, hq ? OptTensor(rows(g[0])) : OptTensor(),
-                                            hk ? OptTensor(rows(g[1])) : OptTensor(), {});
+    auto [dq, dk, dwq, dwk] =
+        rope_backward(in, hq ? OptTensor(rows(gq)) : OptTensor(), hk ? OptTensor(rows(gk)) : OptTensor(), {});
     out[0] = or_none(dq), out[1] = or_none(dk), out[2] = or_none(dwq), out[3] = or_none(dwk);
     return out;
   }
 };
 
 std::tuple<OptTensor, OptTensor> rope_autograd(const RopeIn& in) {
-  const auto o = RopeFn::apply(or_none(in.q), or_none(in.k), or_none(in.q_weight), or_none(in.k_weight), in.positions,
-                               in.cos, in.sin, in.eps, in.interleaved);
-  return {if_defined(o[0]), if_defined(o[1])};
+  TORCH_CHECK_VALUE(in.q || in.k, "pass q or k");
+  const auto o = RopeFn::apply(in.q, in.k, in.q_weight, in.k_weight, in.positions, in.cos, in.sin, in.eps, in.interleaved);
+  return {in.q ? OptTensor(o[0]) : OptTensor(), in.k ? OptTensor(o[in.q ? 1 : 0]) : OptTensor()};
 }
 
 // ---------------------------------------------------------------------------

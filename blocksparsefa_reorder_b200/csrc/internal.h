@@ -63,14 +63,14 @@ int launch_rope_fwd(const bsa_rope_args* a, cudaStream_t st);
 size_t rope_bwd_workspace(const bsa_rope_args* a);
 int launch_rope_bwd(const bsa_rope_args* a, void* workspace, size_t bytes, cudaStream_t st);
 
-// attn_dense.cu: attention over contiguous key ranges (arguments validated
-// by the caller with the *_validate functions).
+// attn_dense.cu: attention over contiguous key ranges (arguments and workspace
+// checked by the caller with the *_validate and *_workspace functions).
 int cross_validate(const bsa_cross_args* a);
 size_t cross_workspace(const bsa_cross_args* a);
-int launch_cross(const bsa_cross_args* a, void* workspace, size_t bytes, cudaStream_t st);
+int launch_cross(const bsa_cross_args* a, void* workspace, cudaStream_t st);
 int prefix_validate(const bsa_prefix_args* a);
 size_t prefix_workspace(const bsa_prefix_args* a);
-int launch_prefix(const bsa_prefix_args* a, void* workspace, size_t bytes, cudaStream_t st);
+int launch_prefix(const bsa_prefix_args* a, void* workspace, cudaStream_t st);
 // attn_dense_bwd.cu: gradient of cross attention
 int cross_bwd_validate(const bsa_cross_bwd_args* a);
 int launch_cross_bwd(const bsa_cross_bwd_args* a, cudaStream_t st);

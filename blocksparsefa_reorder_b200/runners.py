@@ -14,7 +14,9 @@ reference runners (e.g. ``BlockSparseTriton_Naive.py:10-18``): it draws
 after ``REPEATS_WARMUP`` warm-up calls, over ``REPEATS_TIMING`` calls, and
 prints the reference's two lines (``Average time with reordering: X ms`` /
 ``Average time without reordering: X ms``).  Times are taken with CUDA
-events on the current stream.  The reference names
+events on the current stream.  With ``qk_norm_rope`` (no counterpart in the
+reference) it also times the reordered forward with the norm and rotation of q
+and k by the tokens' positions in front of it.  The reference names
 ``run_experiments_BSTriton_Naive`` / ``run_experiments_BSTriton_Fused`` map
 to this runner.
 """
@@ -26,6 +28,8 @@ from typing import Optional
 import torch
 
 from .api import BlockSparsePlan, block_sparse_attention, infer_block, permute_rows
+from .rope import qk_norm_rope as norm_rope
+from .rope import rope_table
 
 REPEATS_WARMUP = 10
 REPEATS_TIMING = 25
@@ -47,7 +51,7 @@ def _time(fn, warmup: int, reps: int) -> float:
 def run_experiments_B200(args, block_mask: torch.Tensor, seq_len: int, row_perm: Optional[torch.Tensor] = None,
                          col_perm: Optional[torch.Tensor] = None, device: str = "cuda:0",
                          dtype: torch.dtype = torch.float16, *, batch_size: int = 1, warmup: int = REPEATS_WARMUP,
-                         reps: int = REPEATS_TIMING, verbose: bool = True) -> dict:
+                         reps: int = REPEATS_TIMING, verbose: bool = True, qk_norm_rope: bool = False) -> dict:
     torch.manual_seed(42)
     nheads, d = args.num_heads, args.head_dim
     q = torch.randn(batch_size, nheads, seq_len, d, device=device, dtype=dtype)
@@ -75,7 +79,19 @@ def run_experiments_B200(args, block_mask: torch.Tensor, seq_len: int, row_perm:
     if verbose:
         print(f"Average time with reordering: {t_with:.3f} ms")
         print(f"Average time without reordering: {t_without:.3f} ms")
-    return {"ms_with_reordering": t_with, "ms_without_reordering": t_without}
+    times = {"ms_with_reordering": t_with, "ms_without_reordering": t_without}
+    if qk_norm_rope:
+        cos, sin = rope_table(seq_len, d // 16 * 16, device=device) if d >= 16 else (None, None)
+        w = torch.ones(d, device=device)
+
+        def with_norm_rope():
+            a, b = norm_rope(q, k, w, w, cos=cos, sin=sin)
+            return block_sparse_attention(a, b, v, plan=plan, q_perm=rp, kv_perm=cp)
+
+        times["ms_with_norm_rope"] = _time(with_norm_rope, warmup, reps)
+        if verbose:
+            print(f"Average time with norm, rotation and reordering: {times['ms_with_norm_rope']:.3f} ms")
+    return times
 
 
 run_experiments_BSTriton_Naive = run_experiments_B200

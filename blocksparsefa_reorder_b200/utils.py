@@ -31,6 +31,7 @@ class Args:
     row_reorder: Optional[Path] = None
     col_reorder: Optional[Path] = None
     mode: str = "B200"
+    qk_norm_rope: bool = False  # beyond the reference: also time the norm and rotation of q and k
 
 
 def read_mtx(path: str):

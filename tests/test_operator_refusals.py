@@ -1,0 +1,203 @@
+"""What the operators of cross attention, shared prefixes and query / key norm
+refuse: on the host through the C ABI (no GPU work is issued, the addresses are
+never read) and through the Python entry points."""
+
+import ctypes
+import struct
+
+import pytest
+import torch
+
+import blocksparsefa_reorder_b200 as lib
+from blocksparsefa_reorder_b200 import _lib
+
+T4 = "Pqqq"
+ROPE = struct.Struct("@8i" + 6 * T4 + "4Pq2iPqfi3P")
+CROSS = struct.Struct("@8i" + 4 * T4 + "4Pf0q")
+CROSS_BWD = struct.Struct("@8i" + 8 * T4 + "5Pf0q")
+PREFIX = struct.Struct("@9i" + 6 * T4 + "3Pf0q")
+P = 0x10000
+F16, BF16, F32 = _lib.DTYPE_F16, _lib.DTYPE_BF16, _lib.DTYPE_F32
+
+
+def t4(data=P, n=64, h=6400, b=64000):
+    return data, b, h, n
+
+
+def _call(fn, packed):
+    n = ctypes.c_size_t()
+    return getattr(_lib.lib(), fn)(packed, ctypes.byref(n)), n.value
+
+
+def _cross(B=2, H=4, Hk=2, M=3, N=100, D=64, dtype=F16, lens_dtype=0, q=t4(), o=t4(), k=t4(), v=t4(), lens=0, lse=0,
+           rest=0, err=0, scale=0.125):
+    return CROSS.pack(B, H, Hk, M, N, D, dtype, lens_dtype, *q, *o, *k, *v, lens, lse, rest, err, scale)
+
+
+@pytest.mark.parametrize("kw,status", [
+    ({}, 0), ({"B": 0}, 1), ({"H": 0}, 1), ({"Hk": 0}, 1), ({"M": 0}, 1), ({"N": -1}, 1), ({"N": 0}, 0),
+    ({"dtype": F32}, 3), ({"dtype": 9}, 3), ({"H": 5}, 2), ({"D": 96}, 5), ({"scale": 0.0}, 5), ({"scale": -1.0}, 5),
+    ({"scale": float("nan")}, 5), ({"scale": float("inf")}, 5), ({"q": t4(0)}, 1), ({"k": t4(0)}, 1), ({"v": t4(0)}, 1),
+    ({"q": t4(P + 8)}, 4), ({"k": t4(n=68)}, 4), ({"v": t4(b=-64)}, 1), ({"o": t4(h=6404)}, 4), ({"rest": P + 4}, 4),
+    ({"lens": P, "lens_dtype": 7}, 3), ({"B": 1 << 16, "H": 1 << 10, "M": 1 << 10}, 5), ({"N": 2 ** 31 - 1}, 5),
+    ({"k": t4(b=0), "v": t4(b=0)}, 0),
+])
+def test_cross_forward_abi(kw, status):
+    assert _call("bsa_cross_fwd_workspace_bytes", _cross(**kw))[0] == status
+
+
+def test_cross_forward_workspace():
+    rc, n = _call("bsa_cross_fwd_workspace_bytes", _cross(B=1, N=65536))
+    assert rc == 0 and n > 0
+    assert _lib.lib().bsa_cross_fwd(_cross(B=1, N=65536), None, 0, None) == 9
+    assert _lib.lib().bsa_cross_fwd(_cross(B=1, N=65536), P, n - 1, None) == 9
+    assert _lib.lib().bsa_cross_fwd_workspace_bytes(None, ctypes.byref(ctypes.c_size_t())) == 1
+    assert _lib.lib().bsa_cross_fwd_workspace_bytes(_cross(), None) == 1
+
+
+def _bwd(B=2, H=4, Hk=2, M=3, N=100, D=64, dtype=F16, lens_dtype=0, lens=0, lse=P, delta=P, rest=0, scale=0.125, **ts):
+    names = ("q", "k", "v", "o", "dout", "dq", "dk", "dv")
+    vals = [x for n in names for x in ts.get(n, t4())]
+    return CROSS_BWD.pack(B, H, Hk, M, N, D, dtype, lens_dtype, *vals, lens, lse, rest, delta, 0, scale)
+
+
+@pytest.mark.parametrize("kw,status", [
+    ({"M": 0}, 1), ({"dtype": F32}, 3), ({"H": 3}, 2), ({"D": 32}, 5), ({"scale": -1.0}, 5), ({"lse": 0}, 1),
+    ({"delta": 0}, 1), ({"rest": P + 2}, 4), ({"dout": t4(0)}, 1), ({"dk": t4(P + 2)}, 4), ({"dq": t4(n=65)}, 4),
+    ({"v": t4(b=-8)}, 1), ({"lens": P, "lens_dtype": 5}, 3),
+])
+def test_cross_backward_abi(kw, status):
+    assert _lib.lib().bsa_cross_bwd(_bwd(**kw), None) == status
+
+
+def _prefix(B=2, H=4, Hk=2, T=1, Pn=100, C=10, D=64, dtype=F16, lens_dtype=0, lens=0, scale=0.125, **ts):
+    vals = [x for n in ("q", "o", "kp", "vp", "k", "v") for x in ts.get(n, t4())]
+    return PREFIX.pack(B, H, Hk, T, Pn, C, D, dtype, lens_dtype, *vals, lens, 0, 0, scale)
+
+
+@pytest.mark.parametrize("kw,status", [
+    ({}, 0), ({"Pn": 0}, 0), ({"C": 0}, 0), ({"Pn": 0, "C": 0}, 0), ({"T": 0}, 1), ({"C": -1}, 1), ({"dtype": F32}, 3),
+    ({"H": 3}, 2), ({"D": 128 + 64}, 5), ({"kp": t4(0)}, 1), ({"vp": t4(P + 8)}, 4), ({"k": t4(n=66)}, 4),
+    ({"lens": P, "lens_dtype": 3}, 3), ({"scale": float("nan")}, 5),
+])
+def test_prefix_abi(kw, status):
+    assert _call("bsa_prefix_fwd_workspace_bytes", _prefix(**kw))[0] == status
+
+
+def _rope(B=2, H=4, Hk=2, N=3, D=64, R=64, dtype=F16, wdtype=F32, qw=P, kw=P, cos=P, sin=P, stride=32, length=100, pdt=0,
+          pos=0, eps=1e-6, dqw=0, **ts):
+    vals = [x for n in ("q", "k", "qo", "ko", "dq", "dk") for x in ts.get(n, t4())]
+    return ROPE.pack(B, H, Hk, N, D, R, dtype, wdtype, *vals, qw, kw, cos, sin, stride, length, pdt, pos, 0, eps, 0, dqw, 0,
+                     0)
+
+
+@pytest.mark.parametrize("kw,status", [
+    ({"B": 0}, 1), ({"H": 0, "Hk": 0}, 1), ({"N": 0}, 1), ({"D": 60}, 5), ({"D": 264}, 5), ({"R": 24}, 5), ({"R": 80}, 5),
+    ({"dtype": 7}, 3), ({"wdtype": BF16}, 3), ({"cos": 0}, 1), ({"sin": 0}, 1), ({"length": 0}, 1), ({"stride": 16}, 2),
+    ({"stride": 33}, 4), ({"cos": P + 4}, 4), ({"pos": P, "pdt": 9}, 3), ({"eps": -1.0}, 1), ({"eps": float("nan")}, 1),
+    ({"q": t4(0)}, 1), ({"ko": t4(P + 2)}, 4), ({"k": t4(n=68)}, 4),
+])
+def test_rope_abi(kw, status):
+    assert _lib.lib().bsa_qk_norm_rope(_rope(**kw), None) == status
+
+
+def test_rope_backward_abi():
+    assert _call("bsa_qk_norm_rope_bwd_workspace_bytes", _rope()) == (0, 0)
+    rc, n = _call("bsa_qk_norm_rope_bwd_workspace_bytes", _rope(dqw=P))
+    assert rc == 0 and n > 0
+    assert _call("bsa_qk_norm_rope_bwd_workspace_bytes", _rope(dq=t4(0)))[0] == 1
+    assert _lib.lib().bsa_qk_norm_rope_bwd(_rope(dqw=P), P, n - 1, None) == 9
+
+
+def test_structures_have_the_compiled_sizes(tmp_path):
+    """The packed layouts above are the header's."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    src = tmp_path / "s.c"
+    inc = Path(__file__).resolve().parent.parent / "include" / "bsattn_b200.h"
+    src.write_text(f'#include <stdio.h>\n#include "{inc}"\nint main(void){{printf("%zu %zu %zu %zu", sizeof(bsa_rope_args), '
+                   "sizeof(bsa_cross_args), sizeof(bsa_cross_bwd_args), sizeof(bsa_prefix_args));}\n")
+    exe = tmp_path / "s"
+    subprocess.run([shutil.which("gcc") or "cc", str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True).stdout.split()]
+    assert got == [ROPE.size, CROSS.size, CROSS_BWD.size, PREFIX.size]
+
+
+def test_python_refuses_cpu_tensors():
+    x = torch.zeros(1, 2, 3, 64, dtype=torch.float16)
+    for call in (lambda: lib.cross_attention(x, x, x), lambda: lib.cross_attention_autograd(x, x, x),
+                 lambda: lib.cross_attention_backward(x, x, x, x, torch.zeros(1, 2, 3), x),
+                 lambda: lib.shared_prefix_attention(x, x[0], x[0], x, x), lambda: lib.qk_norm_rope(x, x),
+                 lambda: lib.qk_norm_rope_autograd(x, None)):
+        with pytest.raises(ValueError, match="must be a CUDA tensor"):
+            call()
+    with pytest.raises(ValueError, match="pass q or k"):
+        lib.qk_norm_rope(None, None)
+    with pytest.raises(TypeError):
+        lib.cross_attention([1], x, x)
+    with pytest.raises(ValueError):
+        lib.rope_table(0, 64, device="cpu")
+    with pytest.raises(ValueError):
+        lib.rope_table(8, 63, device="cpu")
+
+
+def test_rope_table_angles():
+    cos, sin = lib.rope_table(200001, 64, base=1e6, device="cpu")
+    assert cos.shape == sin.shape == (200001, 32) and cos.dtype == torch.float32
+    ang = 200000.0 * 1e6 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    assert (cos[-1].double() - ang.cos()).abs().max() <= 2 ** -24 and (sin[-1].double() - ang.sin()).abs().max() <= 2 ** -24
+
+
+@pytest.mark.gpu
+def test_python_refusals_on_the_gpu(dev):
+    h = torch.float16
+    q, k = torch.zeros(2, 4, 3, 64, dtype=h, device=dev), torch.zeros(2, 2, 9, 64, dtype=h, device=dev)
+    ln = torch.tensor([1, 2], device=dev)
+    bad = [
+        (TypeError, lambda: lib.cross_attention(q.float(), k.float(), k.float())),
+        (TypeError, lambda: lib.cross_attention(q, k.bfloat16(), k)),
+        (ValueError, lambda: lib.cross_attention(q, k, k[:, :, :5])),
+        (ValueError, lambda: lib.cross_attention(q, k[:1], k[:1])),
+        (ValueError, lambda: lib.cross_attention(q[:, :3], k, k)),
+        (ValueError, lambda: lib.cross_attention(q[0], k, k)),
+        (ValueError, lambda: lib.cross_attention(q, k, k, sm_scale=0.0)),
+        (ValueError, lambda: lib.cross_attention(q, k, k, k_lens=ln[:1])),
+        (TypeError, lambda: lib.cross_attention(q, k, k, k_lens=ln.float())),
+        (ValueError, lambda: lib.cross_attention(q, k, k, k_lens=ln.cpu())),
+        (ValueError, lambda: lib.cross_attention(q, k, k, out=torch.zeros(2, 4, 3, 32, dtype=h, device=dev))),
+        (ValueError, lambda: lib.cross_attention(q, k, k, lse_out=torch.zeros(2, 4, 4, device=dev))),
+        (ValueError, lambda: lib.cross_attention(q.transpose(2, 3), k.transpose(2, 3), k.transpose(2, 3))),
+        (_lib.BsaError, lambda: lib.cross_attention(q[..., :32].contiguous(), k[..., :32].contiguous(),
+                                                    k[..., :32].contiguous())),
+        (_lib.BsaError, lambda: lib.cross_attention(torch.zeros(2 * 4 * 3 * 64 + 1, dtype=h, device=dev)[1:].view(q.shape),
+                                                    k, k)),
+        (ValueError, lambda: lib.shared_prefix_attention(q, k[0, :1], k[0, :1], k, k)),
+        (ValueError, lambda: lib.shared_prefix_attention(q, k, k, k, k)),
+        (ValueError, lambda: lib.shared_prefix_attention(q, k[0], k[0], k, k, lens=ln[:1])),
+        (ValueError, lambda: lib.qk_norm_rope(q, k)),
+        (TypeError, lambda: lib.qk_norm_rope(q.int(), None)),
+        (TypeError, lambda: lib.qk_norm_rope(q, None, torch.ones(64, device=dev, dtype=torch.bfloat16))),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, torch.ones(32, device=dev))),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, positions=ln)),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, cos=torch.ones(8, 32, device=dev))),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, cos=torch.ones(8, 32, device=dev), sin=torch.ones(8, 32, device=dev),
+                                              positions=ln)),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, eps=-1.0)),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, out=(q[:1], None))),
+    ]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
+    # the gradient of a gradient is refused, not silently wrong
+    a, b = q.clone().requires_grad_(True), k.clone().requires_grad_(True)
+    for o in (lib.cross_attention_autograd(a, b, b), lib.qk_norm_rope_autograd(a, None)[0]):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(o.float().sum(), a, create_graph=True)
+    # a changed input is noticed
+    o = lib.cross_attention_autograd(a, b, b)
+    with torch.no_grad():
+        b.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
