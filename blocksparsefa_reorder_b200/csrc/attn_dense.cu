@@ -57,8 +57,8 @@ constexpr int kSmemLimitD = 232448;
 // setmaxnreg split: issue / two softmax / epilogue warpgroups, of a launch with 128 a thread
 constexpr int kRegsLaunchD = 128;
 constexpr int kRegsIssueD = 64;
-constexpr int kRegsSoftmaxD = 176;
-constexpr int kRegsEpilogueD = 96;
+constexpr int kRegsSoftmaxD = 168;
+constexpr int kRegsEpilogueD = 112;
 constexpr int kRegsSplitD = kRegsIssueD + 2 * kRegsSoftmaxD + kRegsEpilogueD;
 static_assert(128 * kRegsSplitD <= kThreadsD * kRegsLaunchD, "register split");
 
