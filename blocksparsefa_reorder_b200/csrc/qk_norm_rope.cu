@@ -17,6 +17,7 @@
 // keeps its token's angles in registers and walks over the token's heads.
 #include "common.cuh"
 #include "internal.h"
+#include "softmax.cuh"
 
 namespace bsa {
 
@@ -87,6 +88,25 @@ __device__ __forceinline__ void store8(uint8_t* p, const float (&f)[8]) {
   for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(f[i]);
 #pragma unroll
   for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+}
+
+// The 8 elements as pairs for the paired fp32 instructions: with scalar ones the
+// kernels were bound by issue slots (73 % of them busy at 54 % of the memory rate).
+__device__ __forceinline__ void pairs8(const float (&f)[8], uint64_t (&p)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = f32x2_pack(f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ float pair_sum(uint64_t p) {
+  float a, b;
+  f32x2_unpack(p, a, b);
+  return a + b;
+}
+template <typename T>
+__device__ __forceinline__ void store_pairs(uint8_t* p, const uint64_t (&y)[4]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f32x2_unpack(y[i], f[2 * i], f[2 * i + 1]);
+  store8<T>(p, f);
 }
 
 template <int LPR>
@@ -213,33 +233,45 @@ __global__ void __launch_bounds__(kThreads, 4) rope_fwd_kernel(const RopeParams 
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) A[i] *= t.c[i];
+  uint64_t A2[4], B2[4];
+  pairs8(A, A2);
+  pairs8(B, B2);
   const float inv_d = 1.f / static_cast<float>(p.D);
+  const int64_t xstep = E * sd.xs_h, ystep = E * sd.ys_h;
+  const uint8_t* xn = xp + E * ((h0 + U) * sd.xs_h);
+  yp += E * (h0 * sd.ys_h);
   for (int h = h0; h < h1; h += U) {
     Vec8<T> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       raw[u] = next[u];
-      next[u] = in && h + U + u < h1 ? load8<T>(xp + E * ((h + U + u) * sd.xs_h)) : zero8<T>();
+      next[u] = in && h + U + u < h1 ? load8<T>(xn) : zero8<T>();
+      xn += xstep;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float x[8], o[8];
+      uint64_t x2[4], o2[4];
       unpack8<T>(raw[u], x);
-      float ss = 0.f;
+      pairs8(x, x2);
+      uint64_t s2 = f32x2_mul(x2[0], x2[0]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-      ss = group_sum<LPR>(ss);
+      for (int i = 1; i < 4; ++i) s2 = f32x2_fma(x2[i], x2[i], s2);
+      const float ss = group_sum<LPR>(pair_sum(s2));
       // (a position outside the table: NaN rather than a row that looks right)
       const float r = valid ? rsqrtf(fmaf(ss, inv_d, p.eps)) : NAN;
+      const uint64_t r2 = f32x2_pack(r, r);
       other_half<T, IL>(raw[u], x, t.partner, o);
+      pairs8(o, o2);
       if (t.on) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = r * fmaf(x[i], A[i], o[i] * B[i]);
+        for (int i = 0; i < 4; ++i) x2[i] = f32x2_mul(r2, f32x2_fma(x2[i], A2[i], f32x2_mul(o2[i], B2[i])));
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = r * (x[i] * A[i]);
+        for (int i = 0; i < 4; ++i) x2[i] = f32x2_mul(r2, f32x2_mul(x2[i], A2[i]));
       }
-      if (in && h + u < h1) store8<T>(yp + E * ((h + u) * sd.ys_h), x);
+      if (in && h + u < h1) store_pairs<T>(yp, x2);
+      yp += ystep;
     }
   }
 }
@@ -256,10 +288,11 @@ __global__ void __launch_bounds__(kThreads, 3) rope_bwd_kernel(const RopeParams 
   const int lane = threadIdx.x & 31, l = lane % LPR;
   const RopeSide& sd = p.side[blockIdx.y];
   const bool cols = l * 8 < p.D;
-  float w[8], dw[8];
+  float w[8];
+  uint64_t w2[4], dw2[4] = {0, 0, 0, 0};
   load_weight<T>(sd.w, p.w_f32, l, cols, w);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) dw[i] = 0.f;
+  pairs8(w, w2);
+  const int64_t xstep = E * sd.xs_h, dstep = E * sd.ds_h, ystep = E * sd.ys_h;
   const float inv_d = 1.f / static_cast<float>(p.D);
   const int chunks = (sd.heads + p.chunk - 1) / p.chunk;
   const int64_t items = p.tokens * chunks;
@@ -272,54 +305,68 @@ __global__ void __launch_bounds__(kThreads, 3) rope_bwd_kernel(const RopeParams 
     const int64_t b = token / p.N, n = token - b * p.N;
     const int h0 = static_cast<int>(ck) * p.chunk, h1 = min(h0 + p.chunk, sd.heads);
     const bool in = live && cols;
-    const uint8_t* xp = sd.x + E * (b * sd.xs_b + n * sd.xs_n + l * 8);
-    const uint8_t* dp = sd.dy + E * (b * sd.ds_b + n * sd.ds_n + l * 8);
-    uint8_t* yp = sd.y + E * (b * sd.ys_b + n * sd.ys_n + l * 8);
-    Vec8<T> nx = in ? load8<T>(xp + E * (h0 * sd.xs_h)) : zero8<T>();
-    Vec8<T> nd = in ? load8<T>(dp + E * (h0 * sd.ds_h)) : zero8<T>();
+    const uint8_t* xp = sd.x + E * (b * sd.xs_b + n * sd.xs_n + h0 * sd.xs_h + l * 8);
+    const uint8_t* dp = sd.dy + E * (b * sd.ds_b + n * sd.ds_n + h0 * sd.ds_h + l * 8);
+    uint8_t* yp = sd.y + E * (b * sd.ys_b + n * sd.ys_n + h0 * sd.ys_h + l * 8);
+    Vec8<T> nx = in ? load8<T>(xp) : zero8<T>();
+    Vec8<T> nd = in ? load8<T>(dp) : zero8<T>();
     int64_t pos = 0;
     const bool valid = live && token_pos(p, b, n, pos);
     if (live && !valid && l == 0) set_err(p.err, BSA_DEVERR_COORD);
     Turn t;
     load_turn<IL>(p, l, lane, pos, valid, t);
+    // (turned back: the sines with their signs the other way)
+    uint64_t c2[4], s2[4];
+    pairs8(t.c, c2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s2[i] = f32x2_pack(-t.s[2 * i], -t.s[2 * i + 1]);
     for (int hh = 0; hh < p.chunk; ++hh) {
       const int h = h0 + hh;
       const Vec8<T> rx = nx, rd = nd;
       const bool more = in && hh + 1 < p.chunk && h + 1 < h1;
-      nx = more ? load8<T>(xp + E * ((h + 1) * sd.xs_h)) : zero8<T>();
-      nd = more ? load8<T>(dp + E * ((h + 1) * sd.ds_h)) : zero8<T>();
+      xp += xstep, dp += dstep;
+      nx = more ? load8<T>(xp) : zero8<T>();
+      nd = more ? load8<T>(dp) : zero8<T>();
       float x[8], g[8], o[8];
+      uint64_t x2[4], g2[4], o2[4];
       unpack8<T>(rx, x);
       unpack8<T>(rd, g);
+      pairs8(x, x2);
+      pairs8(g, g2);
       other_half<T, IL>(rd, g, t.partner, o);
+      pairs8(o, o2);
       if (t.on) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = fmaf(g[i], t.c[i], -o[i] * t.s[i]);
+        for (int i = 0; i < 4; ++i) g2[i] = f32x2_fma(g2[i], c2[i], f32x2_mul(o2[i], s2[i]));
       }
-      float ss = 0.f, dot = 0.f;
+      uint64_t ss2 = f32x2_mul(x2[0], x2[0]), u2[4], dot2 = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ss = fmaf(x[i], x[i], ss);
-        dot = fmaf(g[i] * w[i], x[i], dot);
+      for (int i = 0; i < 4; ++i) {
+        if (i) ss2 = f32x2_fma(x2[i], x2[i], ss2);
+        u2[i] = f32x2_mul(g2[i], w2[i]);
+        dot2 = f32x2_fma(u2[i], x2[i], dot2);
       }
-      ss = group_sum<LPR>(ss);
-      dot = group_sum<LPR>(dot);
-      const float r = rsqrtf(fmaf(ss, inv_d, p.eps));
-      const float m = dot * r * inv_d;  // mean(u o n)
+      const float ss = group_sum<LPR>(pair_sum(ss2));
+      const float dot = group_sum<LPR>(pair_sum(dot2));
       const bool ok = in && h < h1;
+      // (a row that is not there adds 0 to dw, whatever eps is)
+      const float r = ok ? (valid ? rsqrtf(fmaf(ss, inv_d, p.eps)) : NAN) : 0.f;
+      const float m = -dot * r * inv_d;  // -mean(u o n)
+      const uint64_t r2 = f32x2_pack(r, r), m2 = f32x2_pack(m, m);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float nn = x[i] * r;
-        if (ok) dw[i] = fmaf(g[i], nn, dw[i]);
-        x[i] = valid ? r * (g[i] * w[i] - nn * m) : NAN;
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t n2 = f32x2_mul(x2[i], r2);
+        dw2[i] = f32x2_fma(g2[i], n2, dw2[i]);
+        x2[i] = f32x2_mul(r2, f32x2_fma(n2, m2, u2[i]));
       }
-      if (ok) store8<T>(yp + E * (h * sd.ys_h), x);
+      if (ok) store_pairs<T>(yp, x2);
+      yp += ystep;
     }
   }
   if (!p.partial) return;
   const int g = threadIdx.x / LPR;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sums[g][l * 8 + i] = dw[i];
+  for (int i = 0; i < 4; ++i) f32x2_unpack(dw2[i], sums[g][l * 8 + 2 * i], sums[g][l * 8 + 2 * i + 1]);
   __syncthreads();
   for (int c = threadIdx.x; c < p.D; c += kThreads) {
     float a = 0.f;
