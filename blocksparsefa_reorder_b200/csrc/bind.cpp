@@ -177,7 +177,9 @@ bsa_rope_args rope_args(const RopeIn& in) {
   a.R = dim(2 * c.size(1), "R");
   a.cos = c.data_ptr<float>(), a.sin = s.data_ptr<float>();
   a.table_len = dim(c.size(0), "the tables' length");
-  a.table_stride = std::max(c.stride(0), c.size(1));
+  // (an expanded row would be read as rows of its own, past its memory)
+  TORCH_CHECK_VALUE(c.size(0) == 1 || c.stride(0) >= c.size(1), "the tables' rows must not overlap");
+  a.table_stride = c.size(0) == 1 ? c.size(1) : c.stride(0);
   if (in.positions) {
     const Tensor& p = *in.positions;
     require_cuda(p, "positions");

@@ -184,6 +184,8 @@ def test_python_refusals_on_the_gpu(dev):
         (ValueError, lambda: lib.qk_norm_rope(q, None, cos=torch.ones(8, 32, device=dev))),
         (ValueError, lambda: lib.qk_norm_rope(q, None, cos=torch.ones(8, 32, device=dev), sin=torch.ones(8, 32, device=dev),
                                               positions=ln)),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, cos=torch.ones(1, 32, device=dev).expand(8, 32),
+                                              sin=torch.ones(1, 32, device=dev).expand(8, 32))),
         (ValueError, lambda: lib.qk_norm_rope(q, None, eps=-1.0)),
         (ValueError, lambda: lib.qk_norm_rope(q, None, out=(q[:1], None))),
     ]
