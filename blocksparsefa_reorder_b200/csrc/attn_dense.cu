@@ -1145,7 +1145,8 @@ int validate(const DenseCall& c) {
   if (!aligned(c.q, c.B, c.H, c.M) || !aligned(c.o, c.B, c.H, c.M)) return BSA_ERR_ALIGNMENT;
   for (int i = 0; i < c.n; ++i) {
     if (c.keys[i] < 0) return BSA_ERR_INVALID_ARG;
-    if (c.keys[i] > INT32_MAX - 65536) return BSA_ERR_UNSUPPORTED;
+    // key numbers are 32-bit, with a range's length added
+    if (c.keys[i] > INT32_MAX / 2) return BSA_ERR_UNSUPPORTED;
     if (!c.keys[i]) continue;
     if (!c.k[i].data || !c.v[i].data) return BSA_ERR_INVALID_ARG;
     const int kb = c.shared_kv[i] ? 1 : c.B;

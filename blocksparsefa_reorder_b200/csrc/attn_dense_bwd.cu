@@ -759,7 +759,7 @@ int cross_bwd_validate(const bsa_cross_bwd_args* a) {
   if (!(a->sm_scale > 0.f) || !(a->sm_scale < INFINITY)) return BSA_ERR_UNSUPPORTED;
   if (!a->lse || !a->delta) return BSA_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(a->o_rest) % 16) return BSA_ERR_ALIGNMENT;
-  if (static_cast<int64_t>(a->B) * a->H * a->M > INT32_MAX / 2 || a->N > INT32_MAX - 65536) return BSA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(a->B) * a->H * a->M > INT32_MAX / 2 || a->N > INT32_MAX / 2) return BSA_ERR_UNSUPPORTED;
   const bsa_tensor4d* qs[] = {&a->q, &a->o, &a->dout, &a->dq};
   const bsa_tensor4d* ks[] = {&a->k, &a->v, &a->dk, &a->dv};
   for (int i = 0; i < 4; ++i) {

@@ -452,7 +452,7 @@ bool rows_aligned(const bsa_tensor4d& t, int B, int H, int N, int eb) {
 
 int validate(const bsa_rope_args* a, bool bwd) {
   if (!a) return BSA_ERR_INVALID_ARG;
-  if (a->B <= 0 || a->H < 0 || a->Hk < 0 || a->H + a->Hk <= 0 || a->N <= 0 || a->D <= 0) return BSA_ERR_INVALID_ARG;
+  if (a->B <= 0 || a->H < 0 || a->Hk < 0 || (a->H == 0 && a->Hk == 0) || a->N <= 0 || a->D <= 0) return BSA_ERR_INVALID_ARG;
   const int eb = dtype_bytes(a->dtype);
   if (!eb) return BSA_ERR_DTYPE;
   if (a->D % 8 || a->D > kMaxD || a->R < 0 || a->R > a->D || a->R % 16) return BSA_ERR_UNSUPPORTED;

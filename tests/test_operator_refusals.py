@@ -40,6 +40,7 @@ def _cross(B=2, H=4, Hk=2, M=3, N=100, D=64, dtype=F16, lens_dtype=0, q=t4(), o=
     ({"scale": float("nan")}, 5), ({"scale": float("inf")}, 5), ({"q": t4(0)}, 1), ({"k": t4(0)}, 1), ({"v": t4(0)}, 1),
     ({"q": t4(P + 8)}, 4), ({"k": t4(n=68)}, 4), ({"v": t4(b=-64)}, 1), ({"o": t4(h=6404)}, 4), ({"rest": P + 4}, 4),
     ({"lens": P, "lens_dtype": 7}, 3), ({"B": 1 << 16, "H": 1 << 10, "M": 1 << 10}, 5), ({"N": 2 ** 31 - 1}, 5),
+    ({"N": 2 ** 30 + 5, "k": t4(n=0), "v": t4(n=0)}, 5),
     ({"k": t4(b=0), "v": t4(b=0)}, 0),
 ])
 def test_cross_forward_abi(kw, status):
@@ -64,7 +65,7 @@ def _bwd(B=2, H=4, Hk=2, M=3, N=100, D=64, dtype=F16, lens_dtype=0, lens=0, lse=
 @pytest.mark.parametrize("kw,status", [
     ({"M": 0}, 1), ({"dtype": F32}, 3), ({"H": 3}, 2), ({"D": 32}, 5), ({"scale": -1.0}, 5), ({"lse": 0}, 1),
     ({"delta": 0}, 1), ({"rest": P + 2}, 4), ({"dout": t4(0)}, 1), ({"dk": t4(P + 2)}, 4), ({"dq": t4(n=65)}, 4),
-    ({"v": t4(b=-8)}, 1), ({"lens": P, "lens_dtype": 5}, 3),
+    ({"v": t4(b=-8)}, 1), ({"lens": P, "lens_dtype": 5}, 3), ({"N": 2 ** 30 + 5}, 5),
 ])
 def test_cross_backward_abi(kw, status):
     assert _lib.lib().bsa_cross_bwd(_bwd(**kw), None) == status
@@ -78,7 +79,7 @@ def _prefix(B=2, H=4, Hk=2, T=1, Pn=100, C=10, D=64, dtype=F16, lens_dtype=0, le
 @pytest.mark.parametrize("kw,status", [
     ({}, 0), ({"Pn": 0}, 0), ({"C": 0}, 0), ({"Pn": 0, "C": 0}, 0), ({"T": 0}, 1), ({"C": -1}, 1), ({"dtype": F32}, 3),
     ({"H": 3}, 2), ({"D": 128 + 64}, 5), ({"kp": t4(0)}, 1), ({"vp": t4(P + 8)}, 4), ({"k": t4(n=66)}, 4),
-    ({"lens": P, "lens_dtype": 3}, 3), ({"scale": float("nan")}, 5),
+    ({"lens": P, "lens_dtype": 3}, 3), ({"scale": float("nan")}, 5), ({"Pn": 2 ** 30 + 5}, 5), ({"C": 2 ** 30 + 5}, 5),
 ])
 def test_prefix_abi(kw, status):
     assert _call("bsa_prefix_fwd_workspace_bytes", _prefix(**kw))[0] == status
@@ -92,7 +93,7 @@ def _rope(B=2, H=4, Hk=2, N=3, D=64, R=64, dtype=F16, wdtype=F32, qw=P, kw=P, co
 
 
 @pytest.mark.parametrize("kw,status", [
-    ({"B": 0}, 1), ({"H": 0, "Hk": 0}, 1), ({"N": 0}, 1), ({"D": 60}, 5), ({"D": 264}, 5), ({"R": 24}, 5), ({"R": 80}, 5),
+    ({"B": 0}, 1), ({"H": 0, "Hk": 0}, 1), ({"H": 2 ** 31 - 1, "Hk": 2 ** 31 - 1}, 5), ({"N": 0}, 1), ({"D": 60}, 5), ({"D": 264}, 5), ({"R": 24}, 5), ({"R": 80}, 5),
     ({"dtype": 7}, 3), ({"wdtype": BF16}, 3), ({"cos": 0}, 1), ({"sin": 0}, 1), ({"length": 0}, 1), ({"stride": 16}, 2),
     ({"stride": 33}, 4), ({"cos": P + 4}, 4), ({"pos": P, "pdt": 9}, 3), ({"eps": -1.0}, 1), ({"eps": float("nan")}, 1),
     ({"q": t4(0)}, 1), ({"ko": t4(P + 2)}, 4), ({"k": t4(n=68)}, 4),
