@@ -6,6 +6,7 @@
 //
 // Wrong types raise TypeError, wrong values ValueError, a refusal by the C ABI
 // BsaError, as in the package's other entry points.
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -84,11 +85,29 @@ Tensor rows(const Tensor& g) {
 
 Tensor contiguous_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 
+// A tensor of the caller's that the call writes: as in PyTorch's own out=
+// arguments its rows lie apart, and autograd learns that it changed.
+void written(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name, " must not be expanded: its rows overlap");
+  TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+                    " requires a gradient: writing it is not differentiable");
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor output(const OptTensor& out, const Tensor& x, const char* name) {
   if (!out) return contiguous_like(x);
   TORCH_CHECK_VALUE(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->device() == x.device(), name,
                     " has the wrong shape, dtype or device");
+  written(*out, name);
   return *out;
+}
+
+// An output over memory that is read (`same`: it may be that very tensor).
+void apart(const OptTensor& out, const Tensor& x, const char* name, bool same = false) {
+  if (!out || !x.numel()) return;
+  const auto s = at::get_overlap_status(*out, x);
+  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Partial && (same || s != at::MemOverlapStatus::Full), name,
+                    " overlaps an input");
 }
 
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
@@ -200,8 +219,16 @@ std::tuple<OptTensor, OptTensor> rope_forward(const RopeIn& in, const OptTensor&
                                               const OptTensor& err) {
   bsa_rope_args a = rope_args(in);
   OptTensor oq, ok;
-  if (in.q) oq = output(q_out, *in.q, "q_out"), a.q_out = t4(*oq, "q_out");
-  if (in.k) ok = output(k_out, *in.k, "k_out"), a.k_out = t4(*ok, "k_out");
+  if (in.q) {
+    apart(q_out, *in.q, "q_out", true);
+    if (in.k) apart(q_out, *in.k, "q_out");
+    oq = output(q_out, *in.q, "q_out"), a.q_out = t4(*oq, "q_out");
+  }
+  if (in.k) {
+    apart(k_out, *in.k, "k_out", true);
+    if (in.q) apart(k_out, *in.q, "k_out");
+    ok = output(k_out, *in.k, "k_out"), a.k_out = t4(*ok, "k_out");
+  }
   if (rope_empty(a)) return {oq, ok};
   const Tensor& x = in.q ? *in.q : *in.k;
   a.err_flag = flag(err);
@@ -332,6 +359,7 @@ OptTensor lse_output(bool want, const OptTensor& out, const Tensor& q) {
     TORCH_CHECK_VALUE(out->sizes() == q.sizes().slice(0, 3) && out->scalar_type() == at::kFloat && out->is_contiguous() &&
                           out->device() == q.device(),
                       "lse_out must be a contiguous float32 [B, H, tokens] tensor on q's device");
+    written(*out, "lse_out");
     return out;
   }
   return want ? OptTensor(at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat))) : OptTensor();
@@ -367,9 +395,11 @@ std::tuple<Tensor, OptTensor> cross_forward(const Tensor& q_, const Tensor& k_, 
   bsa_cross_args a{};
   a.lens_dtype = lens_dtype(k_lens, q_, "k_lens");
   a.sm_scale = scale_of(sm_scale, q_.size(3));
+  for (const Tensor* t : {&q_, &k_, &v_}) apart(out, *t, "out");
   const Tensor o = output(out, q_, "out");
   const OptTensor lse = lse_output(return_lse, lse_out, q_);
   if (o_rest) {
+    for (const Tensor* t : {&q_, &k_, &v_, &o}) apart(o_rest, *t, "o_rest");
     output(o_rest, q_, "o_rest");
     TORCH_CHECK_VALUE(o_rest->strides() == o.strides(), "o_rest must be laid out as the output");
     a.o_rest = o_rest->data_ptr();
@@ -400,8 +430,8 @@ std::tuple<Tensor, Tensor, Tensor> cross_backward(const Tensor& q_, const Tensor
                     "lse must be the forward's contiguous float32 [B, H, M] LSE");
   bsa_cross_bwd_args a{};
   if (o_rest) {
-    output(o_rest, q_, "o_rest");
-    TORCH_CHECK_VALUE(o_rest->strides() == o_.strides(), "o_rest must be laid out as o");
+    like_q(*o_rest, q_, "o_rest");
+    TORCH_CHECK_VALUE(o_rest->sizes() == q_.sizes() && o_rest->strides() == o_.strides(), "o_rest must be laid out as o");
     a.o_rest = o_rest->data_ptr();
   }
   a.lens_dtype = lens_dtype(k_lens, q_, "k_lens");
@@ -468,6 +498,7 @@ std::tuple<Tensor, OptTensor> prefix_forward(const Tensor& q_, const Tensor& kp_
   bsa_prefix_args a{};
   a.lens_dtype = lens_dtype(lens, q_, "lens");
   a.sm_scale = scale_of(sm_scale, q_.size(3));
+  for (const Tensor* t : {&q_, &kp_, &vp_, &k_, &v_}) apart(out, *t, "out");
   const Tensor o = output(out, q_, "out");
   const OptTensor lse = lse_output(return_lse, lse_out, q_);
   if (q_.numel() == 0) return {o, lse};

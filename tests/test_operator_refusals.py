@@ -156,6 +156,7 @@ def test_python_refusals_on_the_gpu(dev):
     h = torch.float16
     q, k = torch.zeros(2, 4, 3, 64, dtype=h, device=dev), torch.zeros(2, 2, 9, 64, dtype=h, device=dev)
     ln = torch.tensor([1, 2], device=dev)
+    flat = torch.zeros(q.numel() + 64, dtype=h, device=dev)
     bad = [
         (TypeError, lambda: lib.cross_attention(q.float(), k.float(), k.float())),
         (TypeError, lambda: lib.cross_attention(q, k.bfloat16(), k)),
@@ -189,6 +190,16 @@ def test_python_refusals_on_the_gpu(dev):
                                               sin=torch.ones(1, 32, device=dev).expand(8, 32))),
         (ValueError, lambda: lib.qk_norm_rope(q, None, eps=-1.0)),
         (ValueError, lambda: lib.qk_norm_rope(q, None, out=(q[:1], None))),
+        # outputs whose rows overlap, lie over an input, or need a gradient
+        (ValueError, lambda: lib.qk_norm_rope(q, None, out=(q[:1].expand(2, 4, 3, 64), None))),
+        (ValueError, lambda: lib.qk_norm_rope(flat[:-64].view(q.shape), None, out=(flat[64:].view(q.shape), None))),
+        (ValueError, lambda: lib.qk_norm_rope(q, q.clone(), out=(None, q))),
+        (ValueError, lambda: lib.qk_norm_rope(q, None, out=(torch.zeros_like(q).requires_grad_(True), None))),
+        (ValueError, lambda: lib.cross_attention(q, k, k, out=q[:1].expand(2, 4, 3, 64))),
+        (ValueError, lambda: lib.cross_attention(q, k, k, out=q)),
+        (ValueError, lambda: lib.cross_attention(q, q, q, out=q)),
+        (ValueError, lambda: lib.cross_attention(q, k, k, o_rest=q)),
+        (ValueError, lambda: lib.shared_prefix_attention(k, k[0], k[0], k, k, out=k)),
     ]
     for kind, call in bad:
         with pytest.raises(kind):
@@ -198,7 +209,14 @@ def test_python_refusals_on_the_gpu(dev):
     for o in (lib.cross_attention_autograd(a, b, b), lib.qk_norm_rope_autograd(a, None)[0]):
         with pytest.raises(RuntimeError, match="differentiable once"):
             torch.autograd.grad(o.float().sum(), a, create_graph=True)
-    # a changed input is noticed
+    # a changed input is noticed, one that an output went into too
+    c = q.clone().requires_grad_(True)
+    x = c * 2
+    y = x * x
+    with torch.no_grad():
+        lib.qk_norm_rope(x, None, out=(x, None))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
     o = lib.cross_attention_autograd(a, b, b)
     with torch.no_grad():
         b.add_(1)
