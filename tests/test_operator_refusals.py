@@ -222,3 +222,38 @@ def test_python_refusals_on_the_gpu(dev):
         b.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         o.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["cross", "rope"])
+def test_captured_backward_and_an_eager_graph_of_the_same_leaves(dev, op):
+    """A capture whose gradient would go to the eager graph's (default) stream is
+    refused; without that graph it is captured."""
+    g = torch.Generator(device=dev).manual_seed(4)
+    q = torch.randn(1, 2, 5, 64, device=dev, dtype=torch.float16, generator=g).requires_grad_(True)
+    k = torch.randn(1, 2, 9, 64, device=dev, dtype=torch.float16, generator=g).requires_grad_(True)
+
+    def forward():
+        return lib.cross_attention_autograd(q, k, k) if op == "cross" else lib.qk_norm_rope_autograd(q, None)[0]
+
+    def capture(step):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        return graph, out
+
+    want, = torch.autograd.grad(forward().sum(), q)
+    eager = forward()
+    for step in (lambda: forward().sum().backward(), lambda: torch.autograd.grad(forward().sum(), q)):
+        with pytest.raises(RuntimeError, match="captured backward pass"):
+            capture(step)
+        torch.cuda.synchronize()
+    del eager
+    graph, (got,) = capture(lambda: torch.autograd.grad(forward().sum(), q))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and q.grad is None
+    graph, _ = capture(lambda: forward().sum().backward())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(q.grad, want)
