@@ -866,7 +866,9 @@ struct Source {
 };
 struct DensePlan {
   Source s[2];
-  bool join;
+  bool join;   // attn_join_kernel joins the partial results
+  bool fused;  // the second source's few-rows kernel joins the first one's
+  bool partial(int i) const { return join || (fused && i == 0); }
   size_t total;
 };
 
@@ -968,9 +970,15 @@ DensePlan plan_of(const DenseCall& c) {
       dense = true;
   }
   if (dense) split_dense(pl.s, c.keys, c.n, c.D, c.n > 1);
-  pl.join = c.n > 1 || pl.s[0].splits > 1;
+  // The second source's kernel joins the first one's partial results with its own
+  // where it has all of a row's keys and its warps have at most four each to join
+  // (64 sequences behind 32,768 keys, 18 ranges: 73 us against 80 with a third
+  // kernel; one sequence, whose 8 CTAs would join 148 ranges: 45 against 41).
+  pl.fused = c.n > 1 && pl.s[1].few && pl.s[1].splits == 1 && pl.s[0].splits <= 32;
+  pl.join = !pl.fused && (c.n > 1 || pl.s[0].splits > 1);
   size_t off = 0;
-  for (int i = 0; pl.join && i < c.n; ++i) {
+  for (int i = 0; i < c.n; ++i) {
+    if (!pl.partial(i)) continue;
     const size_t rows = static_cast<size_t>(pl.s[i].units) * pl.s[i].rows * pl.s[i].splits;
     pl.s[i].o_off = off;
     off += round256(rows * c.D * sizeof(float));
@@ -1026,7 +1034,12 @@ int launch_few(const DenseCall& c, const DensePlan& pl, int i, bool late, uint8_
   p.os_b = c.o.stride_b, p.os_h = c.o.stride_h, p.os_n = c.o.stride_n;
   p.lse = c.lse;
   p.o_rest = static_cast<uint8_t*>(c.o_rest);
-  if (pl.join) p.part_o = part_o(s, ws), p.part_lse = part_lse(s, ws);
+  if (pl.partial(i)) p.part_o = part_o(s, ws), p.part_lse = part_lse(s, ws);
+  if (pl.fused && i == 1) {
+    const Source& other = pl.s[0];
+    p.other_o = part_o(other, ws), p.other_lse = part_lse(other, ws);
+    p.other_splits = other.splits, p.other_rows = other.rows;
+  }
   p.scale_log2 = c.sm_scale * 1.4426950408889634f;
   p.late = late;
   p.err = c.err;
@@ -1065,7 +1078,7 @@ int launch_dense(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStrea
     pt.shared_kv = c.shared_kv[i];
     pt.causal = c.causal[i];
     pt.lens = c.lens[i];
-    if (pl.join) pt.part_o = part_o(s, ws), pt.part_lse = part_lse(s, ws);
+    if (pl.partial(i)) pt.part_o = part_o(s, ws), pt.part_lse = part_lse(s, ws);
     if ((r = map_of(&mq[j], c.q, c.B, c.H, c.M, D, BF16, &pt.qb_mul, s.mt, s.gh, s.nb))) return r;
     if (!c.keys[i]) continue;  // no key tile is ever loaded
     const int kb = c.shared_kv[i] ? 1 : c.B;

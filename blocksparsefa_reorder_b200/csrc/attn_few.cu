@@ -21,7 +21,8 @@
 // permutes pair up along the keys; P^T's operand is S^T's accumulator through
 // movmatrix.  The reference point m of a row moves only when a score exceeds it
 // by the slack, which one vote tells (softmax.cuh).  The warps' sums are joined
-// in shared memory in a fixed order.
+// in shared memory in a fixed order, behind a shared prefix together with the
+// prefix kernel's partial results.
 #include "common.cuh"
 #include "dense.h"
 #include "internal.h"
@@ -65,7 +66,8 @@ __device__ __forceinline__ uint32_t pair_at(const uint4& lo, const uint4& hi, in
   return __byte_perm(word(lo, e >> 1), word(hi, e >> 1), (e & 1) ? 0x7632 : 0x5410);
 }
 
-template <int D, bool BF16, int NR>
+// OTHER: joins the other source's partial results too.
+template <int D, bool BF16, int NR, bool OTHER>
 __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(const __grid_constant__ FewParams p) {
   constexpr int KP = D / 32;  // 16-byte pieces of a K row a lane holds
   constexpr int VP = D / 64;  // and of a V row
@@ -222,6 +224,54 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
       }
     }
   }
+  // The other source's partial results, every eighth of a row to each warp, as if
+  // they were keys of weight 2^lse: a lane takes the dims its accumulators hold.
+  if constexpr (OTHER) {
+    grid_dependency_wait();
+    constexpr int KU = 2 * UB;  // in flight
+    const int64_t row0 = static_cast<int64_t>(hk) * p.other_rows + static_cast<int64_t>(b) * p.G * p.M;
+    for (int k = warp; k < p.other_splits; k += kWarpsF * KU) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        float l[KU][2];
+        float4 f[KU][2][2 * VP];
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = n * 8 + 2 * c + e, kk = k + u * kWarpsF;
+            const bool there = r < p.rows && kk < p.other_splits;
+            const int64_t at = there ? (row0 + r) * p.other_splits + kk : 0;
+            l[u][e] = there ? __ldcg(p.other_lse + at) : -INFINITY;
+            const float4* src = reinterpret_cast<const float4*>(p.other_o + at * D + g * 8);
+#pragma unroll
+            for (int i = 0; i < 2 * VP; ++i)  // (a partial result without keys is only its lse)
+              f[u][e][i] = l[u][e] != -INFINITY ? __ldcg(src + (i >> 1) * 16 + (i & 1)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (l[u][e] == -INFINITY) continue;
+            const float mx = fmaxf(m_run[n][e], l[u][e]);
+            const float alpha = ex2_approx(m_run[n][e] - mx), w = ex2_approx(l[u][e] - mx);
+            m_run[n][e] = mx;
+            l_run[n][e] = fmaf(l_run[n][e], alpha, g == 0 ? w : 0.f);  // (summed over the lanes g below)
+#pragma unroll
+            for (int i = 0; i < 2 * VP; ++i) {
+              const float4 x = f[u][e][i];
+              const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                // element 8 (i / 2) + 4 (i % 2) + t of the lane's dims
+                const int j = VP == 2 ? 4 * (i & 1) + t : 2 * i + (t >> 1), h = VP == 2 ? i >> 1 : t & 1;
+                acc[n][j][2 * h + e] = fmaf(acc[n][j][2 * h + e], alpha, w * xs[t]);
+              }
+            }
+          }
+      }
+    }
+  }
   // ------------------------------------------------ join the warps
 #pragma unroll
   for (int n = 0; n < NR; ++n)
@@ -304,13 +354,13 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
       if (col == 0 && p.lse) p.lse[(static_cast<int64_t>(rb) * p.H + rh) * p.M + rm] = lse;
     }
   }
-  if (p.late) grid_dependency_wait();
+  if (!OTHER && p.late) grid_dependency_wait();
 }
 
-template <int D, bool BF16, int NR>
+template <int D, bool BF16, int NR, bool OTHER>
 int launch_t(const FewParams& p, cudaStream_t st) {
   constexpr int smem = kWarpsF * 8 * NR * (D + 2) * static_cast<int>(sizeof(float));
-  auto kern = attn_few_kernel<D, BF16, NR>;
+  auto kern = attn_few_kernel<D, BF16, NR, OTHER>;
   int rc = opt_in_smem(reinterpret_cast<const void*>(kern), smem);
   if (rc) return rc;
   cudaLaunchAttribute attr[1];
@@ -331,7 +381,8 @@ int launch_t(const FewParams& p, cudaStream_t st) {
 
 int launch_attn_few(const FewParams& p, int D, bool bf16, cudaStream_t st) {
 #define BSA_FEW_CASE(D_, BF_, NR_) \
-  if (D == D_ && bf16 == BF_ && (p.rows > 8 ? 2 : 1) == NR_) return launch_t<D_, BF_, NR_>(p, st);
+  if (D == D_ && bf16 == BF_ && (p.rows > 8 ? 2 : 1) == NR_) \
+    return p.other_o ? launch_t<D_, BF_, NR_, true>(p, st) : launch_t<D_, BF_, NR_, false>(p, st);
   BSA_FEW_CASE(128, true, 1)
   BSA_FEW_CASE(128, true, 2)
   BSA_FEW_CASE(128, false, 1)

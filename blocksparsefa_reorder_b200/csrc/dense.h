@@ -33,6 +33,11 @@ struct FewParams {
   float* lse;
   float* part_o;  // partial results, or null: this is the whole result
   float* part_lse;
+  // Partial results of the same rows from the other source's kernel of the call,
+  // to be joined here (null: none): row b G M + r of shared unit hk.
+  const float* other_o;
+  const float* other_lse;
+  int other_splits, other_rows;
   float scale_log2;
   int late;       // launched behind the other source's kernel of the same call: see attn_few.cu
   int32_t* err;
