@@ -362,6 +362,33 @@ def test_prefix_matches_definition(c, D, dtype):
     assert torch.equal(shared_prefix_attention(q, kp, vp, k, v, lens=ln), o)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, HF)])
+@pytest.mark.parametrize("B,H,Hk,T,P", [(2, 2, 1, 1, 300), (2, 2, 1, 1, 8192), (2, 2, 1, 1, 8500), (1, 8, 1, 1, 8500),
+                                        (3, 4, 2, 4, 8192), (9, 12, 3, 4, 4000), (1, 1, 1, 16, 5000)])
+def test_prefix_partial_results_on_both_sides_of_the_joining_rule(B, H, Hk, T, P, D, dtype):
+    """Few own rows: up to 32 ranges of the prefix are joined by the own keys'
+    kernel, more by one of its own; a NaN query stays in its own rows."""
+    g = torch.Generator(device="cuda").manual_seed(P + B)
+    C = 40
+    q = _rand((B, H, T, D), dtype, g)
+    kp, vp = _rand((Hk, P, D), dtype, g), _rand((Hk, P, D), dtype, g)
+    k, v = _rand((B, Hk, C, D), dtype, g), _rand((B, Hk, C, D), dtype, g)
+    ln = torch.tensor([T if b % 2 else 0 for b in range(B)], device="cuda")
+    _poison(k, ln), _poison(v, ln)
+    t = torch.arange(T, device="cuda")
+    own = torch.arange(C, device="cuda") < (ln[:, None, None] - (T - 1 - t)[:, None])
+    seen = torch.cat((torch.ones(B, T, P, dtype=torch.bool, device="cuda"), own), -1)[:, None].expand(B, H, T, P + C)
+    kk = torch.cat((kp.expand(B, -1, -1, -1), k), 2)
+    vv = torch.cat((vp.expand(B, -1, -1, -1), v), 2)
+    o, lse = shared_prefix_attention(q, kp, vp, k, v, lens=ln, return_lse=True, out=torch.full_like(q, math.nan))
+    _check_o(o, lse, _attend(q, _heads(kk, H), _heads(vv, H), seen, 1 / math.sqrt(D)))
+    q[B - 1, H - 1, T - 1] = math.nan
+    p, lse = shared_prefix_attention(q, kp, vp, k, v, lens=ln, return_lse=True)
+    assert p[B - 1, H - 1, T - 1].isnan().all() and lse[B - 1, H - 1, T - 1].isnan()
+    o[B - 1, H - 1, T - 1] = p[B - 1, H - 1, T - 1] = 0
+    assert torch.equal(o, p)
+
+
 def test_prefix_equals_cross_attention_without_own_keys():
     """No own keys: the prefix alone, the same for every sequence."""
     g = torch.Generator(device="cuda").manual_seed(12)
