@@ -482,3 +482,42 @@ def test_rows_around_the_output_stay():
         cross_attention(q, k, v, out=wide[:, :, 1:M + 1])
         assert (wide[:, :, 0] == 5).all() and (wide[:, :, M + 1] == 5).all()
         assert torch.equal(wide[:, :, 1:M + 1], cross_attention(q, k, v))
+
+
+@pytest.mark.parametrize("G,M", [(2, 3), (3, 40)])
+def test_offsets_beyond_32_bits(G, M):
+    """2 x 64 x (2^24 + 1000) elements: the last keys lie behind 2^31 of them.  All
+    other keys are zero (score 0, value 0), so 100 keys give the 64-bit result.
+    Gradients: P and dS are rounded once and off by the scores' E; Delta holds the
+    output's error (u + E) |dO| A."""
+    g = torch.Generator(device="cuda").manual_seed(G)
+    Hk, D, N, L = 2, 64, 2 ** 24 + 1000, 100
+    n = N - 30
+    k, v = (torch.zeros(1, Hk, N, D, dtype=BF, device="cuda") for _ in range(2))
+    for t in (k, v):
+        t[:, :, N - L:] = _rand((1, Hk, L, D), BF, g)
+        t[:, :, n:] = math.nan
+    q, do = _rand((1, Hk * G, M, D), BF, g, 8.0), _rand((1, Hk * G, M, D), BF, g)
+    ln = torch.tensor([n], device="cuda")
+    rest = torch.empty_like(q)
+    o, lse = cross_attention(q, k, v, k_lens=ln, return_lse=True, o_rest=rest)
+    kk, vv = _heads(k[:, :, N - L:n], Hk * G).double(), _heads(v[:, :, N - L:n], Hk * G).double()
+    s = q.double() @ kk.transpose(-1, -2) / 8
+    rl = torch.cat((s, torch.full_like(s[..., :1], math.log(N - L))), -1).logsumexp(-1)
+    p = (s - rl.unsqueeze(-1)).exp()
+    ro, A = p @ vv, p @ vv.abs()
+    _check_o(o, lse, (ro, rl / math.log(2), A, p))
+    dq, dk, dv = cross_attention_backward(q, k, v, o, lse, do, k_lens=ln, o_rest=rest)
+    assert not dk[:, :, n:].any() and not dv[:, :, n:].any() and not dk[:, :, ::4096].isnan().any()
+    d, u = do.double(), _u(BF)
+
+    def group(x):
+        return x.view(1, Hk, G, *x.shape[2:]).sum(2)
+
+    ds = p * (d @ vv.transpose(-1, -2) - (d * ro).sum(-1, keepdim=True))
+    da = p * (d.abs() @ vv.abs().transpose(-1, -2) + (d.abs() * A).sum(-1, keepdim=True)) * (u + 2 * E)
+    for got, ref, bound in ((dv, group(p.transpose(-1, -2) @ d), group(p.transpose(-1, -2) @ d.abs()) * (u + E)),
+                            (dk, group(ds.transpose(-1, -2) @ q.double() / 8),
+                             group(da.transpose(-1, -2) @ q.double().abs() / 8))):
+        off = (got[:, :, N - L:n].double() - ref).abs()
+        assert (off <= bound + u * ref.abs() * (1 + 2.0 ** -7) + 2.0 ** -24).all()
