@@ -35,8 +35,8 @@
 // Bound: 4 rows keys D flops against the tensor rate and, row by row, the 16
 // exponentials a clock of an SM (as many cycles as the products at D = 128);
 // with few rows the bytes of K and V.  Measured: 37 heads x 1024 rows x 16,384
-// keys x 128 265 us (1,200 TF/s), D = 64 222 us; 16 heads x 4096 rows x 16,384
-// keys 494 us (256 items over 148 SMs); 256 rows x 8 heads x 32,768 shared keys
+// keys x 128 255 us (1,247 TF/s), D = 64 215 us; 16 heads x 4096 rows x 16,384
+// keys 482 us (256 items over 148 SMs); 256 rows x 8 heads x 32,768 shared keys
 // 46 us, of which 27 us are steps.
 //
 // Keys behind a sequence's length take no part: their scores are replaced, and
@@ -45,6 +45,7 @@
 #include <cudaTypedefs.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "dense.h"
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
             return mx * p.scale_log2;
           };
           uint32_t pr[64];
-          auto exps = [&](bool mixed) {
+          auto exps = [&](auto cut) {  // cut: some keys of the tile are masked
             // a row that has seen nothing yet keeps m = -inf: its exponentials are 2^(-inf - 0) = 0
             const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
             float sum = 0.f;
@@ -503,36 +504,36 @@ __global__ void __launch_bounds__(kThreadsD, 1)
               uint32_t (&v)[32] = buf[ch & 1];
               uint32_t pp[16];
               if (ch < 3) tmem_ld32(s_base + (ch + 1) * 32, buf[(ch + 1) & 1]);
-              if (mask) {
+              if constexpr (decltype(cut)::value) {
 #pragma unroll
                 for (int k = 0; k < 32; ++k)
                   if (ch * 32 + k >= valid) v[k] = __float_as_uint(-INFINITY);
               }
-              sum += mixed ? exp_block_mixed<32, BF16>(v, pp, p.scale_log2, neg_m)
-                           : exp_block<32, BF16>(v, pp, p.scale_log2, neg_m);
+              sum += exp_block<32, BF16>(v, pp, p.scale_log2, neg_m);
 #pragma unroll
               for (int k = 0; k < 16; ++k) pr[ch * 16 + k] = pp[k];
               if (ch < 3) tmem_wait_ld32(buf[(ch + 1) & 1]);
             }
             return sum;
           };
-          // the reference point is the max of the row's first seen tile, and
-          // moves only when a tile's sum passes the slack (softmax.cuh)
+          // The reference point is the max of the row's first seen tile, and
+          // moves only when a tile's sum passes the slack (softmax.cuh): a score
+          // any amount above it gives inf.  (On the special function unit alone,
+          // and whole tiles without the masking: 37 heads x 1024 rows x 16,384 keys
+          // take 255 us at D = 128, 215 at 64; a quarter of the exponentials on the
+          // FMA pipe, clamped to give inf there too, 267 and 229; the masking in
+          // every tile 256 and 238.)
           if (__any_sync(0xffffffffu, m_run == -INFINITY && valid > 0)) {
             const float mx = tile_max();
             if (m_run == -INFINITY) m_run = mx;
           }
-          float ls;
-          if (mask || __any_sync(0xffffffffu, m_run == -INFINITY))
-            ls = exps(false);
-          else
-            ls = exps(true);
+          float ls = mask ? exps(std::true_type{}) : exps(std::false_type{});
           if (__any_sync(0xffffffffu, !(ls <= ref_slack<BF16>()))) {
             const float m_new = fmaxf(m_run, tile_max());
             const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m_run - m_new);
             l_run *= alpha;
             m_run = m_new;
-            ls = exps(false);
+            ls = exps(std::true_type{});
             if (i > 0) {
 #pragma unroll
               for (int ch = 0; ch < D / 32; ++ch) {

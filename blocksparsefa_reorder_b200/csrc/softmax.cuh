@@ -99,7 +99,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// 2^x of two values on the FMA pipe, for x below 128: x = n + f with n the
+// 2^x of two values on the FMA pipe, for x below 128 only (from 128.5 on n
+// wraps into the sign): the gradient's x = s - lse is at most 0 but for rounding;
+// a forward pass, whose reference point a later score may pass by any amount,
+// must not use it.  x = n + f with n the
 // nearest integer (adding 1.5 2^23 leaves n in the low bits of the sum), 2^f
 // by the degree-4 polynomial of least relative error on [-1/2, 1/2] (2.6e-6,
 // fitted by Remez exchange; its mean error is 1.4e-8), 2^n from n's bits in
@@ -121,41 +124,6 @@ __device__ __forceinline__ uint64_t ex2_fma_x2(uint64_t x) {
   float t0, t1;
   f32x2_unpack(t, t0, t1);
   return f32x2_mul(p, f32x2_pack(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
-}
-
-// exp_block with a quarter of the exponentials on the FMA pipe.
-template <int BN, bool BF16>
-__device__ __forceinline__ float exp_block_mixed(const uint32_t (&sr)[BN], uint32_t (&pr)[BN / 2], float scale_log2,
-                                                 float neg_m) {
-  const uint64_t sc2 = f32x2_pack(scale_log2, scale_log2);
-  const uint64_t nm2 = f32x2_pack(neg_m, neg_m);
-  uint64_t a01 = f32x2_pack(0.f, 0.f), a23 = a01;
-#pragma unroll
-  for (int i = 0; i < BN / 2; i += 2) {
-    const uint64_t x01 = f32x2_fma(f32x2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sc2, nm2);
-    const uint64_t x23 =
-        f32x2_fma(f32x2_pack(__uint_as_float(sr[2 * i + 2]), __uint_as_float(sr[2 * i + 3])), sc2, nm2);
-    float x0, x1, p0, p1;
-    f32x2_unpack(x01, x0, x1);
-    const uint64_t p01 = f32x2_pack(ex2_approx(x0), ex2_approx(x1));
-    uint64_t p23;
-    if (i % 4 == 2) {
-      p23 = ex2_fma_x2(x23);
-    } else {
-      f32x2_unpack(x23, x0, x1);
-      p23 = f32x2_pack(ex2_approx(x0), ex2_approx(x1));
-    }
-    a01 = f32x2_add(a01, p01);
-    a23 = f32x2_add(a23, p23);
-    f32x2_unpack(p01, p0, p1);
-    pr[i] = pack2<BF16>(p0, p1);
-    f32x2_unpack(p23, p0, p1);
-    pr[i + 1] = pack2<BF16>(p0, p1);
-  }
-  float s0, s1, s2, s3;
-  f32x2_unpack(a01, s0, s1);
-  f32x2_unpack(a23, s2, s3);
-  return (s0 + s2) + (s1 + s3);
 }
 
 // One block of the row's online softmax.  sr: raw scores (keys past the end

@@ -137,6 +137,68 @@ def test_cross_growing_scores(dtype, M):
     assert ((lse.double() - rl).abs() <= 2.0 ** -9 + 2.0 ** -23 * rl.abs()).all()
 
 
+GAPS = (100, 129, 130, 140, 150, 200, 256, 290, 300, 384, 400)
+
+
+def _far_keys(heads, N, tile, D, dtype, g):
+    """One strong key a head in 128-key tile `tile`, at each of 8 neighbouring
+    columns and each gap in turn: with q = e_0 and sm_scale = ln 2 it scores its
+    gap in log2 units, all others 0."""
+    k = torch.zeros(heads, N, D, dtype=dtype, device="cuda")
+    at = torch.tensor([tile * 128 + 40 + i % 8 for i in range(heads)], device="cuda")
+    gap = torch.tensor([float(GAPS[i // 8 % len(GAPS)]) for i in range(heads)], device="cuda")
+    k[torch.arange(heads, device="cuda"), at, 0] = gap.to(dtype)  # (8 bits hold each of them)
+    return k, _rand((heads, N, D), dtype, g), at, gap
+
+
+def _check_far(o, lse, v, at, gap):
+    """The strong key takes the whole weight: the others hold 2^-100 of it each.
+    Its score is off by four roundings (scale, scale log2 e, product, lse)."""
+    own = v[torch.arange(v.shape[0], device="cuda"), at].view(1, -1, 1, v.shape[-1]).expand_as(o)
+    assert torch.equal(o, own)
+    assert ((lse - gap.view(1, -1, 1)).abs() <= 4 * 2.0 ** -24 * 400).all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, HF), (64, BF), (128, HF), (128, BF)])
+@pytest.mark.parametrize("tile", [2, 3])
+@pytest.mark.parametrize("M", [32, 128, 256, 300])
+def test_cross_one_key_far_above_the_first(M, tile, D, dtype):
+    """A score far above the row's first keys, in a later tile of either stream, at
+    whichever column: its exponential passes the range of the first reference
+    point, which has to move."""
+    g = torch.Generator(device="cuda").manual_seed(M + D)
+    heads = 8 * len(GAPS)
+    k, v, at, gap = _far_keys(heads, 640, tile, D, dtype, g)
+    q = torch.zeros(1, heads, M, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    o, lse = cross_attention(q, k[None], v[None], sm_scale=math.log(2), return_lse=True, check_errors=True)
+    _check_far(o, lse, v, at, gap)
+    # two heads alone: the keys are split over the SMs
+    for h in (6, 55):
+        a, al = cross_attention(q[:, h:h + 1], k[None, h:h + 1], v[None, h:h + 1], sm_scale=math.log(2), return_lse=True)
+        _check_far(a, al, v[h:h + 1], at[h:h + 1], gap[h:h + 1])
+    # its gradient: P is 1 at that key, so that dv there is the sum of dout (fp32, rounded once) and dS is rounding alone
+    do = _rand(q.shape, dtype, g)
+    dq, dk, dv = cross_attention_backward(q, k[None], v[None], o, lse, do, sm_scale=math.log(2))
+    ref = do.double().sum(2)
+    got = dv[0, torch.arange(heads, device="cuda"), at].double()[None]
+    assert ((got - ref).abs() <= (_u(dtype) * 1.01) * ref.abs() + (2.0 ** -11 + _u(dtype)) * do.double().abs().sum(2)).all()
+    assert dq.isfinite().all() and dk.isfinite().all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, HF), (64, BF), (128, HF), (128, BF)])
+@pytest.mark.parametrize("B,T", [(32, 1), (130, 1), (40, 7)])
+def test_prefix_one_key_far_above_the_first(B, T, D, dtype):
+    g = torch.Generator(device="cuda").manual_seed(B + D)
+    heads = 8 * len(GAPS)
+    kp, vp, at, gap = _far_keys(heads, 768, 3, D, dtype, g)
+    q = torch.zeros(B, heads, T, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    k, v = torch.zeros(B, heads, T + 2, D, dtype=dtype, device="cuda"), _rand((B, heads, T + 2, D), dtype, g)
+    o, lse = shared_prefix_attention(q, kp, vp, k, v, sm_scale=math.log(2), return_lse=True, check_errors=True)
+    _check_far(o, lse, vp, at, gap)
+
+
 def test_cross_layouts_and_expanded_batch():
     """[B, N, H, D] memory, a slice of a wider projection, k / v shared by the
     batch (expanded) and by the heads, an output view."""
