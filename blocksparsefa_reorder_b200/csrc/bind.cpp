@@ -6,7 +6,6 @@
 //
 // Wrong types raise TypeError, wrong values ValueError, a refusal by the C ABI
 // BsaError, as in the package's other entry points.
-#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -14,6 +13,8 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <array>
 #include <cmath>
 #include <limits>
 
@@ -88,10 +89,114 @@ Tensor rows(const Tensor& g) {
 
 Tensor contiguous_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 
+// Memory of a strided tensor: runs of `run` bytes from `base` on, repeated over
+// n dimensions (strides in bytes, ascending).
+struct Extent {
+  explicit Extent(const Tensor& t)
+      : base(reinterpret_cast<intptr_t>(t.data_ptr())), run(static_cast<int64_t>(t.element_size())) {
+    for (int64_t i = 0; i < t.dim() && n < kDims; ++i)
+      if (t.size(i) > 1) dims[n++] = {t.stride(i) * static_cast<int64_t>(t.element_size()), t.size(i)};
+    std::sort(dims.begin(), dims.begin() + n);
+    int inner = 0;
+    while (inner < n && dims[inner].first == run) run *= dims[inner++].second;
+    std::copy(dims.begin() + inner, dims.begin() + n, dims.begin());
+    n -= inner;
+    end = base + run;
+    for (int i = 0; i < n; ++i) end += dims[i].first * (dims[i].second - 1);
+  }
+  static constexpr int kDims = 5;
+  intptr_t base, end;
+  int64_t run;
+  int n = 0;
+  std::array<std::pair<int64_t, int64_t>, kDims> dims;  // stride, size
+};
+
+// Whether a sum at + sum d_i s_i, each d_i within its range, lies between -below
+// and above (exclusive): largest stride first, so that what the smaller ones can
+// still reach leaves a candidate or two for each d_i where the strides nest.
+struct StridedSum {
+  struct Term {
+    int64_t s, lo, hi;
+  };
+  std::array<Term, 2 * Extent::kDims> terms;
+  int n = 0;
+  int64_t below, above;
+  bool moved_only = false;  // not with every d_i zero
+  int budget = 1 << 16;     // (overlapping strides without end: taken as met)
+  std::array<int64_t, 2 * Extent::kDims + 1> least, most;  // of the terms from i on
+
+  void add(int64_t s, int64_t lo, int64_t hi) {
+    for (int i = 0; i < n; ++i)
+      if (terms[i].s == s) {
+        terms[i].lo += lo, terms[i].hi += hi;
+        return;
+      }
+    terms[n++] = {s, lo, hi};
+  }
+  bool hits(int64_t at) {
+    std::sort(terms.begin(), terms.begin() + n, [](const Term& a, const Term& b) { return a.s > b.s; });
+    least[n] = most[n] = 0;
+    for (int i = n - 1; i >= 0; --i)
+      least[i] = least[i + 1] + terms[i].s * terms[i].lo, most[i] = most[i + 1] + terms[i].s * terms[i].hi;
+    return from(0, at, false);
+  }
+  bool from(int i, int64_t at, bool moved) {
+    if (at + least[i] >= above || at + most[i] <= -below) return false;
+    if (--budget < 0) return true;
+    if (i == n) return moved || !moved_only;
+    const Term& t = terms[i];
+    if (t.s == 0) return from(i + 1, at, moved || t.hi > t.lo);
+    // (the first candidate may miss by the division's rounding, which the test above sees)
+    const int64_t lo = std::max(t.lo, (-below - at - most[i + 1]) / t.s - 1);
+    const int64_t hi = std::min(t.hi, (above - at - least[i + 1]) / t.s + 1);
+    for (int64_t d = lo; d <= hi; ++d)
+      if (from(i + 1, at + d * t.s, moved || d != 0)) return true;
+    return false;
+  }
+};
+
+// Whether two elements of a tensor share memory.
+bool rows_overlap(const Tensor& t) {
+  if (!t.numel()) return false;
+  const Extent x(t);
+  int64_t reach = x.run;
+  bool nested = true;
+  for (int i = 0; i < x.n; ++i) {
+    if (i && x.dims[i].first == x.dims[i - 1].first) return true;  // (1, 0) and (0, 1) are one place
+    nested = nested && x.dims[i].first >= reach;
+    reach += x.dims[i].first * (x.dims[i].second - 1);
+  }
+  if (nested) return false;
+  StridedSum sum;
+  sum.below = sum.above = x.run;
+  sum.moved_only = true;
+  for (int i = 0; i < x.n; ++i) sum.add(x.dims[i].first, 1 - x.dims[i].second, x.dims[i].second - 1);
+  return sum.hits(0);
+}
+
+enum class Overlap { kNone, kSame, kSome };
+
+// What memory two tensors share (kSame: element for element).  PyTorch's own test
+// does not answer for views that are not dense, as those of a fused projection or
+// of a key cache are.
+Overlap overlap_of(const Tensor& a, const Tensor& b) {
+  if (!a.numel() || !b.numel() || a.device() != b.device()) return Overlap::kNone;
+  const Extent x(a), y(b);
+  if (x.end <= y.base || y.end <= x.base) return Overlap::kNone;
+  bool same = x.base == y.base && a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes();
+  for (int64_t i = 0; same && i < a.dim(); ++i) same = a.size(i) == 1 || a.stride(i) == b.stride(i);
+  if (same) return Overlap::kSame;
+  StridedSum sum;
+  sum.below = x.run, sum.above = y.run;
+  for (int i = 0; i < x.n; ++i) sum.add(x.dims[i].first, 0, x.dims[i].second - 1);
+  for (int i = 0; i < y.n; ++i) sum.add(y.dims[i].first, 1 - y.dims[i].second, 0);
+  return sum.hits(x.base - y.base) ? Overlap::kSome : Overlap::kNone;
+}
+
 // A tensor of the caller's that the call writes: as in PyTorch's own out=
 // arguments its rows lie apart, and autograd learns that it changed.
 void written(const Tensor& t, const char* name) {
-  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name, " must not be expanded: its rows overlap");
+  TORCH_CHECK_VALUE(!rows_overlap(t), name, " must not be expanded or overlap itself: every row is written");
   TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), name,
                     " requires a gradient: writing it is not differentiable");
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -105,12 +210,12 @@ Tensor output(const OptTensor& out, const Tensor& x, const char* name) {
   return *out;
 }
 
-// An output over memory that is read (`same`: it may be that very tensor).
-void apart(const OptTensor& out, const Tensor& x, const char* name, bool same = false) {
-  if (!out || !x.numel()) return;
-  const auto s = at::get_overlap_status(*out, x);
-  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Partial && (same || s != at::MemOverlapStatus::Full), name,
-                    " overlaps an input");
+// Refuses an output over other memory of the call, which blocks still read (or
+// write) when others write it; `same`: it may be that very tensor.
+void apart(const OptTensor& out, const OptTensor& x, const char* name, const char* other, bool same = false) {
+  if (!out || !x) return;
+  const Overlap o = overlap_of(*out, *x);
+  TORCH_CHECK_VALUE(o == Overlap::kNone || (same && o == Overlap::kSame), name, " overlaps ", other);
 }
 
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
@@ -222,16 +327,20 @@ std::tuple<OptTensor, OptTensor> rope_forward(const RopeIn& in, const OptTensor&
                                               const OptTensor& err) {
   bsa_rope_args a = rope_args(in);
   OptTensor oq, ok;
-  if (in.q) {
-    apart(q_out, *in.q, "q_out", true);
-    if (in.k) apart(q_out, *in.k, "q_out");
-    oq = output(q_out, *in.q, "q_out"), a.q_out = t4(*oq, "q_out");
+  const OptTensor* outs[] = {&q_out, &k_out};
+  const char* names[] = {"q_out", "k_out"};
+  for (int i = 0; i < 2; ++i) {
+    apart(*outs[i], in.q, names[i], "q", i == 0);
+    apart(*outs[i], in.k, names[i], "k", i == 1);
+    apart(*outs[i], in.q_weight, names[i], "q_weight");
+    apart(*outs[i], in.k_weight, names[i], "k_weight");
+    apart(*outs[i], in.positions, names[i], "positions");
+    apart(*outs[i], in.cos, names[i], "cos");
+    apart(*outs[i], in.sin, names[i], "sin");
   }
-  if (in.k) {
-    apart(k_out, *in.k, "k_out", true);
-    if (in.q) apart(k_out, *in.q, "k_out");
-    ok = output(k_out, *in.k, "k_out"), a.k_out = t4(*ok, "k_out");
-  }
+  apart(q_out, k_out, "q_out", "k_out");
+  if (in.q) oq = output(q_out, *in.q, "q_out"), a.q_out = t4(*oq, "q_out");
+  if (in.k) ok = output(k_out, *in.k, "k_out"), a.k_out = t4(*ok, "k_out");
   if (rope_empty(a)) return {oq, ok};
   const Tensor& x = in.q ? *in.q : *in.k;
   a.err_flag = flag(err);
@@ -392,6 +501,19 @@ OptTensor lse_output(bool want, const OptTensor& out, const Tensor& q) {
   return want ? OptTensor(at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat))) : OptTensor();
 }
 
+// The caller's outputs lie apart from each other and from what the call reads.
+void attention_outputs(const OptTensor& out, const OptTensor& lse_out, const OptTensor& o_rest,
+                       std::initializer_list<std::pair<const Tensor&, const char*>> inputs, const OptTensor& lens,
+                       const char* lens_name) {
+  const std::pair<const OptTensor&, const char*> outs[] = {{out, "out"}, {lse_out, "lse_out"}, {o_rest, "o_rest"}};
+  for (int i = 0; i < 3; ++i) {
+    if (!outs[i].first) continue;
+    for (const auto& x : inputs) apart(outs[i].first, x.first, outs[i].second, x.second);
+    apart(outs[i].first, lens, outs[i].second, lens_name);
+    for (int j = 0; j < i; ++j) apart(outs[i].first, outs[j].first, outs[i].second, outs[j].second);
+  }
+}
+
 template <typename Args>
 void launch(const Args& a, int (*query)(const Args*, size_t*), int (*call)(const Args*, void*, size_t, void*),
             const Tensor& q, const char* name) {
@@ -422,11 +544,10 @@ std::tuple<Tensor, OptTensor> cross_forward(const Tensor& q_, const Tensor& k_, 
   bsa_cross_args a{};
   a.lens_dtype = lens_dtype(k_lens, q_, "k_lens");
   a.sm_scale = scale_of(sm_scale, q_.size(3));
-  for (const Tensor* t : {&q_, &k_, &v_}) apart(out, *t, "out");
+  attention_outputs(out, lse_out, o_rest, {{q_, "q"}, {k_, "k"}, {v_, "v"}}, k_lens, "k_lens");
   const Tensor o = output(out, q_, "out");
   const OptTensor lse = lse_output(return_lse, lse_out, q_);
   if (o_rest) {
-    for (const Tensor* t : {&q_, &k_, &v_, &o}) apart(o_rest, *t, "o_rest");
     output(o_rest, q_, "o_rest");
     TORCH_CHECK_VALUE(o_rest->strides() == o.strides(), "o_rest must be laid out as the output");
     a.o_rest = o_rest->data_ptr();
@@ -526,7 +647,7 @@ std::tuple<Tensor, OptTensor> prefix_forward(const Tensor& q_, const Tensor& kp_
   bsa_prefix_args a{};
   a.lens_dtype = lens_dtype(lens, q_, "lens");
   a.sm_scale = scale_of(sm_scale, q_.size(3));
-  for (const Tensor* t : {&q_, &kp_, &vp_, &k_, &v_}) apart(out, *t, "out");
+  attention_outputs(out, lse_out, {}, {{q_, "q"}, {kp_, "k_prefix"}, {vp_, "v_prefix"}, {k_, "k"}, {v_, "v"}}, lens, "lens");
   const Tensor o = output(out, q_, "out");
   const OptTensor lse = lse_output(return_lse, lse_out, q_);
   if (q_.numel() == 0) return {o, lse};
@@ -576,4 +697,7 @@ PYBIND11_MODULE(_bsattn_torch, m) {
   m.def("cross_attention_backward", &cross_backward, Release());
   m.def("cross_attention_autograd", &cross_autograd, Release());
   m.def("shared_prefix_attention", &prefix_forward, Release());
+  // the memory tests behind the refusals of outputs, which work on any strided tensor
+  m.def("overlap", [](const Tensor& a, const Tensor& b) { return static_cast<int>(overlap_of(a, b)); });
+  m.def("rows_overlap", &rows_overlap);
 }

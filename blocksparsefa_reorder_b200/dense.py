@@ -47,6 +47,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, k_lens
     return_lse: also return the row log-sum-exp in log2 units, ``[B, H, M]``.
     o_rest: optional tensor laid out as the output that receives what rounding
     left of the result (fp32 result - o), for :func:`cross_attention_backward`.
+    Outputs given (out, lse_out, o_rest) that overlap each other or an input are
+    refused.
     """
     err = _error_word(check_errors, q)
     o, lse = _lib.native().cross_attention(q, k, v, k_lens, sm_scale, return_lse, out, lse_out, o_rest, err)
@@ -98,6 +100,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     finite (earlier ones take it times 0).  Lengths outside [0, C] are clamped,
     and an error with ``check_errors`` (which synchronises).
     return_lse: also return the row log-sum-exp in log2 units, ``[B, H, T]``.
+    Outputs given that overlap each other or an input are refused.
     """
     err = _error_word(check_errors, q)
     o, lse = _lib.native().shared_prefix_attention(q, k_prefix, v_prefix, k, v, lens, sm_scale, return_lse, out, lse_out,

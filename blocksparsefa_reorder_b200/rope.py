@@ -56,7 +56,8 @@ def qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], q_weight:
     0 .. N - 1.  A position outside the tables gives a NaN row, and an error
     with ``check_errors`` (which synchronises).
     out: optional ``(q_out, k_out)``, e.g. views of a key cache or the inputs
-    themselves.  Returns ``(q_out, k_out)``; sums, norm and rotation are fp32,
+    themselves; outputs that overlap each other or another input are refused.
+    Returns ``(q_out, k_out)``; sums, norm and rotation are fp32,
     rounded once.
     """
     q_out, k_out = out if out is not None else (None, None)

@@ -151,6 +151,134 @@ def test_rope_table_angles():
     assert (cos[-1].double() - ang.cos()).abs().max() <= 2 ** -24 and (sin[-1].double() - ang.sin()).abs().max() <= 2 ** -24
 
 
+def _places(t):
+    """The byte addresses of every element, by enumeration."""
+    at = torch.full(t.shape, t.data_ptr(), dtype=torch.int64)
+    for i, (n, s) in enumerate(zip(t.shape, t.stride())):
+        at += (torch.arange(n) * s * t.element_size()).view([n if j == i else 1 for j in range(t.dim())])
+    return at.flatten().tolist()
+
+
+def test_overlap_of_strided_views_matches_enumeration():
+    """Random strided views of one buffer, dense, nested, interleaved and
+    overlapping: the answers are those of their elements' addresses."""
+    import random
+
+    rng = random.Random(5)
+    buf = torch.zeros(4000, dtype=torch.float16)
+    seen = {0: 0, 1: 0, 2: 0}
+    rows = {True: 0, False: 0}
+
+    def view():
+        t = buf
+        size = [rng.choice((1, 2, 3, 4, 5)) for _ in range(4)]
+        size[3] = rng.choice((1, 2, 4, 8))
+        if rng.random() < 0.7:  # nested, in some order, with gaps
+            order, stride, reach = rng.sample(range(3), 3), [0, 0, 0, 1], size[3]
+            for i in order:
+                stride[i] = reach + rng.choice((0, 0, 4, 8))
+                reach = stride[i] * (size[i] - 1) + reach
+        else:
+            stride = [rng.choice((0, 1, 2, 4, 6, 8, 12, 20, 64, 100)) for _ in range(3)] + [1]
+        span = sum(s * (n - 1) for s, n in zip(stride, size)) + 1
+        at = rng.randrange(0, min(400, buf.numel() - span), 4)
+        if rng.random() < 0.2 and all(s % 2 == 0 for s in stride[:3]) and size[3] > 1:
+            t, size, stride = buf.view(torch.float32), size[:3] + [size[3] // 2], [s // 2 for s in stride[:3]] + [1]
+            at //= 2
+        return t.as_strided(size, stride, at)
+
+    native = _lib.native()
+    last = view()
+    for _ in range(4000):
+        a, b = view(), last if rng.random() < 0.5 else view()
+        if rng.random() < 0.1:
+            b = a.as_strided(a.shape, a.stride(), a.storage_offset())
+        pa, pb = _places(a), _places(b)
+        assert native.rows_overlap(a) == (len(set(pa)) < len(pa))
+        rows[len(set(pa)) < len(pa)] += 1
+        ba = {x + i for x in pa for i in range(a.element_size())}
+        bb = {x + i for x in pb for i in range(b.element_size())}
+        want = 1 if pa == pb and a.dtype == b.dtype and a.shape == b.shape else 2 if ba & bb else 0
+        got = native.overlap(a, b)
+        # (equal places with other strides, all of them stride 0 or of one element, are told as overlapping)
+        assert got == want or (want == 1 and got == 2 and a.stride() != b.stride()), (a.shape, a.stride(), b.shape, b.stride())
+        assert native.overlap(b, a) == got
+        seen[got] += 1
+        last = b
+    assert min(seen.values()) > 100 and min(rows.values()) > 100
+
+
+def test_overlap_of_the_operators_layouts():
+    """Views of a fused projection and of a key cache: neighbours lie apart."""
+    native = _lib.native()
+    qkv = torch.zeros(2, 5, 12 * 64, dtype=torch.float16)
+
+    def heads(h0, n):
+        return qkv[..., h0 * 64:(h0 + n) * 64].view(2, 5, n, 64).transpose(1, 2)
+
+    q, k, v = heads(0, 4), heads(4, 4), heads(8, 4)
+    assert [native.overlap(q, k), native.overlap(k, v), native.overlap(q, heads(0, 4))] == [0, 0, 1]
+    assert native.overlap(q, heads(1, 4)) == native.overlap(k, heads(3, 2)) == 2
+    assert native.overlap(q, q[:, :, 1:]) == 2 and native.overlap(q[:, :, :2], q[:, :, 2:]) == 0
+    cache = torch.zeros(2, 4, 100, 64, dtype=torch.float16)
+    assert native.overlap(cache[:, :, 7:9], cache[:, :, 9:20]) == 0 and native.overlap(cache[:, :, 7:9], cache[:, :, 8:9]) == 2
+    assert not any(native.rows_overlap(t) for t in (q, k, cache[:, :, 3:7], cache[:, :, :0], q[:, :, :1]))
+    assert native.rows_overlap(q[:1].expand(2, -1, -1, -1)) and native.rows_overlap(cache.as_strided((1, 4, 5, 64), (0, 32, 128, 1)))
+
+
+@pytest.mark.gpu
+def test_outputs_over_other_memory_of_the_call(dev):
+    """Outputs that are views of the buffers the call reads or of each other:
+    refused where they meet, taken where they lie apart."""
+    h = torch.float16
+    qkv = torch.randn(2, 3, 14 * 64, dtype=h, device=dev)
+
+    def heads(h0, n):
+        return qkv[..., h0 * 64:(h0 + n) * 64].view(2, 3, n, 64).transpose(1, 2)
+
+    q, k = heads(0, 4), heads(4, 2)
+    lse = torch.zeros(2 * 4 * 3 + 8, device=dev)
+    ln = torch.tensor([1, 2], device=dev, dtype=torch.int32)
+    both = torch.zeros(2, 3, 6 * 64, dtype=h, device=dev)
+    new = [both[..., a * 64:(a + n) * 64].view(2, 3, n, 64).transpose(1, 2) for a, n in ((0, 4), (2, 2), (4, 2))]
+    kl = torch.zeros(2 * 4 * 3 * 64, dtype=h, device=dev)
+    own_lens = kl.view(torch.int32)[:2]
+    tab = torch.ones(48, 32, device=dev)
+    bad = [
+        lambda: lib.qk_norm_rope(q, None, cos=tab, sin=tab, out=(tab.view(h)[:24].view(2, 4, 3, 64), None)),
+        lambda: lib.qk_norm_rope(q, k, out=(heads(1, 4), None)),
+        lambda: lib.qk_norm_rope(q, None, out=(heads(1, 4), None)),
+        lambda: lib.qk_norm_rope(q, k, out=(None, heads(3, 2))),
+        lambda: lib.qk_norm_rope(q, k, out=(new[0], new[1])),
+        lambda: lib.qk_norm_rope(q, None, out=(both.as_strided((2, 4, 3, 64), (3 * 384, 32, 384, 1)), None)),
+        lambda: lib.cross_attention(q, k, k, out=heads(2, 4)),
+        lambda: lib.cross_attention(q, heads(6, 2), heads(8, 2), out=heads(8, 4)),
+        lambda: lib.cross_attention(q, k, k, out=heads(0, 4)),
+        lambda: lib.cross_attention(q, k, k, out=heads(6, 4), o_rest=heads(8, 4)),
+        lambda: lib.cross_attention(q, k, k, k_lens=own_lens, out=kl.view(2, 4, 3, 64)),
+        lambda: lib.cross_attention(q, k, k, lse_out=qkv.view(-1).view(torch.float32)[:24].view(2, 4, 3)),
+        lambda: lib.cross_attention(q, k, k, out=kl.view(2, 4, 3, 64), lse_out=kl.view(torch.float32)[-24:].view(2, 4, 3)),
+        lambda: lib.shared_prefix_attention(q, k[0], k[0], k, k, out=heads(3, 4)),
+        lambda: lib.shared_prefix_attention(q, k[0], k[0], k, k, lse_out=qkv.view(-1).view(torch.float32)[:24].view(2, 4, 3)),
+        lambda: lib.shared_prefix_attention(q, k[0], k[0], k, k, lens=own_lens, out=kl.view(2, 4, 3, 64)),
+    ]
+    before = qkv.clone()
+    for call in bad:
+        with pytest.raises(ValueError, match="overlap|wrong shape"):
+            call()
+    torch.cuda.synchronize()
+    assert torch.equal(qkv, before)
+    # in place, and into other heads of the same buffer
+    ref = lib.qk_norm_rope(q, k)
+    o = lib.cross_attention(q, k, heads(6, 2), k_lens=ln)
+    got = lib.cross_attention(q, k, heads(6, 2), k_lens=ln, out=heads(8, 4), lse_out=lse[:24].view(2, 4, 3))
+    assert torch.equal(got, o)
+    lib.qk_norm_rope(q, k, out=(heads(8, 4), heads(12, 2)))
+    assert torch.equal(heads(8, 4), ref[0]) and torch.equal(heads(12, 2), ref[1])
+    lib.qk_norm_rope(q, k, out=(heads(0, 4), heads(4, 2)))
+    assert torch.equal(q, ref[0]) and torch.equal(k, ref[1]) and torch.equal(heads(6, 2), before[..., 384:512].view(2, 3, 2, 64).transpose(1, 2))
+
+
 @pytest.mark.gpu
 def test_python_refusals_on_the_gpu(dev):
     h = torch.float16
