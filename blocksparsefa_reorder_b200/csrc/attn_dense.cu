@@ -292,8 +292,10 @@ __global__ void __launch_bounds__(kThreadsD, 1)
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ producer
       tma_prefetch_desc(&tmQ0);
-      tma_prefetch_desc(&tmK0);
-      tma_prefetch_desc(&tmV0);
+      if (p.part[0].keys > 0) {  // (without keys there is no map of them)
+        tma_prefetch_desc(&tmK0);
+        tma_prefetch_desc(&tmV0);
+      }
       int c = 0;      // loads so far
       int nq = 0;     // non-empty items so far
       bool ok = true;

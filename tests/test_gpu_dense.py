@@ -451,6 +451,39 @@ def test_prefix_partial_results_on_both_sides_of_the_joining_rule(B, H, Hk, T, P
     assert torch.equal(o, p)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("B,T,C", [(3, 40, 50), (2, 20, 20), (30, 1, 9), (2, 140, 0), (3, 1, 0), (60, 1, 0)])
+def test_prefix_of_no_keys(B, T, C, D, dtype):
+    """An empty prefix in front of own keys, or of none: more rows than the
+    few-rows kernel takes (T or the batch), and fewer."""
+    g = torch.Generator(device="cuda").manual_seed(B + T + C)
+    H, Hk = 4, 2
+    q, k, v = _rand((B, H, T, D), dtype, g), _rand((B, Hk, C, D), dtype, g), _rand((B, Hk, C, D), dtype, g)
+    none = torch.empty(Hk, 0, D, dtype=dtype, device="cuda")
+    o, lse = shared_prefix_attention(q, none, none, k, v, return_lse=True, out=torch.full_like(q, math.nan),
+                                     check_errors=True)
+    if C == 0:
+        assert (o == 0).all() and (lse == -math.inf).all()
+        return
+    t = torch.arange(T, device="cuda")
+    seen = (torch.arange(C, device="cuda") < (C - (T - 1 - t)[:, None])).expand(B, H, T, C)
+    _check_o(o, lse, _attend(q, _heads(k, H), _heads(v, H), seen, 1 / math.sqrt(D)))
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, HF)])
+@pytest.mark.parametrize("B,H,Hk,M", [(2, 4, 2, 100), (1, 3, 3, 300), (2, 8, 1, 5), (1, 2, 2, 1)])
+def test_cross_of_no_keys(B, H, Hk, M, D, dtype):
+    g = torch.Generator(device="cuda").manual_seed(M)
+    q, do = _rand((B, H, M, D), dtype, g), _rand((B, H, M, D), dtype, g)
+    none = torch.empty(B, Hk, 0, D, dtype=dtype, device="cuda")
+    for lens in (None, torch.zeros(B, dtype=torch.int32, device="cuda")):
+        o, lse = cross_attention(q, none, none, k_lens=lens, return_lse=True, out=torch.full_like(q, math.nan),
+                                 check_errors=True)
+        assert (o == 0).all() and (lse == -math.inf).all()
+        dq, dk, dv = cross_attention_backward(q, none, none, o, lse, do, k_lens=lens, check_errors=True)
+        assert (dq == 0).all() and dk.shape == dv.shape == none.shape
+
+
 def test_prefix_equals_cross_attention_without_own_keys():
     """No own keys: the prefix alone, the same for every sequence."""
     g = torch.Generator(device="cuda").manual_seed(12)
