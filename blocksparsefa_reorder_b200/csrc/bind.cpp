@@ -10,13 +10,14 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/engine.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/extension.h>
 
 #include <algorithm>
 #include <array>
 #include <cmath>
 #include <limits>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/bsattn_b200.h"
 
@@ -392,26 +393,35 @@ void once(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its gradient has none (create_graph)");
 }
 
-// A captured backward pass that hands a gradient to a leaf whose node an eager
-// graph, still alive, has made on the default stream: that stream cannot join
-// the capture, which the engine's attempt invalidates (the process may end with
-// it).  Refused here, before it gets there.
-void capturable_leaves() {
+// A captured backward pass that reaches a node made on the default stream: a
+// leaf's, which an eager graph, still alive, holds, or one of an eager graph
+// behind this operator's inputs.  That stream cannot join the capture, which the
+// engine's attempt invalidates (the process may end with it).  Refused here,
+// before it gets there, through whatever lies between (views of a fused
+// projection, casts).
+void capturable_graph() {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  const auto node = torch::autograd::get_current_node();
+  const auto self = torch::autograd::get_current_node();
   const auto* info = torch::autograd::get_current_graph_task_exec_info();
-  if (!node) return;
-  for (const auto& edge : node->next_edges()) {
-    auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
-    if (!leaf) continue;
-    if (info && !info->empty()) {
-      const auto it = info->find(leaf);
-      if (it == info->end() || !it->second.should_execute()) continue;
+  if (!self) return;
+  std::unordered_set<torch::autograd::Node*> seen;
+  std::vector<torch::autograd::Node*> open{self.get()};
+  while (!open.empty()) {
+    auto* node = open.back();
+    open.pop_back();
+    for (const auto& edge : node->next_edges()) {
+      auto* next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (info && !info->empty()) {
+        const auto it = info->find(next);
+        if (it == info->end() || !it->second.should_execute()) continue;
+      }
+      const auto s = next->stream();
+      TORCH_CHECK(!s || *s != c10::cuda::getDefaultCUDAStream(s->device_index()).unwrap(),
+                  "a captured backward pass cannot reach a leaf (or another node) that an eager graph on the default "
+                  "stream still holds: free that graph first, or run it on the capture's stream");
+      open.push_back(next);
     }
-    const auto s = leaf->stream();
-    TORCH_CHECK(!s || *s != c10::cuda::getDefaultCUDAStream(s->device_index()).unwrap(),
-                "a captured backward pass cannot reach a leaf that an eager graph on the default stream still holds: free "
-                "that graph first, or run it on the capture's stream");
   }
 }
 
@@ -433,7 +443,7 @@ struct RopeFn : torch::autograd::Function<RopeFn> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     once("qk_norm_rope");
-    capturable_leaves();
+    capturable_graph();
     const auto s = ctx->get_saved_variables();
     // a side that is absent, or whose output took no part, has no gradient
     const Tensor gq = s[0].defined() ? g[0] : Tensor(), gk = s[1].defined() ? g[s[0].defined() ? 1 : 0] : Tensor();
@@ -613,7 +623,7 @@ struct CrossFn : torch::autograd::Function<CrossFn> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     once("cross_attention");
-    capturable_leaves();
+    capturable_graph();
     const auto s = ctx->get_saved_variables();
     const auto scale = ctx->saved_data["scale"].toOptional<double>();
     auto [dq, dk, dv] = cross_backward(s[0], s[1], s[2], s[3], s[4], rows(g[0]), if_defined(s[6]), scale, if_defined(s[5]), {});

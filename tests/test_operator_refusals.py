@@ -385,3 +385,44 @@ def test_captured_backward_and_an_eager_graph_of_the_same_leaves(dev, op):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(q.grad, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["cross", "rope"])
+@pytest.mark.parametrize("between", ["views", "products", "eager"])
+def test_captured_backward_reaches_the_leaf_through_other_nodes(dev, op, between):
+    """The same where views or products lie between the leaf and the operator, and
+    where the eager graph itself is what the captured backward pass would run."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    w = torch.randn(1, 7, 6 * 64, device=dev, dtype=torch.float16, generator=g).requires_grad_(True)
+
+    def inputs():
+        x = w * 0.5 if between == "products" else w
+        return [x[..., a * 64:(a + n) * 64].view(1, 7, n, 64).transpose(1, 2) for a, n in ((0, 2), (2, 2), (4, 2))]
+
+    def forward(qkv=None):
+        q, k, v = qkv or inputs()
+        return lib.cross_attention_autograd(q, k, v) if op == "cross" else lib.qk_norm_rope_autograd(q, k)[1]
+
+    def capture(step):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        return graph, out
+
+    want, = torch.autograd.grad(forward().sum(), w)
+    held = inputs() if between == "eager" else None
+    eager = None if held else forward()
+    for step in (lambda: forward(held).sum().backward(), lambda: torch.autograd.grad(forward(held).sum(), w)):
+        with pytest.raises(RuntimeError, match="captured backward pass"):
+            capture(step)
+        torch.cuda.synchronize()
+    del eager, held
+    graph, (got,) = capture(lambda: torch.autograd.grad(forward().sum(), w))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and w.grad is None
+    graph, _ = capture(lambda: forward().sum().backward())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(w.grad, want)
