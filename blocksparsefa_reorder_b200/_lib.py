@@ -90,6 +90,7 @@ PROTOS = {
     "bsa_cross_fwd_workspace_bytes": ([_vp, ctypes.POINTER(_sz)], ctypes.c_int),
     "bsa_cross_fwd": ([_vp, _vp, _sz, _vp], ctypes.c_int),
     "bsa_cross_bwd": ([_vp, _vp], ctypes.c_int),
+    "bsa_cross_bwd_scaled": ([_vp, _vp, _vp], ctypes.c_int),
     "bsa_prefix_fwd_workspace_bytes": ([_vp, ctypes.POINTER(_sz)], ctypes.c_int),
     "bsa_prefix_fwd": ([_vp, _vp, _sz, _vp], ctypes.c_int),
 }

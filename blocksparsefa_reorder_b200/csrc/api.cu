@@ -308,7 +308,15 @@ extern "C" int bsa_cross_bwd(const bsa_cross_bwd_args* a, void* stream) {
   int rc = cross_bwd_validate(a);
   if (rc) return rc;
   if ((rc = check_device())) return rc;
-  return launch_cross_bwd(a, static_cast<cudaStream_t>(stream));
+  return launch_cross_bwd(a, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int bsa_cross_bwd_scaled(const bsa_cross_bwd_args* a, float* dout_max, void* stream) {
+  int rc = cross_bwd_validate(a);
+  if (rc) return rc;
+  if (!dout_max) return BSA_ERR_WORKSPACE;
+  if ((rc = check_device())) return rc;
+  return launch_cross_bwd(a, dout_max, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int bsa_prefix_fwd_workspace_bytes(const bsa_prefix_args* a, size_t* bytes) {

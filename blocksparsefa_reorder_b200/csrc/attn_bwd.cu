@@ -104,16 +104,22 @@ __device__ __forceinline__ void zero_row(uint8_t* row) {
 
 // Delta[b, h, n] = sum_d dO[n, d] * O[n, d] in fp32: each row read by D / 8
 // lanes with 16-byte loads (two rows per warp at D = 128, four at D = 64).
-// `rest` (optional, laid out as O) holds what O's rounding left.
+// `rest` (optional, laid out as O) holds what O's rounding left.  A group of
+// group_rows rows has blocks of its own, group_blocks of them, and dout_max
+// (optional) receives the largest |dO| of every block's rows.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(256) bwd_delta_kernel(const uint8_t* o, const uint8_t* rest, int64_t o_b, int64_t o_h, int64_t o_n,
                                                         const uint8_t* dout, int64_t d_b, int64_t d_h, int64_t d_n,
-                                                        float* delta, int B, int H, int N) {
+                                                        float* delta, int H, int N, int64_t group_rows, int group_blocks,
+                                                        float* dout_max) {
   constexpr int LPR = D / 8;  // lanes per row
   const int lane = threadIdx.x & 31;
-  const int64_t r = (static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * (32 / LPR) + lane / LPR;
-  const bool live = r < static_cast<int64_t>(B) * H * N;
-  float acc = 0.f;
+  const int group = static_cast<int>(blockIdx.x) / group_blocks;
+  const int block = static_cast<int>(blockIdx.x) - group * group_blocks;
+  const int64_t at_group = (static_cast<int64_t>(block) * 8 + (threadIdx.x >> 5)) * (32 / LPR) + lane / LPR;
+  const int64_t r = group * group_rows + at_group;
+  const bool live = at_group < group_rows;
+  float acc = 0.f, top = 0.f;
   if (live) {
     const int64_t bh = r / N, n = r - bh * N, b = bh / H, h = bh - b * H;
     const int d = (lane % LPR) * 8;
@@ -133,11 +139,22 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const uint8_t* o, const 
         o0 += r0, o1 += r1;
       }
       acc = fmaf(o0, d0, fmaf(o1, d1, acc));
+      if (dout_max) top = fmaxf(top, fmaxf(fabsf(d0), fabsf(d1)));
     }
   }
 #pragma unroll
   for (int off = LPR / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
   if (live && lane % LPR == 0) delta[r] = acc;
+  if (!dout_max) return;
+  __shared__ uint32_t tops[8];
+  // (a float that is not negative orders as its bits do)
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if (lane == 0) tops[threadIdx.x >> 5] = bits;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const uint32_t all = __reduce_max_sync(0xffffffffu, lane < 8 ? tops[lane] : 0u);
+    if (lane == 0) dout_max[blockIdx.x] = __uint_as_float(all);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -570,16 +587,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
 }  // namespace
 
+int bwd_delta_rows(int D) { return 8 * (32 / (D / 8)); }
+
 int launch_bwd_delta(const bsa_tensor4d& o, const void* rest, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
-                     bool bf16, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(B) * H * N;
-  const int64_t rows_per_block = 8 * (32 / (D / 8));
-  const unsigned grid = static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block);
+                     bool bf16, cudaStream_t st, float* dout_max, int G) {
+  const int64_t rows = static_cast<int64_t>(B) * H * N, per = bwd_delta_rows(D);
+  const int64_t group_rows = dout_max ? static_cast<int64_t>(G) * N : rows;
+  const int64_t group_blocks = (group_rows + per - 1) / per, blocks = group_blocks * (rows / group_rows);
+  if (blocks > INT32_MAX) return BSA_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(blocks);
 #define BSA_DELTA_CASE(BF_, D_)                                                                                     \
   if (bf16 == BF_ && D == D_)                                                                                      \
     bwd_delta_kernel<BF_, D_><<<grid, 256, 0, st>>>(                                                               \
         static_cast<const uint8_t*>(o.data), static_cast<const uint8_t*>(rest), o.stride_b, o.stride_h, o.stride_n, \
-        static_cast<const uint8_t*>(dout.data), dout.stride_b, dout.stride_h, dout.stride_n, delta, B, H, N);
+        static_cast<const uint8_t*>(dout.data), dout.stride_b, dout.stride_h, dout.stride_n, delta, H, N,          \
+        group_rows, static_cast<int>(group_blocks), dout_max);
   BSA_DELTA_CASE(true, 128)
   BSA_DELTA_CASE(false, 128)
   BSA_DELTA_CASE(true, 64)

@@ -5,6 +5,12 @@
 //   dQ = sm_scale dS K,  dK = sm_scale sum_g dS^T Q,  dV = sum_g P^T dO
 // with Delta = rowsum(dO o O) and the sums over the query heads g of a key /
 // value head.  No atomics: every gradient row is written by one CTA.
+// fp16: dS of a long row is about dO / keys, below what fp16 resolves (2^-24)
+// already for dO of 2^-8.  So it is held times the power of two that brings the
+// largest |dO| of the rows summed up, found by the Delta kernel, into [4, 8) (dO of
+// N(0, 1): 1), which dQ and dK take off again in fp32.  (2 x 16 heads x 2048 x
+// 4096 x 128 in fp16 387 us, 386 without; 3 x 6 heads x 777 x 1531 x 64 40, 39 without.
+// One maximum a group by atomics, behind a memset: 394 and 50.)
 //
 // Bound by the tensor cores: dQ needs three products of a 128 x 128 tile (S,
 // dP, dS K), dK / dV four.  Both kernels keep them fed by the order in which
@@ -46,6 +52,9 @@ struct DBwdParams {
   float scale_log2, sm_scale;
   const float* lse;    // [B, H, M]
   const float* delta;  // [B, H, M]
+  // largest |dout| of every max_rows rows of a head group, [B, Hk, maxima], or null: dS as it is
+  const float* dout_max;
+  int max_rows, maxima;
   uint8_t *dq, *dk, *dv;
   int64_t dq_b, dq_h, dq_n, dk_b, dk_h, dk_n, dv_b, dv_h, dv_n;
   int32_t* err;
@@ -82,6 +91,13 @@ __device__ __forceinline__ bool query_of(const DBwdParams& p, int t, int rl, int
   m = (t - gi * p.nm) * p.mt + rl - q * p.mt;
   g = gi * p.gh + q;
   return q < p.gh && m < p.M;
+}
+
+// What dS is held times (see above) for a largest |dO| of the given bits; 1 where
+// it is zero or not finite.
+__device__ __forceinline__ float ds_scale(uint32_t bits) {
+  if (bits == 0u || bits >= 0x7F800000u) return 1.f;
+  return __uint_as_float((2 * 127 + 2 - (bits >> 23)) << 23);  // (an fp16 value is a normal fp32 one)
 }
 
 // -lse as the exponent's offset; a row without any weight (lse -inf) and a row
@@ -156,6 +172,13 @@ __device__ __forceinline__ void ex2_pair(uint64_t x, bool fma, float& p0, float&
     p0 = ex2_approx(x0);
     p1 = ex2_approx(x1);
   }
+}
+
+// dP - Delta of two columns, times what dS is held times (Delta has it in it).
+template <bool BF16>
+__device__ __forceinline__ uint64_t dp_minus(uint32_t dp0, uint32_t dp1, uint64_t held2, uint64_t neg_delta2) {
+  const uint64_t dp = f32x2_pack(__uint_as_float(dp0), __uint_as_float(dp1));
+  return BF16 ? f32x2_add(dp, neg_delta2) : f32x2_fma(dp, held2, neg_delta2);
 }
 
 // C (+)= A B^T of two 128 x D shared-memory tiles (K-major descriptors)
@@ -331,7 +354,12 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
       const float neg_lse = neg_lse_of(p, live, ri);
       const float dlt = live ? __ldg(&p.delta[ri]) : 0.f;
       const uint64_t sc2 = f32x2_pack(p.scale_log2, p.scale_log2), nl2 = f32x2_pack(neg_lse, neg_lse);
-      const uint64_t nd2 = f32x2_pack(-dlt, -dlt);
+      // (a row of dQ may have a scale of its own: the maximum of the rows around it)
+      float held = 1.f;
+      if (!BF16 && p.dout_max && live)
+        held = ds_scale(__ldg(reinterpret_cast<const uint32_t*>(p.dout_max) + static_cast<int64_t>(bh) * p.maxima +
+                              (static_cast<int64_t>(g) * p.M + m) / p.max_rows));
+      const uint64_t held2 = f32x2_pack(held, held), nd2 = f32x2_pack(-dlt * held, -dlt * held);
       bool ok = true;
       for (int j = 0; j < n; ++j) {
         const uint32_t s_col = (j & 1) * 128 + half * 64;
@@ -365,7 +393,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const uint64_t g = f32x2_add(f32x2_pack(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), nd2);
+            const uint64_t g = dp_minus<BF16>(dp[k], dp[k + 1], held2, nd2);
             float g0, g1;
             f32x2_unpack(g, g0, g1);
             ds[k / 2] = pack2<BF16>(pv[c * 32 + k] * g0, pv[c * 32 + k + 1] * g1);
@@ -391,7 +419,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
       ok = ok && wait_all(done, 0);
       if (ok) {
         tc_fence_after();
-        store_half_row<D, BF16>(lane_base + kDQ, half, p.sm_scale, orow, live, false);
+        store_half_row<D, BF16>(lane_base + kDQ, half, p.sm_scale / held, orow, live, false);
       }
     }
   }
@@ -570,13 +598,22 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
       }
     } else {
       const uint64_t sc2 = f32x2_pack(p.scale_log2, p.scale_log2);
-      // the first warpgroup stages -lse, the second -Delta, of the step's 128
+      float held = 1.f;
+      if (!BF16 && p.dout_max) {
+        const uint32_t* tops = reinterpret_cast<const uint32_t*>(p.dout_max) + static_cast<int64_t>(bh) * p.maxima;
+        uint32_t top = 0;
+#pragma unroll 8
+        for (int i = lane; i < p.maxima; i += 32) top = max(top, __ldg(tops + i));
+        held = ds_scale(__reduce_max_sync(0xffffffffu, top));
+      }
+      const uint64_t held2 = f32x2_pack(held, held);
+      // the first warpgroup stages -lse, the second -Delta (scaled), of the step's 128
       // query rows; the value of the next step is fetched a step ahead
       auto fetch = [&](int i) -> float {
         int g, m;
         const bool in = query_of(p, i, row, g, m);
         const int64_t at = (static_cast<int64_t>(b) * p.H + hk * p.G + g) * p.M + m;
-        return half == 0 ? neg_lse_of(p, in, at) : (in ? -__ldg(&p.delta[at]) : 0.f);
+        return half == 0 ? neg_lse_of(p, in, at) : (in ? -__ldg(&p.delta[at]) * held : 0.f);
       };
       float next = fetch(0);
       bool ok = true;
@@ -620,8 +657,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const float2 nd = *reinterpret_cast<const float2*>(db + c * 32 + k);
-            const uint64_t g =
-                f32x2_add(f32x2_pack(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), f32x2_pack(nd.x, nd.y));
+            const uint64_t g = dp_minus<BF16>(dp[k], dp[k + 1], held2, f32x2_pack(nd.x, nd.y));
             float g0, g1;
             f32x2_unpack(g, g0, g1);
             ds[k / 2] = pack2<BF16>(pv[c * 32 + k] * g0, pv[c * 32 + k + 1] * g1);
@@ -639,7 +675,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
         // keys past the length have no gradient
         const bool zero = krow >= len;
         store_half_row<D, BF16>(lane_base + 256, half, 1.f, vrow_out, live, zero);
-        store_half_row<D, BF16>(lane_base + 256 + D, half, p.sm_scale, krow_out, live, zero);
+        store_half_row<D, BF16>(lane_base + 256 + D, half, p.sm_scale / held, krow_out, live, zero);
       }
     }
   }
@@ -680,7 +716,7 @@ int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16
 }
 
 template <int D, bool BF16>
-int launch_t(const bsa_cross_bwd_args* a, cudaStream_t st) {
+int launch_t(const bsa_cross_bwd_args* a, float* dout_max, cudaStream_t st) {
   using C = DBwdCfg<D>;
   auto kern = dense_bwd_kernel<D, BF16>;
   static std::atomic<bool> ready[64] = {};
@@ -712,7 +748,8 @@ int launch_t(const bsa_cross_bwd_args* a, cudaStream_t st) {
     if ((r = map_of(&mk, a->k, a->B, a->Hk, a->N, D, BF16, &p.kb_mul))) return r;
     if ((r = map_of(&mv, a->v, a->B, a->Hk, a->N, D, BF16, &p.vb_mul))) return r;
   }
-  if ((r = launch_bwd_delta(a->o, a->o_rest, a->dout, a->delta, a->B, a->H, a->M, D, BF16, st))) return r;
+  if (BF16) dout_max = nullptr;
+  if ((r = launch_bwd_delta(a->o, a->o_rest, a->dout, a->delta, a->B, a->H, a->M, D, BF16, st, dout_max, G))) return r;
   p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.G = G, p.M = a->M, p.N = a->N;
   p.k_tiles = (a->N + 127) / 128;
   p.lens = a->k_lens;
@@ -721,6 +758,9 @@ int launch_t(const bsa_cross_bwd_args* a, cudaStream_t st) {
   p.sm_scale = a->sm_scale;
   p.lse = a->lse;
   p.delta = a->delta;
+  p.dout_max = dout_max;
+  p.max_rows = bwd_delta_rows(D);
+  p.maxima = static_cast<int>((static_cast<int64_t>(G) * a->M + p.max_rows - 1) / p.max_rows);
   p.dq = static_cast<uint8_t*>(a->dq.data), p.dq_b = a->dq.stride_b, p.dq_h = a->dq.stride_h, p.dq_n = a->dq.stride_n;
   p.dk = static_cast<uint8_t*>(a->dk.data), p.dk_b = a->dk.stride_b, p.dk_h = a->dk.stride_h, p.dk_n = a->dk.stride_n;
   p.dv = static_cast<uint8_t*>(a->dv.data), p.dv_b = a->dv.stride_b, p.dv_h = a->dv.stride_h, p.dv_n = a->dv.stride_n;
@@ -773,10 +813,10 @@ int cross_bwd_validate(const bsa_cross_bwd_args* a) {
   return BSA_OK;
 }
 
-int launch_cross_bwd(const bsa_cross_bwd_args* a, cudaStream_t st) {
+int launch_cross_bwd(const bsa_cross_bwd_args* a, float* dout_max, cudaStream_t st) {
   const bool bf = a->dtype == BSA_DTYPE_BF16;
-  if (a->D == 128) return bf ? launch_t<128, true>(a, st) : launch_t<128, false>(a, st);
-  return bf ? launch_t<64, true>(a, st) : launch_t<64, false>(a, st);
+  if (a->D == 128) return bf ? launch_t<128, true>(a, dout_max, st) : launch_t<128, false>(a, dout_max, st);
+  return bf ? launch_t<64, true>(a, dout_max, st) : launch_t<64, false>(a, dout_max, st);
 }
 
 }  // namespace bsa

@@ -598,17 +598,19 @@ std::tuple<Tensor, Tensor, Tensor> cross_backward(const Tensor& q_, const Tensor
   if (q_.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
   const Tensor q = spread(q_, true), k = spread(k_), v = spread(v_), dout = spread(dout_, true);
   const Tensor o = o_rest ? o_ : spread(o_, true);
-  const Tensor delta = at::empty(lse.sizes(), lse.options());
+  // Delta of every row, then the maxima of |dout|
+  const int64_t rows = lse.numel();
+  const Tensor work = at::empty({2 * rows}, lse.options());
   a.B = dim(q.size(0), "B"), a.H = dim(q.size(1), "H"), a.Hk = dim(k.size(1), "Hk"), a.M = dim(q.size(2), "M");
   a.N = dim(k.size(2), "N"), a.D = dim(q.size(3), "D"), a.dtype = dtype_of(q.scalar_type());
   a.q = t4(q, "q"), a.k = t4(k, "k"), a.v = t4(v, "v"), a.o = t4(o, "o"), a.dout = t4(dout, "dout");
   a.dq = t4(dq, "dq"), a.dk = t4(dk, "dk"), a.dv = t4(dv, "dv");
   a.k_lens = ptr(k_lens);
   a.lse = lse.data_ptr<float>();
-  a.delta = delta.data_ptr<float>();
+  a.delta = work.data_ptr<float>();
   a.err_flag = flag(err);
   const c10::cuda::CUDAGuard guard(q.device());
-  check(bsa_cross_bwd(&a, stream_of(q)), "bsa_cross_bwd");
+  check(bsa_cross_bwd_scaled(&a, a.delta + rows, stream_of(q)), "bsa_cross_bwd");
   return {dq, dk, dv};
 }
 

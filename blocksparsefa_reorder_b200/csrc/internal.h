@@ -35,9 +35,12 @@ int launch_attn_simt(const bsa_fwd_args* a, cudaStream_t st);
 // The backward kernels (attn_bwd.cu): Delta, dQ, dK / dV; arguments validated.
 int launch_attn_bwd(const bsa_bwd_args* a, cudaStream_t st);
 // Delta = rowsum(dout o (o + rest)) per query row, contiguous fp32 [B, H, N] (D 64
-// / 128); rest (optional, laid out as o): what o's rounding left.
+// / 128); rest (optional, laid out as o): what o's rounding left; dout_max
+// (optional): receives the largest |dout| of every bwd_delta_rows(D) rows of a group
+// of G heads, [B, H / G, ceil(G N / those rows)].
+int bwd_delta_rows(int D);
 int launch_bwd_delta(const bsa_tensor4d& o, const void* rest, const bsa_tensor4d& dout, float* delta, int B, int H, int N, int D,
-                     bool bf16, cudaStream_t st);
+                     bool bf16, cudaStream_t st, float* dout_max = nullptr, int G = 1);
 
 // tma_maps.cu: whether the tcgen05 path takes these arguments (bf16 / fp16,
 // D 64 or 128, BLOCK 64 or 128, 16-byte-aligned rows), and the 4-D TMA map
@@ -73,7 +76,7 @@ size_t prefix_workspace(const bsa_prefix_args* a);
 int launch_prefix(const bsa_prefix_args* a, void* workspace, cudaStream_t st);
 // attn_dense_bwd.cu: gradient of cross attention
 int cross_bwd_validate(const bsa_cross_bwd_args* a);
-int launch_cross_bwd(const bsa_cross_bwd_args* a, cudaStream_t st);
+int launch_cross_bwd(const bsa_cross_bwd_args* a, float* dout_max, cudaStream_t st);
 
 }  // namespace bsa
 

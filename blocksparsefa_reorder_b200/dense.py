@@ -67,7 +67,9 @@ def cross_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     zero behind ``k_lens[b]``; every gradient row is written by one CTA (no
     atomics, deterministic).  o_rest: the forward's, so that ``rowsum(dout o)``
     is formed from the unrounded output; without it o's rounding is in dq and dk
-    (over few keys as much of it as their own).
+    (over few keys as much of it as their own).  P and dS are rounded to the
+    inputs' type for the products, dS of fp16 inputs relative to the largest
+    output gradient of its key / value head.
     """
     err = _error_word(check_errors, q)
     g = _lib.native().cross_attention_backward(q, k, v, o, lse, dout, k_lens, sm_scale, o_rest, err)

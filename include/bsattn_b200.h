@@ -324,6 +324,13 @@ typedef struct bsa_cross_bwd_args {
   float sm_scale;
 } bsa_cross_bwd_args;
 BSA_API int bsa_cross_bwd(const bsa_cross_bwd_args* args, void* stream);
+/* The same with dS of fp16 tensors held relative to the largest |dout| of its
+ * batch entry and key / value head (scaled by the power of two that brings it into
+ * [4, 8), taken off dq and dk in fp32), so that small gradients keep their bits
+ * and large ones do not overflow.  bsa_cross_bwd rounds it as it is: there dout
+ * below 2^-8 or so loses bits of dq and dk over thousands of keys.  dout_max:
+ * workspace of delta's size (bf16: not used, but not NULL). */
+BSA_API int bsa_cross_bwd_scaled(const bsa_cross_bwd_args* args, float* dout_max, void* stream);
 
 /* Attention of a batch behind a shared prefix: T new tokens of each of B
  * sequences, q, o [B, H, T, D], over k_prefix, v_prefix [Hk, P, D] (stride_b

@@ -337,6 +337,64 @@ def test_cross_rounding_rest(M, N, G, dtype):
     assert all(((x.double() - r).abs() <= t).all() for x, r, t in zip(got, ref, bound))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,N,G,e", [(300, 4096, 2, -17), (40, 5000, 1, -12), (2000, 700, 1, -20), (130, 300, 3, 9),
+                                     (1, 9000, 1, -16)])
+def test_cross_gradient_of_small_and_large_output_gradients(M, N, G, e, D):
+    """fp16, dout around 2^e, a second sequence's at 2^0: dS is held relative to the
+    largest dout of its key / value head (which comes to lie in [4, 8)), so that it
+    is rounded by at most half of 2^-24 in that measure, or relatively by u.  The
+    result itself may be subnormal: half of 2^-24."""
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    B, Hk, u = 2, 2, _u(HF)
+    q, k, v = _rand((B, Hk * G, M, D), HF, g), _rand((B, Hk, N, D), HF, g), _rand((B, Hk, N, D), HF, g)
+    do = _rand(q.shape, HF, g)
+    do[0] = (do[0].float() * 2.0 ** e).to(HF)
+    ln = torch.tensor([N, N - 5], device="cuda")
+    rest, scale = torch.empty_like(q), 1 / math.sqrt(D)
+    o, lse = cross_attention(q, k, v, k_lens=ln, return_lse=True, o_rest=rest)
+    got = cross_attention_backward(q, k, v, o, lse, do, k_lens=ln, o_rest=rest, check_errors=True)
+    ro, _, A, p = _cross_ref(q, k, v, ln, scale)
+    gone = ~(torch.arange(N, device="cuda") < ln[:, None])[:, None, :, None]
+    kh, vh = (_heads(t.double().masked_fill(gone, 0), Hk * G) for t in (k, v))
+    d, qd = do.double(), q.double()
+    ds = p * (d @ vh.transpose(-1, -2) - (d * ro).sum(-1, keepdim=True))
+    # Delta from o + rest: P's and the scores' errors through A, and fp32 sums of D terms
+    e_delta = (d.abs() * ((u + E) * A + 2 * u * u * ro.abs())).sum(-1, keepdim=True)
+    sums = 2.0 ** -16 * (d.abs() @ vh.abs().transpose(-1, -2) + (d * ro).abs().sum(-1, keepdim=True))
+    top = do.double().abs().view(B, Hk, -1).amax(-1).log2().floor().exp2() / 4  # 1 where dout is N(0, 1)
+    quantum = top.repeat_interleave(G, 1)[..., None, None] * 2.0 ** -25
+    e_ds = (u + 4 * E) * ds.abs() + p * (e_delta + sums) + quantum
+    fold = lambda t: t.view(B, Hk, G, N, -1).sum(2)  # noqa: E731
+    ref = (scale * ds @ kh, fold(scale * ds.transpose(-1, -2) @ qd), fold(p.transpose(-1, -2) @ d))
+    # P is off by u and the scores' error, and by half of 2^-24 where it is subnormal
+    bound = (scale * e_ds @ kh.abs(), fold(scale * e_ds.transpose(-1, -2) @ qd.abs()),
+             fold(((u + 4 * E) * p + 2.0 ** -25).transpose(-1, -2) @ d.abs()))
+    for name, x, r, t in zip(("dq", "dk", "dv"), got, ref, bound):
+        assert x.isfinite().all(), name
+        off, t = (x.double() - r).abs(), t + u * r.abs() * 1.01 + 2.0 ** -25
+        assert (off <= t).all(), f"{name}: worst {(off / t).max().item():.2f}x, {(off > t).sum().item()} off"
+    again = cross_attention_backward(q, k, v, o, lse, do, k_lens=ln, o_rest=rest)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_cross_gradient_of_degenerate_output_gradients():
+    """All zero: zero gradients.  Infinite or NaN in one head: its own group's alone."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    q, k, v = _rand((1, 4, 140, 64), HF, g), _rand((1, 2, 200, 64), HF, g), _rand((1, 2, 200, 64), HF, g)
+    o, lse = cross_attention(q, k, v, return_lse=True)
+    assert all((x == 0).all() for x in cross_attention_backward(q, k, v, o, lse, torch.zeros_like(q)))
+    do = _rand(q.shape, HF, g, 2.0 ** -10)
+    want = cross_attention_backward(q, k, v, o, lse, do)
+    for bad in (math.inf, math.nan):
+        spoilt = do.clone()
+        spoilt[0, 1, 7, 3] = bad
+        got = cross_attention_backward(q, k, v, o, lse, spoilt)
+        assert not got[0][0, 1, 7].isfinite().any() and not got[2][0, 0].isfinite().all()
+        assert torch.equal(got[0][:, 2:], want[0][:, 2:]) and torch.equal(got[1][:, 1], want[1][:, 1])
+        assert torch.equal(got[2][:, 1], want[2][:, 1])
+
+
 def test_cross_gradient_matches_differences():
     """Central differences of the 64-bit definition along random directions."""
     g = torch.Generator(device="cuda").manual_seed(8)

@@ -71,6 +71,12 @@ def test_cross_backward_abi(kw, status):
     assert _lib.lib().bsa_cross_bwd(_bwd(**kw), None) == status
 
 
+def test_scaled_cross_backward_abi():
+    assert _lib.lib().bsa_cross_bwd_scaled(_bwd(dtype=F32), P, None) == 3
+    assert _lib.lib().bsa_cross_bwd_scaled(_bwd(), None, None) == 9
+    assert _lib.lib().bsa_cross_bwd_scaled(None, P, None) == 1
+
+
 def _prefix(B=2, H=4, Hk=2, T=1, Pn=100, C=10, D=64, dtype=F16, lens_dtype=0, lens=0, scale=0.125, **ts):
     vals = [x for n in ("q", "o", "kp", "vp", "k", "v") for x in ts.get(n, t4())]
     return PREFIX.pack(B, H, Hk, T, Pn, C, D, dtype, lens_dtype, *vals, lens, 0, 0, scale)
