@@ -10,7 +10,9 @@
 // largest |dO| of the rows summed up, found by the Delta kernel, into [4, 8) (dO of
 // N(0, 1): 1), which dQ and dK take off again in fp32.  (2 x 16 heads x 2048 x
 // 4096 x 128 in fp16 387 us, 386 without; 3 x 6 heads x 777 x 1531 x 64 40, 39 without.
-// One maximum a group by atomics, behind a memset: 394 and 50.)
+// One maximum a group by atomics, behind a memset: 394 and 50.)  The same for P on
+// its way to dV: at most 1 but for rounding, it is held times 2^12, so that a key
+// of little weight in every row keeps its sum (an exponent's offset; no cost).
 //
 // Bound by the tensor cores: dQ needs three products of a 128 x 128 tile (S,
 // dP, dS K), dK / dV four.  Both kernels keep them fed by the order in which
@@ -606,14 +608,17 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
         for (int i = lane; i < p.maxima; i += 32) top = max(top, __ldg(tops + i));
         held = ds_scale(__reduce_max_sync(0xffffffffu, top));
       }
-      const uint64_t held2 = f32x2_pack(held, held);
+      // P comes with 2^kHeldP in it, which dS takes off with dP - Delta
+      constexpr float kHeldP = BF16 ? 0.f : 12.f, kTakeP = BF16 ? 1.f : 1.f / 4096.f;
+      const float held_p = held * kTakeP;
+      const uint64_t held2 = f32x2_pack(held_p, held_p);
       // the first warpgroup stages -lse, the second -Delta (scaled), of the step's 128
       // query rows; the value of the next step is fetched a step ahead
       auto fetch = [&](int i) -> float {
         int g, m;
         const bool in = query_of(p, i, row, g, m);
         const int64_t at = (static_cast<int64_t>(b) * p.H + hk * p.G + g) * p.M + m;
-        return half == 0 ? neg_lse_of(p, in, at) : (in ? -__ldg(&p.delta[at]) * held : 0.f);
+        return half == 0 ? neg_lse_of(p, in, at) + kHeldP : (in ? -__ldg(&p.delta[at]) * held_p : 0.f);
       };
       float next = fetch(0);
       bool ok = true;
@@ -674,7 +679,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
         tc_fence_after();
         // keys past the length have no gradient
         const bool zero = krow >= len;
-        store_half_row<D, BF16>(lane_base + 256, half, 1.f, vrow_out, live, zero);
+        store_half_row<D, BF16>(lane_base + 256, half, kTakeP, vrow_out, live, zero);
         store_half_row<D, BF16>(lane_base + 256 + D, half, p.sm_scale / held, krow_out, live, zero);
       }
     }

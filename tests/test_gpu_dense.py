@@ -378,6 +378,29 @@ def test_cross_gradient_of_small_and_large_output_gradients(M, N, G, e, D):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("D,dtype", [(64, HF), (128, HF), (64, BF)])
+def test_cross_gradient_of_keys_of_little_weight(D, dtype):
+    """Keys whose weight is about 2^-26 in every row get their sum over many rows:
+    fp16's P is held times 2^12, so it is rounded by at most half of 2^-36."""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    M, N = 2000, 4096
+    q = _rand((1, 2, M, D), dtype, g, 0.1)
+    q[..., 0] = 1
+    k, v = _rand((1, 2, N, D), dtype, g, 0.1), _rand((1, 2, N, D), dtype, g)
+    k[..., 0] = -10.0
+    k[:, :, ::64, 0] = 10.0
+    do = (1 + _rand(q.shape, dtype, g, 0.1).abs()).to(dtype)
+    scale = math.log(2)
+    o, lse = cross_attention(q, k, v, sm_scale=scale, return_lse=True)
+    dv = cross_attention_backward(q, k, v, o, lse, do, sm_scale=scale)[2]
+    p = _cross_ref(q, k, v, None, scale)[3]
+    u, d = _u(dtype), do.double()
+    ref = p.transpose(-1, -2) @ d
+    tiny = 2.0 ** -37 if dtype == HF else 0
+    bound = ((u + 4 * E) * p + tiny).transpose(-1, -2) @ d + u * ref * 1.01 + (2.0 ** -25 if dtype == HF else 0)
+    assert ((dv.double() - ref).abs() <= bound).all(), ((dv.double() - ref).abs() / bound).max()
+
+
 def test_cross_gradient_of_degenerate_output_gradients():
     """All zero: zero gradients.  Infinite or NaN in one head: its own group's alone."""
     g = torch.Generator(device="cuda").manual_seed(21)
