@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
                 if (ch * 32 + k >= valid) v[k] = __float_as_uint(-INFINITY);
             }
           };
-          auto tile_max = [&]() {
+          auto reference = [&]() {  // from the tile's max
             float mx = -INFINITY;
 #pragma unroll
             for (int ch = 0; ch < 4; ++ch) {
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
               load(ch, v);
               mx = fmaxf(mx, row_max<32>(v));
             }
-            return mx * p.scale_log2;
+            return mx * p.scale_log2 - ref_below<BF16>();
           };
           uint32_t pr[64];
           auto exps = [&](auto cut) {  // cut: some keys of the tile are masked
@@ -526,12 +526,12 @@ __global__ void __launch_bounds__(kThreadsD, 1)
           // FMA pipe, clamped to give inf there too, 267 and 229; the masking in
           // every tile 256 and 238.)
           if (__any_sync(0xffffffffu, m_run == -INFINITY && valid > 0)) {
-            const float mx = tile_max();
+            const float mx = reference();
             if (m_run == -INFINITY) m_run = mx;
           }
           float ls = mask ? exps(std::true_type{}) : exps(std::false_type{});
           if (__any_sync(0xffffffffu, !(ls <= ref_slack<BF16>()))) {
-            const float m_new = fmaxf(m_run, tile_max());
+            const float m_new = fmaxf(m_run, reference());
             const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m_run - m_new);
             l_run *= alpha;
             m_run = m_new;

@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "dense.h"
 #include "internal.h"
+#include "softmax.cuh"
 
 namespace bsa {
 
@@ -184,14 +185,14 @@ __global__ void __launch_bounds__(kThreadsF, NR == 1 ? 2 : 1) attn_few_kernel(co
             over = over || (x[t] - m_run[n][e] > kSlack);
           }
           if (__any_sync(0xffffffffu, over)) {
-            // a new reference point: the block's max of each row, over the 8 lanes that hold its keys
+            // a new reference point, from the block's max of each row, over the 8 lanes that hold its keys
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float mx = fmaxf(x[e], x[2 + e]);
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              mx = fmaxf(mx, m_run[n][e]);
+              mx = fmaxf(mx - ref_below<BF16>(), m_run[n][e]);
               const float alpha = mx == -INFINITY ? 1.f : ex2_approx(m_run[n][e] - mx);
               m_run[n][e] = mx;
               l_run[n][e] *= alpha;

@@ -199,6 +199,32 @@ def test_prefix_one_key_far_above_the_first(B, T, D, dtype):
     _check_far(o, lse, vp, at, gap)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,N", [(1, 300), (3, 9000), (40, 200), (128, 1500), (300, 257)])
+def test_cross_one_heavy_key_and_many_light_ones(M, N, D):
+    """fp16: one key holds nearly all of the weight, with small values; the others
+    have about 2^-25 each.  The reference point lies 2^4 below the maximum, so that
+    a weight is off by u, or by half of 2^-24 / 2^4 where it is subnormal."""
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    q = torch.zeros(1, 2, M, D, dtype=HF, device="cuda")
+    q[..., 0] = 1
+    k, v = torch.zeros(1, 2, N, D, dtype=HF, device="cuda"), 1 + _rand((1, 2, N, D), HF, g).abs()
+    k[..., 0] = -25 - torch.rand(1, 2, N, generator=g, device="cuda").to(HF)
+    for h, at in enumerate((0, N - 1)):
+        k[0, h, at, 0] = 0
+        v[0, h, at] *= 2.0 ** -14
+    o, lse = cross_attention(q, k, v, sm_scale=math.log(2), return_lse=True)
+    ro, rl, A, _ = _cross_ref(q, k, v, None, math.log(2))
+    u = _u(HF)
+    bound = (u + E) * A + u * ro.abs() * 1.01 + 2.0 ** -25 + 2.0 ** -29 * _heads(v, 2).double().sum(2, keepdim=True)
+    off = (o.double() - ro).abs()
+    assert (off <= bound).all(), (off / bound).max()
+    assert ((lse.double() - rl).abs() <= 2 * E).all()
+    none = torch.empty(1, 2, 0, D, dtype=HF, device="cuda")
+    o = shared_prefix_attention(q, k[0], v[0], none, none, sm_scale=math.log(2))
+    assert ((o.double() - ro).abs() <= bound).all()
+
+
 def test_cross_layouts_and_expanded_batch():
     """[B, N, H, D] memory, a slice of a wider projection, k / v shared by the
     batch (expanded) and by the heads, an output view."""
