@@ -56,6 +56,8 @@ def parse_args(argv: Optional[list] = None):
                 "include; use --mode B200")
     if ns.block_size not in (64, 128):
         p.error("--block-size must be 64 or 128 for the B200 kernels.")
+    if ns.qk_norm_rope and (ns.head_dim % 8 or ns.head_dim > 256):
+        p.error("--qk-norm-rope takes a --head-dim that is a multiple of 8, at most 256.")
     return Args(matrix_mtx=ns.matrix_mtx, block_size=ns.block_size, head_dim=ns.head_dim, num_heads=ns.num_heads,
                 row_reorder=ns.row_reorder, col_reorder=ns.col_reorder, mode=ns.mode, qk_norm_rope=ns.qk_norm_rope)
 

@@ -150,6 +150,20 @@ def test_python_refuses_cpu_tensors():
         lib.rope_table(8, 63, device="cpu")
 
 
+@pytest.mark.parametrize("dim,ok", [("60", False), ("264", False), ("8", True), ("256", True)])
+def test_command_line_refuses_head_dims_the_norm_and_rotation_does_not_take(dim, ok, capsys):
+    from blocksparsefa_reorder_b200.__main__ import parse_args
+
+    args = ["pattern.mtx", "--head-dim", dim]
+    assert parse_args(args).head_dim == int(dim)
+    if ok:
+        assert parse_args([*args, "--qk-norm-rope"]).qk_norm_rope
+        return
+    with pytest.raises(SystemExit):
+        parse_args([*args, "--qk-norm-rope"])
+    assert "multiple of 8" in capsys.readouterr().err
+
+
 def test_rope_table_angles():
     cos, sin = lib.rope_table(200001, 64, base=1e6, device="cpu")
     assert cos.shape == sin.shape == (200001, 32) and cos.dtype == torch.float32
