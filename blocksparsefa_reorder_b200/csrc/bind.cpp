@@ -102,11 +102,9 @@ struct Extent {
     while (inner < n && dims[inner].first == run) run *= dims[inner++].second;
     std::copy(dims.begin() + inner, dims.begin() + n, dims.begin());
     n -= inner;
-    end = base + run;
-    for (int i = 0; i < n; ++i) end += dims[i].first * (dims[i].second - 1);
   }
   static constexpr int kDims = 5;
-  intptr_t base, end;
+  intptr_t base;
   int64_t run;
   int n = 0;
   std::array<std::pair<int64_t, int64_t>, kDims> dims;  // stride, size
@@ -156,6 +154,13 @@ struct StridedSum {
   }
 };
 
+// The end of a tensor's memory.
+intptr_t end_of(const Tensor& t) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += t.stride(i) * (t.size(i) - 1);
+  return reinterpret_cast<intptr_t>(t.data_ptr()) + (last + 1) * static_cast<int64_t>(t.element_size());
+}
+
 // Whether two elements of a tensor share memory.
 bool rows_overlap(const Tensor& t) {
   if (!t.numel()) return false;
@@ -182,8 +187,9 @@ enum class Overlap { kNone, kSame, kSome };
 // of a key cache are.
 Overlap overlap_of(const Tensor& a, const Tensor& b) {
   if (!a.numel() || !b.numel() || a.device() != b.device()) return Overlap::kNone;
+  if (end_of(a) <= reinterpret_cast<intptr_t>(b.data_ptr()) || end_of(b) <= reinterpret_cast<intptr_t>(a.data_ptr()))
+    return Overlap::kNone;
   const Extent x(a), y(b);
-  if (x.end <= y.base || y.end <= x.base) return Overlap::kNone;
   bool same = x.base == y.base && a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes();
   for (int64_t i = 0; same && i < a.dim(); ++i) same = a.size(i) == 1 || a.stride(i) == b.stride(i);
   if (same) return Overlap::kSame;
@@ -213,10 +219,12 @@ Tensor output(const OptTensor& out, const Tensor& x, const char* name) {
 
 // Refuses an output over other memory of the call, which blocks still read (or
 // write) when others write it; `same`: it may be that very tensor.
-void apart(const OptTensor& out, const OptTensor& x, const char* name, const char* other, bool same = false) {
-  if (!out || !x) return;
-  const Overlap o = overlap_of(*out, *x);
+void apart(const Tensor& out, const Tensor& x, const char* name, const char* other, bool same = false) {
+  const Overlap o = overlap_of(out, x);
   TORCH_CHECK_VALUE(o == Overlap::kNone || (same && o == Overlap::kSame), name, " overlaps ", other);
+}
+void apart(const OptTensor& out, const OptTensor& x, const char* name, const char* other, bool same = false) {
+  if (out && x) apart(*out, *x, name, other, same);
 }
 
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
@@ -331,6 +339,7 @@ std::tuple<OptTensor, OptTensor> rope_forward(const RopeIn& in, const OptTensor&
   const OptTensor* outs[] = {&q_out, &k_out};
   const char* names[] = {"q_out", "k_out"};
   for (int i = 0; i < 2; ++i) {
+    if (!*outs[i]) continue;
     apart(*outs[i], in.q, names[i], "q", i == 0);
     apart(*outs[i], in.k, names[i], "k", i == 1);
     apart(*outs[i], in.q_weight, names[i], "q_weight");
@@ -518,7 +527,7 @@ void attention_outputs(const OptTensor& out, const OptTensor& lse_out, const Opt
   const std::pair<const OptTensor&, const char*> outs[] = {{out, "out"}, {lse_out, "lse_out"}, {o_rest, "o_rest"}};
   for (int i = 0; i < 3; ++i) {
     if (!outs[i].first) continue;
-    for (const auto& x : inputs) apart(outs[i].first, x.first, outs[i].second, x.second);
+    for (const auto& x : inputs) apart(*outs[i].first, x.first, outs[i].second, x.second);
     apart(outs[i].first, lens, outs[i].second, lens_name);
     for (int j = 0; j < i; ++j) apart(outs[i].first, outs[j].first, outs[i].second, outs[j].second);
   }
