@@ -207,19 +207,6 @@ struct Ring {
   }
 };
 
-// The values loaded by tcgen05.ld may be used from here on: they pass through
-// the wait, so that no use of them can move ahead of it.
-__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
-}
-
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreadsD, 1)
     attn_dense_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant__ CUtensorMap tmK0,
@@ -344,9 +331,10 @@ __global__ void __launch_bounds__(kThreadsD, 1)
       if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, nullptr, nullptr, p.wait_ns);
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issue
-      // One thread, with nothing between the MMAs but adding to descriptors:
-      // a group of 8 occupies the tensor cores for 512 cycles, and they queue
-      // about half of one, so an issuer slower than that leaves them idle.
+      // The whole warp, one elected lane, with nothing between the MMAs but
+      // adding to descriptors: a group of 8 occupies the tensor cores for 512
+      // cycles, and they queue about half of one, so an issuer slower than that
+      // leaves them idle.
       constexpr uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128, false, false);
       constexpr uint32_t idesc_pv = make_idesc_f16(BF16, 128, D, false, true);
       const uint64_t qd = make_sw128_desc(smem_u32(sQ), 16, 1024);
@@ -992,18 +980,6 @@ DensePlan plan_of(const DenseCall& c) {
   return pl;
 }
 
-// A tensor map's batch dimension of 1 where the batch shares one copy.
-int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul, int rows = 128, int heads = 1,
-           int batch = 1) {
-  const bool one = B == 1 || t.stride_b == 0;
-  *mul = one ? 0 : 1;
-  // a dimension of length 1 has no stride of its own
-  if (one) t.stride_b = 8;
-  if (H == 1) t.stride_h = 8;
-  if (N == 1) t.stride_n = 8;
-  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, rows, heads, batch);
-}
-
 cudaLaunchConfig_t config(unsigned grid, int threads, int smem, cudaStream_t st, cudaLaunchAttribute* attr) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1140,11 +1116,6 @@ int launch_all(const DenseCall& c, const DensePlan& pl, uint8_t* ws, cudaStream_
     BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16, 1>, j));
   }
   return BSA_OK;
-}
-
-bool aligned(const bsa_tensor4d& t, int B, int H, int N) {
-  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && (B == 1 || t.stride_b * 2 % 16 == 0) &&
-         (H == 1 || t.stride_h * 2 % 16 == 0) && (N == 1 || t.stride_n * 2 % 16 == 0);
 }
 
 // Checks common to both operators; the sources' keys may be zero.

@@ -15,15 +15,15 @@
 // of little weight in every row keeps its sum (an exponent's offset; no cost).
 //
 // Bound by the tensor cores: dQ needs three products of a 128 x 128 tile (S,
-// dP, dS K), dK / dV four.  Both kernels keep them fed by the order in which
-// the MMA warp issues:
+// dP, dS K), dK / dV four.  Both kinds of CTA keep them fed by the order in
+// which the MMA warp issues:
 //  * dQ: S two tiles ahead in two buffers; once dS_j is written, dP_j+1, then
 //    dQ += dS_j K_j, then S_j+2.  The exponentials of tile j+1 run under dP_j+1;
 //  * dK / dV: P_i^T ready -> dV += P_i^T dO_i, S_i+1^T (over P_i); dS_i^T ready
 //    -> dK += dS_i^T Q_i, dP_i+1^T (over dS_i).  The exponentials of step i+1
 //    run under the last two.
-// Roles of a CTA: warp 0 TMA producer, warp 1 MMA issue (one thread each),
-// warpgroups 1 and 2 elementwise: a row is shared by two threads, one of each warpgroup, with 64
+// Roles of a CTA: warp 0 TMA producer (one thread), warp 1 MMA issue (the whole
+// warp, one elected lane: see attn_dense.cu), warpgroups 1 and 2 elementwise: a row is shared by two threads, one of each warpgroup, with 64
 // of the tile's 128 columns, so that each 16-bit result lies over columns its
 // own thread has read (columns 0-31 and 64-95 of the score buffer).
 // Measured: 2 x 16 heads x 2048 x 4096 x 128 375 us (917 TF/s of the five
@@ -31,9 +31,8 @@
 // Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and all roles drain.
 #include <cudaTypedefs.h>
 
-#include <atomic>
-
 #include "common.cuh"
+#include "dense.h"
 #include "internal.h"
 #include "softmax.cuh"
 
@@ -109,17 +108,6 @@ __device__ __forceinline__ float neg_lse_of(const DBwdParams& p, bool in, int64_
   return l == -INFINITY ? -INFINITY : -l;
 }
 
-__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
-}
-
 // Half of an accumulator's columns (this thread's D / 2 of one row) times
 // `scale`, as 16-bit values; `row`: the row's place, `keep`: whether it is
 // stored, `zero`: as zeros.  8 lanes write 128 bytes of a row at D = 128.
@@ -131,7 +119,7 @@ __device__ __forceinline__ void store_half_row(uint32_t base, int half, float sc
   for (int c = 0; c < D / 64; ++c) {
     uint32_t a[32];
     tmem_ld32(base + half * (D / 2) + c * 32, a);
-    tmem_wait32(a);
+    tmem_wait_ld32(a);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       uint4& v = x[c * 4 + g];
@@ -373,7 +361,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
         for (int c = 0; c < 2; ++c) {
           uint32_t sv[32];
           tmem_ld32(lane_base + s_col + c * 32, sv);
-          tmem_wait32(sv);
+          tmem_wait_ld32(sv);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const uint64_t x = f32x2_fma(f32x2_pack(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc2, nl2);
@@ -386,7 +374,7 @@ __device__ void dq_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CU
         for (int c = 0; c < 2; ++c) {
           uint32_t dp[32], ds[16];
           tmem_ld32(lane_base + kDP + half * 64 + c * 32, dp);
-          tmem_wait32(dp);
+          tmem_wait_ld32(dp);
           if (valid < 64) {
             // keys past the length: dS = 0, whatever their scores and values are
 #pragma unroll
@@ -637,7 +625,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
         for (int c = 0; c < 2; ++c) {
           uint32_t sv[32], pt[16];
           tmem_ld32(lane_base + half * 64 + c * 32, sv);
-          tmem_wait32(sv);
+          tmem_wait_ld32(sv);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const float2 nl = *reinterpret_cast<const float2*>(lb + c * 32 + k);
@@ -658,7 +646,7 @@ __device__ void dkdv_tile(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
         for (int c = 0; c < 2; ++c) {
           uint32_t dp[32], ds[16];
           tmem_ld32(lane_base + 128 + half * 64 + c * 32, dp);
-          tmem_wait32(dp);
+          tmem_wait_ld32(dp);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const float2 nd = *reinterpret_cast<const float2*>(db + c * 32 + k);
@@ -711,30 +699,14 @@ __global__ void __launch_bounds__(kThreadsB, 1)
     dq_tile<D, BF16>(tmQ, tmK, tmV, tmDO, p, smem, item - kv_items);
 }
 
-int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul, int rows = 128, int heads = 1) {
-  const bool one = B == 1 || t.stride_b == 0;
-  *mul = one ? 0 : 1;
-  if (one) t.stride_b = 8;
-  if (H == 1) t.stride_h = 8;
-  if (N == 1) t.stride_n = 8;
-  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, rows, heads);
-}
-
 template <int D, bool BF16>
 int launch_t(const bsa_cross_bwd_args* a, float* dout_max, cudaStream_t st) {
   using C = DBwdCfg<D>;
   auto kern = dense_bwd_kernel<D, BF16>;
-  static std::atomic<bool> ready[64] = {};
-  int dev = 0;
-  BSA_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return BSA_ERR_DEVICE;
-  if (!ready[dev].load(std::memory_order_acquire)) {
-    BSA_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    ready[dev].store(true, std::memory_order_release);
-  }
+  int r;
+  if ((r = opt_in_smem(reinterpret_cast<const void*>(kern), C::SMEM))) return r;
   DBwdParams p{};
   CUtensorMap mq, mk{}, mv{}, mdo;
-  int r;
   // The tile shape with the fewest query tiles (8 tokens of 8 heads in one tile
   // instead of eight): the tokens in equal parts, then heads that divide a group.
   const int G = a->H / a->Hk;
@@ -786,11 +758,6 @@ int launch_t(const bsa_cross_bwd_args* a, float* dout_max, cudaStream_t st) {
   cfg.numAttrs = 1;
   BSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, mdo, p));
   return BSA_OK;
-}
-
-bool aligned(const bsa_tensor4d& t, int B, int H, int N) {
-  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && (B == 1 || t.stride_b * 2 % 16 == 0) &&
-         (H == 1 || t.stride_h * 2 % 16 == 0) && (N == 1 || t.stride_n * 2 % 16 == 0);
 }
 
 }  // namespace

@@ -2,6 +2,7 @@
 // (attn_dense.cu, attn_few.cu, attn_dense_bwd.cu).
 #pragma once
 
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -43,6 +44,24 @@ struct FewParams {
   int32_t* err;
 };
 int launch_attn_few(const FewParams& p, int D, bool bf16, cudaStream_t st);
+
+// A tensor map's batch dimension of 1 where the batch shares one copy.
+inline int map_of(CUtensorMap* m, bsa_tensor4d t, int B, int H, int N, int D, bool bf16, int* mul, int rows = 128, int heads = 1,
+           int batch = 1) {
+  const bool one = B == 1 || t.stride_b == 0;
+  *mul = one ? 0 : 1;
+  // a dimension of length 1 has no stride of its own
+  if (one) t.stride_b = 8;
+  if (H == 1) t.stride_h = 8;
+  if (N == 1) t.stride_n = 8;
+  return make_tensor_map_4d(m, t, one ? 1 : B, H, N, D, bf16, rows, heads, batch);
+}
+
+// Rows that 16-byte accesses and tensor maps can take.
+inline bool aligned(const bsa_tensor4d& t, int B, int H, int N) {
+  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && (B == 1 || t.stride_b * 2 % 16 == 0) &&
+         (H == 1 || t.stride_h * 2 % 16 == 0) && (N == 1 || t.stride_n * 2 % 16 == 0);
+}
 
 // The dynamic shared memory opt-in of a kernel, once per device.
 inline int opt_in_smem(const void* kern, int bytes) {
