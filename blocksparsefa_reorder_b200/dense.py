@@ -81,7 +81,13 @@ def cross_attention_autograd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
                              k_lens: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None) -> torch.Tensor:
     """:func:`cross_attention` as a differentiable op (gradients of q, k, v);
     k and v expanded over the batch get the sum of its gradients.  The gradient
-    itself is not differentiable."""
+    itself is not differentiable.
+
+    The forward writes, beside the output, a second tensor of its size (what
+    rounding left of it) and the LSE, whether a gradient is recorded or not, and
+    the graph keeps them with q, k and v; the gradients of q, k and v are all
+    computed, whichever are asked for.  Where none is recorded,
+    :func:`cross_attention` does the same without."""
     return _lib.native().cross_attention_autograd(q, k, v, k_lens, sm_scale)
 
 
