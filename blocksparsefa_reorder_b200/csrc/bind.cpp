@@ -121,7 +121,7 @@ struct StridedSum {
   int n = 0;
   int64_t below, above;
   bool moved_only = false;  // not with every d_i zero
-  int budget = 1 << 16;     // (overlapping strides without end: taken as met)
+  int visits = 1 << 16;     // (more of them: taken as met)
   std::array<int64_t, 2 * Extent::kDims + 1> least, most;  // of the terms from i on
 
   void add(int64_t s, int64_t lo, int64_t hi) {
@@ -141,7 +141,7 @@ struct StridedSum {
   }
   bool from(int i, int64_t at, bool moved) {
     if (at + least[i] >= above || at + most[i] <= -below) return false;
-    if (--budget < 0) return true;
+    if (--visits < 0) return true;
     if (i == n) return moved || !moved_only;
     const Term& t = terms[i];
     if (t.s == 0) return from(i + 1, at, moved || t.hi > t.lo);
